@@ -12,7 +12,8 @@ Public surface (same names as the reference package ``kv_compression``):
   ``convert_model``                               manager (packed model weights, decoded just in time)
   ``main_lossless_comp``                          the runner (``python -m adacode_b200.main_lossless_comp``)
 and, without a reference counterpart, ``decode_attention`` (attention) — one decode step of
-attention computed from the packed planes.
+attention computed from the packed planes — ``append_rotary`` and ``paged_attention`` (paged) — new tokens rotated
+into a paged cache, and their attention over it — and ``sample_tokens`` (sampling) — the draw from the logits.
 """
 from .attention import decode_attention
 from .best_bit_analysis_kv_cache import export_initial_compress_parameters
@@ -22,10 +23,12 @@ from .float_cache_utils import Float11Cache, float11Layer
 from .mla_float_cache_utils import MLAFloat11Cache, MLALatentFloat11DenseRopeLayer
 from .manager import convert_model
 from .model_configs import model_config_map
+from .paged import append_rotary, paged_attention
+from .sampling import sample_tokens
 
 __all__ = [
     'Float11Cache', 'float11Layer', 'MLAFloat11Cache', 'MLALatentFloat11DenseRopeLayer',
     'TiledCompressedTensor', 'compress_tiled_tensor', 'materialize_tiled_state',
     'export_initial_compress_parameters', 'model_config_map', 'decode_attention', 'CompressorBitMap',
-    'convert_model',
+    'convert_model', 'append_rotary', 'paged_attention', 'sample_tokens',
 ]

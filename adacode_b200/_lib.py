@@ -22,6 +22,8 @@ STATUS_ESCAPE_OVERFLOW = 1
 STATUS_ESCAPE_UNDERRUN = 2
 STATUS_TIMEOUT = 4
 STATUS_MISALIGNED = 8
+STATUS_BAD_PAGE = 16
+BF16, FP16, FP32 = 0, 1, 2
 
 # every symbol include/adacode.h declares
 EXPORTED_SYMBOLS = (
@@ -31,6 +33,7 @@ EXPORTED_SYMBOLS = (
     'adacode_decode_attn_workspace_bytes', 'adacode_decode_attn', 'adacode_copy_to_host',
     'adacode_pack_jobs', 'adacode_pack_jobs_report', 'adacode_wait_report', 'adacode_unpack_jobs', 'adacode_unpack_jobs_with_rows', 'adacode_copy_rows', 'adacode_max_jobs', 'adacode_debug_set_wait_limit',
     'adacode_flat_block_elems', 'adacode_pack_flat', 'adacode_unpack_flat', 'adacode_unpack_flat_ragged',
+    'adacode_append_rotary', 'adacode_paged_attn_workspace_bytes', 'adacode_paged_attn', 'adacode_sample_tokens',
 )
 
 
@@ -70,6 +73,27 @@ class RowCopy(ctypes.Structure):
         ('src_b', ctypes.c_int64), ('src_h', ctypes.c_int64), ('src_s', ctypes.c_int64),
         ('dst_b', ctypes.c_int64), ('dst_h', ctypes.c_int64), ('dst_s', ctypes.c_int64),
         ('B', ctypes.c_int32), ('H', ctypes.c_int32), ('rows', ctypes.c_int32), ('D', ctypes.c_int32),
+    ]
+
+
+class PagedCache(ctypes.Structure):
+    """``struct adacode_paged_cache``."""
+    _fields_ = [
+        ('key_pages', ctypes.c_void_p), ('value_pages', ctypes.c_void_p),
+        ('key_page', ctypes.c_int64), ('key_head', ctypes.c_int64), ('key_slot', ctypes.c_int64),
+        ('value_page', ctypes.c_int64), ('value_head', ctypes.c_int64), ('value_slot', ctypes.c_int64),
+        ('block_table', ctypes.c_void_p), ('table_stride', ctypes.c_int64), ('seq_lens', ctypes.c_void_p), ('cu_seqlens', ctypes.c_void_p),
+        ('table_width', ctypes.c_int32), ('B', ctypes.c_int32), ('n_pages', ctypes.c_int32), ('page_size', ctypes.c_int32),
+        ('Hkv', ctypes.c_int32), ('D', ctypes.c_int32), ('dtype', ctypes.c_int32), ('N', ctypes.c_int32),
+    ]
+
+
+class Rotary(ctypes.Structure):
+    """``struct adacode_rotary``."""
+    _fields_ = [
+        ('cos', ctypes.c_void_p), ('sin', ctypes.c_void_p), ('axis_stride', ctypes.c_int64), ('token_stride', ctypes.c_int64),
+        ('axes', ctypes.c_int32), ('section', ctypes.c_int32 * 4), ('half', ctypes.c_int32), ('interleaved', ctypes.c_int32),
+        ('dtype', ctypes.c_int32),
     ]
 
 
@@ -148,6 +172,14 @@ def lib() -> ctypes.CDLL:
     L.adacode_unpack_jobs_with_rows.argtypes = [vp, i32, i32, i32, i32, i32, vp, i32, vp, vp]
     L.adacode_copy_rows.restype = i32
     L.adacode_copy_rows.argtypes = [vp, i32, vp]
+    L.adacode_append_rotary.restype = i32
+    L.adacode_append_rotary.argtypes = [vp, vp, vp, i64, i64, i32, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, vp]
+    L.adacode_paged_attn_workspace_bytes.restype = sz
+    L.adacode_paged_attn_workspace_bytes.argtypes = [i32]
+    L.adacode_paged_attn.restype = i32
+    L.adacode_paged_attn.argtypes = [vp, vp, i64, i64, i32, vp, i64, i64, vp, i32, ctypes.c_float, i32, i32, vp, sz, vp, vp]
+    L.adacode_sample_tokens.restype = i32
+    L.adacode_sample_tokens.argtypes = [vp, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp]
     _lib = L
     return L
 

@@ -144,6 +144,7 @@ _STATUS_TEXT = (
     (_lib.STATUS_ESCAPE_UNDERRUN, 'escape list shorter than the code plane requires during unpack'),
     (_lib.STATUS_TIMEOUT, 'a bounded on-chip wait gave up (results of that launch are invalid)'),
     (_lib.STATUS_MISALIGNED, 'a plane pointer in a segment record is not 16-byte aligned (tile skipped)'),
+    (_lib.STATUS_BAD_PAGE, 'a position has no page of the pool (it was left out)'),
 )
 
 

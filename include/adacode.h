@@ -44,6 +44,12 @@ extern "C" {
 #define ADACODE_STATUS_ESCAPE_UNDERRUN 2 /* unpack: a tile wanted an escape beyond n_escapes */
 #define ADACODE_STATUS_TIMEOUT 4         /* a bounded on-chip wait gave up; results are invalid */
 #define ADACODE_STATUS_MISALIGNED 8      /* a plane pointer inside a segment record is not 16-byte aligned */
+#define ADACODE_STATUS_BAD_PAGE 16       /* a position has no page: its table entry is none of the pool's, or it lies behind the table */
+
+/* element types of the operators below that take more than bf16 */
+#define ADACODE_BF16 0
+#define ADACODE_FP16 1
+#define ADACODE_FP32 2
 
 /* Library version, major*10000 + minor*100 + patch. */
 int adacode_version(void);
@@ -383,6 +389,79 @@ int adacode_decode_attn(const void *q_bf16, int64_t q_stride_b, int64_t q_stride
                         int64_t tail_stride_h, int64_t tail_stride_s, int B, int Hq, int Hkv, int seq_tile, int D,
                         float scale, void *out_bf16, void *workspace, size_t workspace_bytes, int n_splits,
                         int32_t *status, void *stream);
+
+/*
+ * Keys and values of B sequences in pages of page_size tokens each, as the two operators below see them: position p of
+ * sequence b is slot p % page_size of page block_table[b][p / page_size].  Element strides, unit stride along D; pages,
+ * heads and slots may lie in any order.  seq_lens counts the tokens of a sequence WITH the new ones of the call, which are its
+ * last.  All pointers but this struct's own are device memory and nothing of them is read by the host, so that a call can be
+ * captured into a graph and replayed with other lengths, tables and contents.
+ * A table entry that is none of 0 .. n_pages - 1, or a position behind the table, is never followed: ADACODE_STATUS_BAD_PAGE.
+ */
+typedef struct adacode_paged_cache {
+    void *key_pages, *value_pages;           /* [n_pages][Hkv][page_size][D] */
+    int64_t key_page, key_head, key_slot;    /* strides */
+    int64_t value_page, value_head, value_slot;
+    const int32_t *block_table;              /* [B][table_width], rows table_stride entries apart */
+    int64_t table_stride;
+    const int32_t *seq_lens;                 /* [B] */
+    const int32_t *cu_seqlens;               /* [B + 1]: new token i is of the sequence b with cu[b] <= i < cu[b + 1]; NULL: N / B each */
+    int32_t table_width, B, n_pages, page_size, Hkv, D, dtype; /* ADACODE_BF16 or ADACODE_FP16 */
+    int32_t N;                               /* new tokens that the call's tensors have room for; those from cu[B] on are left alone */
+} adacode_paged_cache;
+
+/* Rotary positions of adacode_append_rotary: the cosine and sine of half angles per token, for 1 to 4 axes.  Frequency f
+ * is taken from the axis that its section belongs to: the first section[0] from axis 0, the next section[1] from axis 1, ... */
+typedef struct adacode_rotary {
+    const void *cos, *sin;                   /* [axes][N][half], element strides below, unit stride along half */
+    int64_t axis_stride, token_stride;
+    int32_t axes, section[4];                /* sections sum up to half */
+    int32_t half;                            /* the first 2 half columns of a head are rotated, 2 half <= D */
+    int32_t interleaved;                     /* pairs of columns: (2 f, 2 f + 1) if set, (f, f + half) if not */
+    int32_t dtype;                           /* of cos and sin */
+} adacode_rotary;
+
+/*
+ * New tokens on their way into a paged cache: every pair (x, y) of columns of a query's or key's head becomes
+ * (x cos - y sin, y cos + x sin), in 32 bits and rounded once; rotated keys and the values are written to their pages, rotated queries
+ * to query_out (which may be `query`).  query may be NULL (Hq = 0).  query, key, value [N][heads][D] with element strides, unit
+ * stride along D.
+ * (A model's apply_rotary_pos_emb and the cache's update, float_cache_utils.py:860-881, one torch operation after the other.)
+ */
+int adacode_append_rotary(const adacode_paged_cache *cache, const adacode_rotary *rotary, const void *query, int64_t query_token,
+                          int64_t query_head, int Hq, void *query_out, int64_t out_token, int64_t out_head, const void *key,
+                          int64_t key_token, int64_t key_head, const void *value, int64_t value_token, int64_t value_head,
+                          int32_t *status, void *stream);
+
+/*
+ * Attention of new tokens over the pages of their sequences, themselves included (they have been appended):
+ *   out[i][h] = softmax over j of (scale * query[i][h] . K[j][h / G]) times V[j][h / G],   G = Hq / Hkv,
+ * for the new token at position p over the cached positions j with seq_starts[b] <= j < seq_lens[b], j <= p if `causal`, and
+ * j > p - window if window > 0.  A token that sees nothing, and one all of whose scores are minus infinity, gets 0.  What a hidden position
+ * holds has no influence, infinities and NaN included; a NaN score that is seen makes its row NaN; an infinite or NaN value that is seen
+ * gives its column what it has in 32-bit arithmetic.  Products of 16-bit values are summed up in 32 bits, the weights enter the
+ * second product in the type of the pages, their sum in 32 bits.
+ * max_query_len: the most new tokens of one sequence (an upper bound; it chooses the kernel).  D 64 or 128; pages of 16, 32, 64 or a
+ * multiple of 128 tokens, or one page per sequence (table_width 1) of any size; pointers on 16-byte boundaries, strides
+ * multiples of 8.  The workspace is adacode_paged_attn_workspace_bytes() for calls of any shape; calls that share one must be
+ * ordered on one stream.  seq_starts may be NULL.
+ */
+size_t adacode_paged_attn_workspace_bytes(int D);
+int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int64_t query_token, int64_t query_head, int Hq,
+                       void *out, int64_t out_token, int64_t out_head, const int32_t *seq_starts, int max_query_len, float scale, int causal,
+                       int window, void *workspace, size_t workspace_bytes, int32_t *status, void *stream);
+
+/*
+ * One token per row of logits [B][V] (rows row_stride elements apart) from one uniform number in [0, 1) each.  In the order of
+ * descending logit, lower token first among equals: the first top_k stay (<= 0: all); of those, each whose predecessors' softmax
+ * weights at the row's temperature add up to less than top_p of all (>= 1: all; the first always stays); of those, each whose weight is
+ * at least min_p times the largest.  The token drawn is the first, in the order of the vocabulary, at which the running sum of what stays exceeds
+ * uniform times its total.  temperature <= 0: the first token of the largest logit.  Minus infinity and NaN are never drawn, plus infinity counts as
+ * the largest finite number; a row without a token to draw gives -1.  Weights and sums are of 64 bits.
+ * temperature, top_p, min_p (fp32) and top_k (int32) are device arrays of B entries; each but temperature may be NULL (off).
+ */
+int adacode_sample_tokens(const void *logits, int64_t row_stride, int dtype, int B, int V, const float *uniforms, const float *temperature,
+                          const int32_t *top_k, const float *top_p, const float *min_p, int64_t *tokens, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,122 @@
+"""The sampler against one row after the other in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from tests import serving_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+TYPES = {'bf16': torch.bfloat16, 'fp16': torch.float16, 'fp32': torch.float32}
+
+
+def check(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, **more):
+    """Every row equal, but for rows whose draw lies within 1e-10 of the border of another outcome (64-bit sums of up to 2**18 weights:
+    2**18 x 2**-53 = 3e-11 at worst)."""
+    from adacode_b200 import sample_tokens
+    got = sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p, **more).tolist()
+    f = lambda x, b: x[b].item() if isinstance(x, torch.Tensor) else float(torch.tensor(x, dtype=torch.float32))   # noqa: E731
+    for b in range(logits.shape[0]):
+        want, near = oracle.sample(logits[b].cpu(), f(uniforms, b), f(temperature, b), int(f(top_k, b)), f(top_p, b), f(min_p, b))
+        assert got[b] == want or near < 1e-10, (b, got[b], want, near)
+    return got
+
+
+SETTINGS = [dict(), dict(temperature=0.0), dict(temperature=0.3), dict(top_k=1), dict(top_k=7), dict(top_k=50, top_p=0.9), dict(top_p=0.5),
+            dict(top_p=0.0), dict(top_p=0.95, min_p=0.01, temperature=1.7), dict(min_p=0.2), dict(min_p=1.0), dict(top_k=100000, top_p=0.999),
+            dict(top_k=900, temperature=3.0), dict(top_k=3000, top_p=0.7, temperature=5.0)]
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16', 'fp32'])
+@pytest.mark.parametrize('V', [1, 2, 31, 257, 5000, 32000, 151936])
+def test_sampling(V, dtype):
+    g = torch.Generator('cpu').manual_seed(V)
+    B = 7 if V < 10000 else 3
+    for n, s in enumerate(SETTINGS):
+        logits = (torch.randn((B, V), generator=g) * 2.5).to(TYPES[dtype]).cuda()
+        check(logits, torch.rand(B, generator=g).cuda(), **s)
+
+
+def test_settings_per_row():
+    g = torch.Generator('cpu').manual_seed(3)
+    B, V = 64, 3001
+    logits = (torch.randn((B, V), generator=g) * 3).cuda()
+    check(logits, torch.rand(B, generator=g).cuda(), temperature=torch.tensor([0.0, 0.5, 1.0, 2.0] * 16, device='cuda'),
+          top_k=torch.tensor([0, 5, 40, 4000, -1, 1, 3001, 77] * 8, dtype=torch.int32, device='cuda'),
+          top_p=torch.tensor([1.0, 0.9, 0.3, 0.0, 1.5, 0.99, 0.5, 0.8] * 8, device='cuda').roll(3),
+          min_p=torch.tensor([0.0, 0.1, 0.0, 0.01] * 16, device='cuda').roll(1))
+
+
+@pytest.mark.parametrize('s', [dict(top_k=3), dict(top_k=40), dict(top_p=0.5), dict(top_p=0.31, top_k=60), dict(min_p=0.9), dict()],
+                         ids=lambda s: '-'.join(f'{k}{v}' for k, v in s.items()))
+@pytest.mark.parametrize('V', [64, 1000, 40000])
+def test_ties(V, s):
+    """Rows of few different values: the lower tokens of a value stay."""
+    g = torch.Generator('cpu').manual_seed(V)
+    for values in (1, 2, 5):
+        logits = torch.randint(0, values, (4, V), generator=g).float().cuda()
+        u = torch.tensor([0.0, 0.25, 0.6, 1 - 2.0 ** -24], device='cuda')
+        check(logits, u, **s)
+        check((logits * 0.5 - 0.5).bfloat16(), u, **s)                              # minus zero and zero are one value
+    signed = torch.zeros((1, V), device='cuda')
+    signed[0, ::2] = -0.0
+    assert check(signed, torch.zeros(1, device='cuda'), **s) == [0]
+
+
+def test_forbidden_tokens_and_empty_rows():
+    V = 1000
+    logits = torch.randn((6, V), generator=torch.Generator('cpu').manual_seed(1)).cuda()
+    logits[0] = -math.inf
+    logits[1] = math.nan
+    logits[2, :900] = -math.inf
+    logits[3, 3:] = math.nan
+    logits[4, 17], logits[4, 400] = math.inf, math.inf
+    logits[5, 1:] = -math.inf
+    for s in (dict(), dict(top_k=300), dict(top_p=0.99), dict(top_k=2000, top_p=0.9), dict(min_p=0.001), dict(temperature=0.0)):
+        for u in (0.0, 0.3, 0.7, 1 - 2.0 ** -24):
+            got = check(logits, torch.full((6,), u, device='cuda'), **s)
+            assert got[0] == got[1] == -1 and got[2] >= 900 and 0 <= got[3] < 3 and got[4] in (17, 400) and got[5] == 0
+
+
+def test_distribution():
+    """Even steps of the uniform number give every token its share, to within one step."""
+    from adacode_b200 import sample_tokens
+    n = 4096
+    row = torch.tensor([0.3, -1.0, 2.0, 0.0, 1.0, -3.0, 0.5], device='cuda')
+    u = (torch.arange(n, device='cuda') + 0.5) / n
+    got = torch.bincount(sample_tokens(row.expand(n, 7), u, temperature=0.8), minlength=7).double().cpu() / n
+    assert bool(((got - torch.softmax(row.double().cpu() / 0.8, 0)).abs() <= 1.0 / n).all())
+
+
+def test_strides_out_streams_and_graphs():
+    from adacode_b200 import sample_tokens
+    g = torch.Generator('cpu').manual_seed(9)
+    wide = torch.randn((5, 3, 777), generator=g).cuda()
+    u = torch.rand(5, generator=g).cuda()
+    check(wide[:, 1], u, top_k=20)                                                   # rows of a larger tensor
+    check(wide[:, :, 5].t().contiguous().t(), u)                                     # no unit stride
+    check(wide[:, 1, 3:], u, top_p=0.9)                                              # rows off every boundary
+    check(wide[:, 1].bfloat16()[:, 1:], u, top_p=0.9)
+    out = torch.zeros(5, dtype=torch.int64, device='cuda')
+    want = check(wide[:, 1], u, top_k=20, out=out)
+    assert out.tolist() == want
+    logits, side = wide[:, 1].contiguous(), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    k = torch.full((5,), 20, dtype=torch.int32, device='cuda')
+    t = torch.ones(5, device='cuda')
+    with torch.cuda.graph(graph):
+        sample_tokens(logits, u, t, k, out=out)
+    logits.copy_(wide[:, 2])
+    u.copy_(torch.rand(5, generator=g))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        graph.replay()
+    side.synchronize()
+    assert out.tolist() == check(wide[:, 2], u, t, k)
+    assert sample_tokens(logits[:0], u[:0]).shape == (0,)
+
+
+def test_many_rows():
+    g = torch.Generator('cpu').manual_seed(11)
+    logits = (torch.randn((600, 513), generator=g) * 2).bfloat16().cuda()
+    check(logits, torch.rand(600, generator=g).cuda(), top_k=40, top_p=0.9)
