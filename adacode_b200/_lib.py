@@ -175,7 +175,7 @@ def lib() -> ctypes.CDLL:
     L.adacode_append_rotary.restype = i32
     L.adacode_append_rotary.argtypes = [vp, vp, vp, i64, i64, i32, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, vp]
     L.adacode_paged_attn_workspace_bytes.restype = sz
-    L.adacode_paged_attn_workspace_bytes.argtypes = [i32]
+    L.adacode_paged_attn_workspace_bytes.argtypes = [i32, i32, i32, i32]
     L.adacode_paged_attn.restype = i32
     L.adacode_paged_attn.argtypes = [vp, vp, i64, i64, i32, vp, i64, i64, vp, i32, ctypes.c_float, i32, i32, vp, sz, vp, vp]
     L.adacode_sample_tokens.restype = i32

@@ -1,4 +1,4 @@
-// New tokens of a serving step and their paged cache: rotation and append, attention over the pages.
+// New tokens of a serving step on their way into a paged cache: rotation and append.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -10,45 +10,7 @@ namespace {
 
 constexpr unsigned kFull = 0xFFFFFFFFu;
 
-__device__ __forceinline__ float widen(float v) { return v; }
-__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
-__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T narrow(float v);
-template <>
-__device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
-
-// Sequence of new token i (B if it is behind the last), found by the whole warp, and the tokens of the call up to its end.
-__device__ __forceinline__ int sequence_of(const adacode_paged_cache &c, int i, int &end) {
-    if (!c.cu_seqlens) {
-        const int each = c.N / c.B, b = i / each;
-        end = (b + 1) * each;
-        return b;
-    }
-    const int lane = threadIdx.x & 31;
-    int b = 0;
-    for (int k = 0; k < c.B; k += 32) {
-        const int e = k + lane < c.B ? c.cu_seqlens[k + lane + 1] : INT32_MAX;
-        const unsigned before = __ballot_sync(kFull, e <= i);
-        b += __popc(before);
-        if (before != kFull) {
-            end = __shfl_sync(kFull, e, __popc(before));
-            break;
-        }
-    }
-    return b;
-}
-
-// The page of position `at` of sequence b, or -1.
-__device__ __forceinline__ int page_of(const adacode_paged_cache &c, int b, int at, int &slot) {
-    const int n = at / c.page_size;
-    slot = at - n * c.page_size;
-    if (at < 0 || n >= c.table_width) return -1;
-    const int page = c.block_table[b * c.table_stride + n];
-    return page >= 0 && page < c.n_pages ? page : -1;
-}
+#include "adacode_pages.cuh"
 
 // ---------------------------------------------------------------------------------------
 // rotation and append
@@ -161,92 +123,6 @@ void launch_append(const AppendArgs &a, bool wide, cudaStream_t st) {
     else launch_append<T, T>(a, wide, st);
 }
 
-bool valid(const adacode_paged_cache *c) {
-    return c && c->key_pages && c->value_pages && c->block_table && c->seq_lens && c->B > 0 && c->n_pages > 0 && c->page_size > 0 &&
-           c->table_width > 0 && c->Hkv > 0 && c->N >= 0 && (c->dtype == ADACODE_BF16 || c->dtype == ADACODE_FP16) &&
-           (c->cu_seqlens || c->N % c->B == 0);
-}
-
-// ---------------------------------------------------------------------------------------
-// attention over pages
-// ---------------------------------------------------------------------------------------
-
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct PagedArgs {
-    adacode_paged_cache cache;
-    const void *query;
-    void *out;
-    long long q_n, q_h, o_n, o_h;
-    const int32_t *starts;
-    int Hq, G, causal, window;
-    float scale;              // times log2 e
-    int32_t *status;
-};
-
-// One warp per token and head, one cached token after the other.  A value whose weight is 0 has no influence.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) k_paged_rows(const __grid_constant__ PagedArgs a) {
-    constexpr int E = D / 32;
-    const adacode_paged_cache &c = a.cache;
-    const int lane = threadIdx.x & 31;
-    const long long w = blockIdx.x * 4ll + threadIdx.x / 32;
-    const int i = (int)(w / a.Hq), h = (int)(w - (long long)i * a.Hq);
-    if (i >= c.N) return;
-    int end = 0;
-    const int b = sequence_of(c, i, end);
-    if (b >= c.B) return;
-    const int len = c.seq_lens[b], at = len - end + i;
-    int lo = a.starts ? a.starts[b] : 0, hi = a.causal && at + 1 < len ? at + 1 : len;
-    if (a.window > 0 && lo < at - a.window + 1) lo = at - a.window + 1;
-    if (lo < 0) lo = 0;
-    const T *q = reinterpret_cast<const T *>(a.query) + i * a.q_n + h * a.q_h + lane * E;
-    float x[E], acc[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = widen(q[e]) * a.scale, acc[e] = 0.f;
-    // twice over the tokens: the weights' sum first, so that values are added up with weights below 1 and large ones do not overflow
-#pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {
-        const float base = m == -INFINITY ? 0.f : m, share = pass ? 1.f / l : 0.f;
-        for (int j = lo; j < hi; ++j) {
-            int slot;
-            const int page = page_of(c, b, j, slot);
-            if (page < 0) {
-                if (lane == 0) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
-                continue;
-            }
-            const T *k = reinterpret_cast<const T *>(c.key_pages) + page * c.key_page + (h / a.G) * c.key_head + slot * c.key_slot + lane * E;
-            float s = 0.f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) s = fmaf(x[e], widen(k[e]), s);
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(kFull, s, d);
-            if (pass == 0) {
-                const float top = fmaxf(m, s), from = top == -INFINITY ? 0.f : top;
-                l = l * exp2f(m - from) + exp2f(s - from);
-                m = top;
-                continue;
-            }
-            const float p = exp2f(s - base) * share;
-            if (p == 0.f) continue;
-            const T *v = reinterpret_cast<const T *>(c.value_pages) + page * c.value_page + (h / a.G) * c.value_head + slot * c.value_slot + lane * E;
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(p, widen(v[e]), acc[e]);
-        }
-        if (l == 0.f) break;
-    }
-    T *out = reinterpret_cast<T *>(a.out) + i * a.o_n + h * a.o_h + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) out[e] = narrow<T>(l == 0.f ? 0.f : acc[e]);
-}
-
-template <typename T>
-void launch_paged(const PagedArgs &a, cudaStream_t st) {
-    const unsigned grid = (unsigned)(((long long)a.cache.N * a.Hq + 3) / 4);
-    if (a.cache.D == 128) k_paged_rows<T, 128><<<grid, 128, 0, st>>>(a);
-    else k_paged_rows<T, 64><<<grid, 128, 0, st>>>(a);
-}
-
 }  // namespace
 
 extern "C" {
@@ -278,27 +154,6 @@ int adacode_append_rotary(const adacode_paged_cache *cache, const adacode_rotary
     const bool wide = (pointers & 15) == 0 && (strides & 7) == 0 && cache->D % 16 == 0 && r.half % 8 == 0;
     if (cache->dtype == ADACODE_BF16) launch_append<__nv_bfloat16>(a, wide, (cudaStream_t)stream);
     else launch_append<__half>(a, wide, (cudaStream_t)stream);
-    return cudaGetLastError() == cudaSuccess ? ADACODE_OK : ADACODE_ERR_CUDA;
-}
-
-size_t adacode_paged_attn_workspace_bytes(int D) { return D > 0 ? 16 : 0; }
-
-int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int64_t query_token, int64_t query_head, int Hq,
-                       void *out, int64_t out_token, int64_t out_head, const int32_t *seq_starts, int max_query_len, float scale, int causal,
-                       int window, void *workspace, size_t workspace_bytes, int32_t *status, void *stream) {
-    if (!valid(cache) || !status || Hq <= 0 || Hq % cache->Hkv != 0 || window < 0 || max_query_len < 0) return ADACODE_ERR_INVALID_ARG;
-    if (cache->D != 64 && cache->D != 128) return ADACODE_ERR_INVALID_ARG;
-    if (cache->table_width > 1 && cache->page_size % 128 != 0 && cache->page_size != 16 && cache->page_size != 32 && cache->page_size != 64)
-        return ADACODE_ERR_INVALID_ARG;
-    if (cache->N == 0) return ADACODE_OK;
-    if (!query || !out) return ADACODE_ERR_INVALID_ARG;
-    const uintptr_t pointers = (uintptr_t)query | (uintptr_t)out | (uintptr_t)cache->key_pages | (uintptr_t)cache->value_pages;
-    const int64_t strides = query_token | query_head | out_token | out_head | cache->key_page | cache->key_head | cache->key_slot |
-                            cache->value_page | cache->value_head | cache->value_slot;
-    if ((pointers & 15) != 0 || (strides & 7) != 0) return ADACODE_ERR_INVALID_ARG;
-    const PagedArgs a{*cache, query, out, query_token, query_head, out_token, out_head, seq_starts, Hq, Hq / cache->Hkv, causal, window, scale * kLog2e, status};
-    if (cache->dtype == ADACODE_BF16) launch_paged<__nv_bfloat16>(a, (cudaStream_t)stream);
-    else launch_paged<__half>(a, (cudaStream_t)stream);
     return cudaGetLastError() == cudaSuccess ? ADACODE_OK : ADACODE_ERR_CUDA;
 }
 

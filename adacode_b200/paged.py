@@ -10,7 +10,8 @@ A page of 128 tokens is what ``compress_tiled_tensor`` packs, and a dense cache 
 after the other along the first dimension; ``cu_seqlens`` int32 ``[B + 1]`` says where each sequence begins (without it all have equally
 many), and tokens from ``cu_seqlens[B]`` on are padding, which is left alone.  Tables and lengths stay on the device: a call
 never waits for them, and a captured call may be replayed with others.  What only they can show to be wrong, a position without a page
-of the pool, is never followed: it is left out and reported in the device's status word (``codec.check_device_status``).
+of the pool, is never followed: nothing is written there, zeros are read, and the device's
+status word says so (``codec.check_device_status``).
 
 The reference has neither: its caches concatenate (float_cache_utils.py:860-881) what the model has rotated with torch
 operations, and rebuild dense keys and values for the model's own attention (:1342).
@@ -201,7 +202,7 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
         scale = D ** -0.5
     with on_device(dev):
         stream = stream_ptr(dev)
-        need = int(_lib.lib().adacode_paged_attn_workspace_bytes(D))
+        need = int(_lib.lib().adacode_paged_attn_workspace_bytes(max_query_len, Hq, cache.Hkv, D))
         # (a captured graph runs on other streams than the one that it is captured on: it has memory of its own)
         ws = (torch.empty(need, dtype=torch.uint8, device=dev) if torch.cuda.is_current_stream_capturing()
               else sc.partials.get(stream, need))

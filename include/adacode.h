@@ -396,7 +396,8 @@ int adacode_decode_attn(const void *q_bf16, int64_t q_stride_b, int64_t q_stride
  * heads and slots may lie in any order.  seq_lens counts the tokens of a sequence WITH the new ones of the call, which are its
  * last.  All pointers but this struct's own are device memory and nothing of them is read by the host, so that a call can be
  * captured into a graph and replayed with other lengths, tables and contents.
- * A table entry that is none of 0 .. n_pages - 1, or a position behind the table, is never followed: ADACODE_STATUS_BAD_PAGE.
+ * A table entry that is none of 0 .. n_pages - 1, or a position behind the table, is never followed (nothing is written there,
+ * and zeros are read): ADACODE_STATUS_BAD_PAGE.
  */
 typedef struct adacode_paged_cache {
     void *key_pages, *value_pages;           /* [n_pages][Hkv][page_size][D] */
@@ -443,10 +444,10 @@ int adacode_append_rotary(const adacode_paged_cache *cache, const adacode_rotary
  * second product in the type of the pages, their sum in 32 bits.
  * max_query_len: the most new tokens of one sequence (an upper bound; it chooses the kernel).  D 64 or 128; pages of 16, 32, 64 or a
  * multiple of 128 tokens, or one page per sequence (table_width 1) of any size; pointers on 16-byte boundaries, strides
- * multiples of 8.  The workspace is adacode_paged_attn_workspace_bytes() for calls of any shape; calls that share one must be
- * ordered on one stream.  seq_starts may be NULL.
+ * multiples of 8.  The workspace (on a 16-byte boundary) has adacode_paged_attn_workspace_bytes() for the current device; calls that
+ * share one must be ordered on one stream.  seq_starts may be NULL.
  */
-size_t adacode_paged_attn_workspace_bytes(int D);
+size_t adacode_paged_attn_workspace_bytes(int max_query_len, int Hq, int Hkv, int D);
 int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int64_t query_token, int64_t query_head, int Hq,
                        void *out, int64_t out_token, int64_t out_head, const int32_t *seq_starts, int max_query_len, float scale, int causal,
                        int window, void *workspace, size_t workspace_bytes, int32_t *status, void *stream);
