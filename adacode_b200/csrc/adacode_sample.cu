@@ -1,7 +1,18 @@
 // One token per row of logits: temperature, top-k, top-p, min-p and the draw from a given uniform number.
 //
-// Logits become 32-bit keys whose order is the logits' order.  Every cut (the top_k first, the nucleus) is a prefix of the
-// order (descending logit, ascending token) and is kept as a key and the number of that key's tokens that are inside.
+// Every cut (the top_k first, the nucleus, min_p) keeps a prefix of the order (descending logit, ascending token); tokens are kept
+// as 64-bit keys of that order.  A row has a cluster of 1 to 8 CTAs, whose warps own consecutive spans of the vocabulary.  Passes over the row, which
+// after the first come from L2:
+//   1  the largest logit.
+//   top_k up to kMostK: the tokens above a border that a sample of the row says is low enough are listed (their number is checked); the
+//      list is sorted, and all else happens in it.  No weight of any other token is computed.
+//   top_p alone: 2 adds up the weights, all of them in 64 bits and per interval of the logit (2048 intervals) in about 24, which tells the
+//      interval in which the nucleus ends; 3 adds up, per span, what lies above the interval in 64 bits and lists what lies in it.
+//      The sums of 3 say exactly whether the interval was right (if not, its neighbour is next); the sorted list says where the nucleus ends.
+//   neither: 3 alone.
+//   Then the span in which the draw falls is walked again.
+// What fits no list (thousands of equal logits at a border, a larger top_k) goes the slow way: bisection of the keys by one CTA.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -10,73 +21,174 @@
 
 #include "adacode.h"
 
+namespace cg = cooperative_groups;
+
 namespace {
 
 constexpr unsigned kFull = 0xFFFFFFFFu;
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMostCtas = 8;             // per row
+constexpr int kStep = 256;               // tokens that a warp takes at a time, eight per lane
+constexpr int kBins = 2048;
+constexpr int kSample = 4096;            // tokens that the sample has
+constexpr int kList = 4096;
+constexpr int kMostK = 1024;
 
 struct SampleArgs {
     const void *logits;
     long long row_stride;
     int V;
+    bool wide;                           // rows on 16-byte boundaries
     const float *uniforms, *temperature, *top_p, *min_p;
     const int32_t *top_k;
     int64_t *tokens;
 };
 
-template <typename T>
-__device__ __forceinline__ float widen(T v);
-template <>
 __device__ __forceinline__ float widen(float v) { return v; }
-template <>
 __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
-template <>
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+// plus infinity counts as the largest number; NaN stays
+__device__ __forceinline__ float clean(float v) { return v > FLT_MAX ? FLT_MAX : v; }
 
-// NaN and minus infinity have key 0 (never drawn), plus infinity that of the largest finite number, both zeros one key.
-__device__ __forceinline__ uint32_t key_of(float x) {
-    if (!(x > -INFINITY)) return 0;
-    x = fminf(x, FLT_MAX) + 0.f;
-    const uint32_t u = __float_as_uint(x);
+// NaN and minus infinity have key 0 (never drawn), both zeros one key.
+__device__ __forceinline__ uint32_t key_of(float v) {
+    if (!(v > -INFINITY)) return 0;
+    const uint32_t u = __float_as_uint(v + 0.f);
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key); }
+// the order: descending logit, ascending token
+__device__ __forceinline__ uint64_t place_of(float v, int token) { return (uint64_t)key_of(v) << 32 | (0xFFFFFFFFu - (uint32_t)token); }
+__device__ __forceinline__ int token_of(uint64_t place) { return (int)(0xFFFFFFFFu - (uint32_t)place); }
+
+struct Shared {
+    double roots[32];                    // 2**(j / 32)
+    union {
+        float weight[kBins];
+        uint32_t count[kBins];
+    } bin;
+    uint64_t list[kList];
+    double line[kMostK];
+    double span_all[kMostCtas * kWarps], span_kept[kMostCtas * kWarps];
+    double scan[kWarps + 1];
+    uint64_t best[kWarps];
+    uint64_t cta_best;
+    double cta_sum;
+    float low[kWarps];
+    int scan_n[kWarps];
+    int listed, found, decided;
+    uint64_t border;
+};
+
+// exp(x / T) = 2**(x k): x k rounded to 1/32, the rest's power by its Taylor series (degree 4, |rest ln 2| <= ln 2 / 64: the next
+// term is below 1.3e-12), 32 roots of 2.  Half the time of exp() (64-bit), whose last bits no draw needs.
+__device__ __forceinline__ double weight_of(float v, double largest, double k, const double *roots) {
+    const double t = ((double)v - largest) * k;
+    if (!(t > -1000.0)) return 0.0;
+    constexpr double kShift = 6755399441055744.0 / 32.0;       // 1.5 x 2**52 / 32
+    const double shifted = t + kShift;
+    const int n = __double2loint(shifted);
+    const double r = (t - (shifted - kShift)) * 0.69314718055994530942;
+    const double power = fma(fma(fma(fma(r, 1.0 / 24.0, 1.0 / 6.0), r, 0.5), r, 1.0), r, 1.0) * roots[n & 31];
+    return __hiloint2double(__double2hiint(power) + ((n >> 5) << 20), __double2loint(power));
+}
 
 template <typename R, typename Op>
-__device__ R block_reduce(R v, Op op, R *shared) {
+__device__ __forceinline__ R warp_reduce(R v, Op op) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v = op(v, __shfl_xor_sync(kFull, v, d));
+    return v;
+}
+template <typename R, typename Op>
+__device__ R block_reduce(R v, Op op, R *shared) {
+    v = warp_reduce(v, op);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
     __syncthreads();
     R r = shared[0];
-    for (int w = 1; w < kThreads / 32; ++w) r = op(r, shared[w]);
+    for (int w = 1; w < kWarps; ++w) r = op(r, shared[w]);
     return r;
 }
+struct Plus {
+    template <typename R>
+    __device__ __forceinline__ R operator()(R p, R q) const { return p + q; }
+};
+struct Most {
+    template <typename R>
+    __device__ __forceinline__ R operator()(R p, R q) const { return p > q ? p : q; }
+};
+struct Least {
+    template <typename R>
+    __device__ __forceinline__ R operator()(R p, R q) const { return p < q ? p : q; }
+};
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
-    __shared__ double s_d[32];
-    __shared__ unsigned long long s_u[32];
-    __shared__ double s_line[kThreads];
-    __shared__ int s_ties[kThreads];
-    const int row = blockIdx.x, tid = threadIdx.x, V = a.V;
-    const T *x = reinterpret_cast<const T *>(a.logits) + row * a.row_stride;
-    const auto plus = [](auto p, auto q) { return p + q; };
-    const auto most = [](auto p, auto q) { return p > q ? p : q; };
-    // largest key, and the first token that has it
-    unsigned long long best = 0;
-    for (int i = tid; i < V; i += kThreads) best = most(best, (unsigned long long)key_of(widen(x[i])) << 32 | (0xFFFFFFFFu - (uint32_t)i));
-    best = block_reduce(best, most, s_u);
-    const uint32_t top = (uint32_t)(best >> 32);
-    const float t = a.temperature[row];
-    if (top == 0 || !(t > 0.f)) {
-        if (tid == 0) a.tokens[row] = top == 0 ? -1 : (int64_t)(0xFFFFFFFFu - (uint32_t)best);
-        return;
+// Sum of all threads' values before this thread's; `total`: of all.
+template <typename R>
+__device__ R block_scan(R v, R &total, R *shared) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    R incl = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const R u = __shfl_up_sync(kFull, incl, d);
+        if (lane >= d) incl += u;
     }
-    const double largest = value_of(top), temperature = t;
-    const auto weight = [&](uint32_t key) { return key == 0 ? 0.0 : exp(((double)value_of(key) - largest) / temperature); };
-    // the cut: tokens of keys above `cut`, and the first `ties` tokens of key `cut`
+    __syncthreads();
+    if (lane == 31) shared[warp] = incl;
+    __syncthreads();
+    R before = 0;
+    total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) before = total;
+        total += shared[w];
+    }
+    return before + (incl - v);
+}
+
+// Descending bitonic sort of n (at most kList) places, padded with zeros to a power of two.
+__device__ void sort_places(uint64_t *list, int n) {
+    int size = 2;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
+    __syncthreads();
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+                const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+                const uint64_t p = list[lo], q = list[hi];
+                if ((p < q) == ((lo & k) == 0)) list[lo] = q, list[hi] = p;
+            }
+            __syncthreads();
+        }
+}
+
+// The smallest weight that stays; the largest weight, 1, always does.
+__device__ __forceinline__ double least_of(const SampleArgs &a, int row) {
+    const float p = a.min_p ? a.min_p[row] : 0.f;
+    return p > 0.f ? fminf(p, 1.f) : 0.f;
+}
+
+// Eight consecutive logits; NaN behind the row's end.
+template <typename T>
+__device__ __forceinline__ void load_eight(const T *x, int i, int V, bool wide, float (&v)[8]) {
+    if (wide && i + 8 <= V) {
+        T raw[8];
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4 *>(raw)[j] = __ldg(reinterpret_cast<const uint4 *>(x + i) + j);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = clean(widen(raw[j]));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = i + j < V ? clean(widen(x[i + j])) : NAN;
+    }
+}
+
+// One CTA, bisection of the keys: (cut, ties) are a key and the number of its tokens that stay, lower tokens first.
+template <typename T>
+__device__ void sample_slowly(const SampleArgs &a, Shared &s, const T *x, int row, uint32_t top, double largest, double scale) {
+    const int tid = threadIdx.x, V = a.V;
+    const auto weight = [&](uint32_t key) { return key == 0 ? 0.0 : weight_of(value_of(key), largest, scale, s.roots); };
+    const auto key_at = [&](int i) { return key_of(clean(widen(x[i]))); };
+    unsigned long long *s_u = reinterpret_cast<unsigned long long *>(s.best);
     uint32_t cut = 1;
     long long ties = V;
     const int k = a.top_k ? a.top_k[row] : 0;
@@ -87,8 +199,8 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
         while (lo < hi) {
             const uint32_t mid = lo + (hi - lo) / 2 + 1;
             unsigned long long n = 0;
-            for (int i = tid; i < V; i += kThreads) n += key_of(widen(x[i])) >= mid;
-            n = block_reduce(n, plus, s_u);
+            for (int i = tid; i < V; i += kThreads) n += key_at(i) >= mid;
+            n = block_reduce(n, Plus(), s_u);
             if ((long long)n >= k) lo = mid;
             else hi = mid - 1, above = (long long)n;
         }
@@ -99,17 +211,15 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
     if (p < 1.f) {
         const auto total = [&](uint32_t from) {           // weight of the tokens of keys from `from` on, inside the cut
             double w = 0.0;
+            unsigned long long n = 0;
             for (int i = tid; i < V; i += kThreads) {
-                const uint32_t key = key_of(widen(x[i]));
+                const uint32_t key = key_at(i);
                 if (key >= from && key > cut) w += weight(key);
+                n += key == cut;
             }
-            w = block_reduce(w, plus, s_d);
-            if (from <= cut) {
-                unsigned long long n = 0;
-                for (int i = tid; i < V; i += kThreads) n += key_of(widen(x[i])) == cut;
-                n = block_reduce(n, plus, s_u);
-                if (n > 0) w += (double)((long long)n < ties ? (long long)n : ties) * weight(cut);   // (no token has a NaN's key)
-            }
+            w = block_reduce(w, Plus(), s.scan);
+            n = block_reduce(n, Plus(), s_u);
+            if (from <= cut && n > 0) w += (double)((long long)n < ties ? (long long)n : ties) * weight(cut);   // (no token has a NaN's key)
             return w;
         };
         const double aim = (double)p * total(cut);
@@ -128,43 +238,431 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
         ties = lo == cut && ties < n ? ties : n;
         cut = lo;
     }
-    const double least = a.min_p ? (double)a.min_p[row] : 0.0;
+    const double least = least_of(a, row);
     // runs of consecutive tokens per thread: ties before it, weight before it, the token
     const int per = (V + kThreads - 1) / kThreads, i0 = min(tid * per, V), i1 = min(i0 + per, V);
-    int same = 0;
-    for (int i = i0; i < i1; ++i) same += key_of(widen(x[i])) == cut;
-    s_ties[tid] = same;
-    __syncthreads();
-    long long before = 0;
-    for (int j = 0; j < tid; ++j) before += s_ties[j];
+    int same = 0, all_same = 0;
+    for (int i = i0; i < i1; ++i) same += key_at(i) == cut;
+    const long long before = block_scan(same, all_same, s.scan_n);
     const auto walk = [&](double from, double aim, int &found) {
         long long n = before;
         for (int i = i0; i < i1; ++i) {
-            const uint32_t key = key_of(widen(x[i]));
+            const uint32_t key = key_at(i);
             if (key == 0 || key < cut || (key == cut && n++ >= ties)) continue;
             const double w = weight(key);
             if (w < least || w == 0.0) continue;
+            found = i;
             from += w;
-            if (from > aim) {
-                found = i;
-                return from;
-            }
+            if (from > aim) return from;
         }
         return from;
     };
     int found = -1;
-    s_line[tid] = walk(0.0, INFINITY, found);
-    __syncthreads();
-    double from = 0.0, all = 0.0;
-    for (int j = 0; j < kThreads; ++j) {
-        if (j == tid) from = all;
-        all += s_line[j];
-    }
+    const double mine = walk(0.0, INFINITY, found);
+    double all = 0.0;
+    const double from = block_scan(mine, all, s.scan);
     const double aim = (double)a.uniforms[row] * all;
-    if (s_line[tid] > 0.0 && from <= aim && from + s_line[tid] > aim) {
-        walk(from, aim, found);
-        if (found >= 0) a.tokens[row] = found;
+    // the first run that ends behind the aim; rounding may leave none, then the last that has a token
+    if (tid == 0) s.found = INT32_MAX;
+    __syncthreads();
+    if (mine > 0.0 && from + mine > aim) atomicMin(&s.found, tid);
+    __syncthreads();
+    if (s.found == INT32_MAX) {
+        __syncthreads();
+        if (tid == 0) s.found = -1;
+        __syncthreads();
+        if (mine > 0.0) atomicMax(&s.found, tid);
+        __syncthreads();
     }
+    if (tid == s.found) {
+        walk(from, aim, found);
+        a.tokens[row] = found;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ SampleArgs a) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    Shared &s = *reinterpret_cast<Shared *>(raw);
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int ctas = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / ctas, V = a.V;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const T *x = reinterpret_cast<const T *>(a.logits) + row * a.row_stride;
+    Shared &first = *cluster.map_shared_rank(&s, 0);           // of the CTA that finishes the row
+    // a warp's span: whole steps
+    const int spans = ctas * kWarps, span = ((V + spans - 1) / spans + kStep - 1) / kStep * kStep;
+    const int me = rank * kWarps + warp, i0 = min((long long)me * span, (long long)V), i1 = min((long long)i0 + span, (long long)V);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    // ---- 1: the largest logit, the lowest token that has it
+    float most = -INFINITY;
+    int at = -1;
+    for (int i = i0 + lane * 8; i < i1; i += kStep) {
+        float v[8];
+        load_eight(x, i, V, a.wide, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (v[j] > most) most = v[j], at = i + j;
+    }
+    if (tid < 32) s.roots[tid] = exp2((double)tid / 32.0);
+    if (tid == 0) s.listed = 0;
+    const uint64_t here = block_reduce(at < 0 ? (uint64_t)0 : place_of(most, at), Most(), s.best);
+    if (tid == 0) s.cta_best = here;
+    cluster.sync();
+    uint64_t best = 0;
+    for (int r = 0; r < ctas; ++r) best = Most()(best, cluster.map_shared_rank(&s, r)->cta_best);
+    const float t = a.temperature[row];
+    if (best == 0 || !(t > 0.f)) {
+        if (rank == 0 && tid == 0) a.tokens[row] = best == 0 ? -1 : token_of(best);
+        cluster.sync();
+        return;
+    }
+    const float top = value_of((uint32_t)(best >> 32));
+    const double largest = top, scale = 1.4426950408889634074 / (double)t, least = least_of(a, row);
+    const int k = a.top_k ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : 1.f;
+    const bool use_k = k > 0 && k < V, use_p = p < 1.f;
+    bool slow = use_k && k > kMostK;
+
+    // ---- intervals of the logit, from the largest one down to a sample's smallest (or to where weights vanish)
+    const int sampled = V < kSample ? V : kSample;
+    float per_bin = 0.f;
+    if (!slow && (use_k || use_p)) {
+        const double stride = (double)V / sampled;
+        float low = INFINITY;
+        float v[kSample / kThreads];
+#pragma unroll
+        for (int j = 0; j < kSample / kThreads; ++j) {
+            const int i = tid + j * kThreads;
+            v[j] = i < sampled ? clean(widen(x[(int)(i * stride)])) : NAN;
+            if (v[j] > -INFINITY && v[j] < low) low = v[j];
+        }
+        low = block_reduce(low, Least(), s.low);
+        float range = top - low;                                // (minus infinity without a finite sample)
+        if (!use_k && range > 30.f * t) range = 30.f * t;
+        per_bin = range > 0.f ? fminf(kBins / range, FLT_MAX) : 0.f;
+        for (int i = tid; i < kBins; i += kThreads) s.bin.count[i] = 0;
+        __syncthreads();
+        if (use_k) {
+#pragma unroll
+            for (int j = 0; j < kSample / kThreads; ++j)
+                if (v[j] > -INFINITY) atomicAdd(&s.bin.count[min(kBins - 1, (int)((top - v[j]) * per_bin))], 1u);
+            __syncthreads();
+        }
+    }
+    const auto bin_of = [&](float v) { return min(kBins - 1, (int)((top - v) * per_bin)); };
+
+    if (use_k && !slow) {
+        // ---- the lowest interval that is listed: what the sample says holds some hundreds more than k
+        const int need = sampled == V ? k : (int)((long long)(k + k / 2 + 400) * sampled / V) + 8;
+        uint32_t c[kBins / kThreads], sum = 0;
+#pragma unroll
+        for (int j = 0; j < kBins / kThreads; ++j) c[j] = s.bin.count[tid * (kBins / kThreads) + j], sum += c[j];
+        if (tid == 0) s.decided = kBins - 1;
+        int total;
+        int before = block_scan((int)sum, total, s.scan_n);
+#pragma unroll
+        for (int j = 0; j < kBins / kThreads; ++j) {
+            if (before < need && before + (int)c[j] >= need) s.decided = tid * (kBins / kThreads) + j;
+            before += c[j];
+        }
+        __syncthreads();
+        const int lowest = s.decided;
+        for (int i = i0 + lane * 8; i - lane * 8 < i1; i += kStep) {
+            float v[8];
+            load_eight(x, i, i1, a.wide, v);
+            unsigned in = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) in |= (v[j] > -INFINITY && bin_of(v[j]) <= lowest ? 1u : 0u) << j;
+            if (in) {
+                int n = atomicAdd(&first.listed, __popc(in));
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (in >> j & 1) {
+                        if (n < kList) first.list[n] = place_of(v[j], i + j);
+                        ++n;
+                    }
+            }
+        }
+        cluster.sync();
+        if (rank != 0) return;
+        const int n = s.listed;
+        slow = n > kList || (n < k && lowest < kBins - 1);
+        if (!slow) {
+            sort_places(s.list, n);
+            const int kept_k = n < k ? n : k;
+            // weights of the first k, two consecutive ones per thread; all cuts keep a prefix
+            double w[2], sum_w = 0.0, all;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int i = 2 * tid + j;
+                w[j] = i < kept_k ? weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots) : 0.0;
+                sum_w += w[j];
+            }
+            double before_w = block_scan(sum_w, all, s.scan);
+            int kept = 0;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int i = 2 * tid + j;
+                if (i < kept_k && (i == 0 || !use_p || before_w < (double)p * all) && w[j] >= least && w[j] > 0.0) {
+                    ++kept;
+                    s.line[i] = w[j];
+                }
+                before_w += w[j];
+            }
+            int total_kept;
+            block_scan(kept, total_kept, s.scan_n);
+            __syncthreads();
+            // in the order of the vocabulary: descending complement of the token, with the place in the sorted list
+            for (int i = tid; i < total_kept; i += kThreads) s.list[i] = s.list[i] << 32 | (uint32_t)i;
+            __syncthreads();
+            sort_places(s.list, total_kept);
+            sum_w = 0.0;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int i = 2 * tid + j;
+                w[j] = i < total_kept ? s.line[(uint32_t)s.list[i]] : 0.0;
+                sum_w += w[j];
+            }
+            before_w = block_scan(sum_w, all, s.scan);
+            const double aim = (double)a.uniforms[row] * all;
+            if (tid == 0) s.found = total_kept - 1;             // (rounding may leave no sum above the aim)
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int i = 2 * tid + j;
+                before_w += w[j];
+                if (i < total_kept && before_w > aim) atomicMin(&s.found, i);
+            }
+            __syncthreads();
+            // (a weight that counts was computed from the first token on, so there is one)
+            if (tid == 0) a.tokens[row] = (int64_t)(0xFFFFFFFFu - (uint32_t)(s.list[s.found] >> 32));
+            return;
+        }
+        sample_slowly(a, s, x, row, (uint32_t)(best >> 32), largest, scale);
+        return;
+    }
+    if (slow) {
+        cluster.sync();
+        if (rank == 0) sample_slowly(a, s, x, row, (uint32_t)(best >> 32), largest, scale);
+        return;
+    }
+
+    // ---- 2: weights, and the interval in which the nucleus ends
+    int edge = kBins;                                           // everything lies above it
+    double all = 0.0;
+    if (use_p) {
+        double w_sum = 0.0;
+        for (int i = i0 + lane * 8; i < i1; i += kStep) {
+            float v[8];
+            load_eight(x, i, i1, a.wide, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (!(v[j] > -INFINITY)) continue;
+                const double w = weight_of(v[j], largest, scale, s.roots);
+                w_sum += w;
+                atomicAdd(&s.bin.weight[bin_of(v[j])], (float)w);
+            }
+        }
+        w_sum = block_reduce(w_sum, Plus(), s.scan);
+        if (tid == 0) s.cta_sum = w_sum;
+        cluster.sync();
+        for (int r = 0; r < ctas; ++r) all += cluster.map_shared_rank(&s, r)->cta_sum;
+        // (every CTA adds the same numbers in the same order)
+        float c[kBins / kThreads];
+        double sum = 0.0, total;
+#pragma unroll
+        for (int j = 0; j < kBins / kThreads; ++j) {
+            c[j] = 0.f;
+            for (int r = 0; r < ctas; ++r) c[j] += cluster.map_shared_rank(&s, r)->bin.weight[tid * (kBins / kThreads) + j];
+            sum += c[j];
+        }
+        if (tid == 0) s.decided = kBins - 1;
+        double before = block_scan(sum, total, s.scan);
+        const double aim = (double)p * all;
+#pragma unroll
+        for (int j = 0; j < kBins / kThreads; ++j) {
+            if ((before < aim || (tid == 0 && j == 0)) && before + c[j] >= aim) atomicMin(&s.decided, tid * (kBins / kThreads) + j);
+            before += c[j];
+        }
+        __syncthreads();
+        edge = s.decided;
+    }
+
+    // ---- 3: what lies above the interval, per span, and what lies in it
+    uint64_t border = 0;                                        // the last place that stays
+    for (int tries = 0;; ++tries) {
+        double above = 0.0, kept = 0.0;
+        for (int i = i0 + lane * 8; i < i1; i += kStep) {
+            float v[8];
+            load_eight(x, i, i1, a.wide, v);
+            unsigned in = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (!(v[j] > -INFINITY)) continue;
+                const int bin = edge < kBins ? bin_of(v[j]) : 0;
+                if (bin < edge) {
+                    const double w = weight_of(v[j], largest, scale, s.roots);
+                    above += w;
+                    if (w >= least) kept += w;
+                } else if (bin == edge) {
+                    in |= 1u << j;
+                }
+            }
+            if (in) {
+                int n = atomicAdd(&first.listed, __popc(in));
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (in >> j & 1) {
+                        if (n < kList) first.list[n] = place_of(v[j], i + j);
+                        ++n;
+                    }
+            }
+        }
+        above = warp_reduce(above, Plus()), kept = warp_reduce(kept, Plus());
+        if (lane == 0) first.span_all[me] = above, first.span_kept[me] = kept;
+        cluster.sync();
+        if (!use_p) break;
+        if (rank == 0) {
+            const int n = s.listed;
+            int next = -1;                                      // -1: done, -2: the slow way, else: the interval to look at
+            if (n > kList) {
+                next = -2;
+            } else {
+                sort_places(s.list, n);
+                double over = 0.0, total, running = 0.0;
+                for (int i = 0; i < spans; ++i) over += s.span_all[i];
+                // eight consecutive places per thread
+                constexpr int kEach = kList / kThreads;
+                double w[kEach], sum = 0.0;
+#pragma unroll
+                for (int j = 0; j < kEach; ++j) {
+                    const int i = tid * kEach + j;
+                    w[j] = i < n ? weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots) : 0.0;
+                    sum += w[j];
+                }
+                running = over + block_scan(sum, total, s.scan);
+                const double aim = (double)p * all;
+                if (over >= aim && edge > 0) next = edge - 1;
+                else if (over + total < aim && edge < kBins - 1) next = edge + 1;
+                if (tries == 4 && next >= 0) next = -2;
+                if (next == -1) {
+                    int inside = 0, total_inside;
+#pragma unroll
+                    for (int j = 0; j < kEach; ++j) {
+                        const int i = tid * kEach + j;
+                        if (i < n && (running < aim || s.list[i] == best))
+                            ++inside;
+                        running += w[j];
+                    }
+                    block_scan(inside, total_inside, s.scan_n);
+                    if (tid == 0) s.border = total_inside > 0 ? s.list[total_inside - 1] : 1;
+                    __syncthreads();
+                    // spans' sums in a fixed order: a warp each, over the places that stay
+                    for (int sp = warp; sp < spans; sp += kWarps) {
+                        double more = 0.0;
+                        for (int i = lane; i < total_inside; i += 32)
+                            if (token_of(s.list[i]) / span == sp) {
+                                const double v = weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots);
+                                if (v >= least) more += v;
+                            }
+                        more = warp_reduce(more, Plus());
+                        if (lane == 0) s.span_kept[sp] += more;
+                    }
+                }
+            }
+            if (tid == 0) {
+                s.listed = 0;
+                s.decided = next;
+            }
+            __syncthreads();
+        }
+        cluster.sync();
+        const int next = first.decided;
+        border = first.border;
+        cluster.sync();
+        if (next == -2) {
+            if (rank == 0) sample_slowly(a, s, x, row, (uint32_t)(best >> 32), largest, scale);
+            return;
+        }
+        if (next == -1) break;
+        edge = next;
+    }
+    if (rank != 0) return;
+
+    // ---- the span in which the draw falls, walked by one warp
+    if (warp != 0) return;
+    double total = 0.0, from = 0.0;
+    for (int i = 0; i < spans; ++i) total += s.span_kept[i];
+    const double aim = (double)a.uniforms[row] * total;
+    int chosen = -1, last = 0;
+    double sum = 0.0;
+    for (int i = 0; i < spans; ++i) {
+        const double w = s.span_kept[i];
+        if (w > 0.0) last = i;
+        if (chosen < 0 && w > 0.0 && sum + w > aim) chosen = i, from = sum;
+        sum += w;
+    }
+    if (chosen < 0) chosen = last, from = total - s.span_kept[last];
+    int token = -1;
+    const int j0 = chosen * span, j1 = min(j0 + span, V);
+    for (int i = j0 + lane * 8; i - lane * 8 < j1; i += kStep) {
+        float v[8];
+        load_eight(x, i, j1, a.wide, v);
+        double w[8], mine = 0.0;
+        int mine_last = -1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            w[j] = 0.0;
+            if (v[j] > -INFINITY && place_of(v[j], i + j) >= border) w[j] = weight_of(v[j], largest, scale, s.roots);
+            if (w[j] < least) w[j] = 0.0;
+            if (w[j] > 0.0) mine_last = i + j;
+            mine += w[j];
+        }
+        double incl = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const double u = __shfl_up_sync(kFull, incl, d);
+            if (lane >= d) incl += u;
+        }
+        const unsigned over = __ballot_sync(kFull, mine > 0.0 && from + incl > aim);
+        if (over) {
+            const int who = __ffs(over) - 1;
+            if (lane == who) {
+                double f = from + (incl - mine);
+                token = mine_last;
+                for (int j = 0; j < 8; ++j) {
+                    f += w[j];
+                    if (w[j] > 0.0 && f > aim) {
+                        token = i + j;
+                        break;
+                    }
+                }
+            }
+            token = __shfl_sync(kFull, token, who);
+            break;
+        }
+        // (rounding may leave no sum above the aim: then it is the last token that stays)
+        token = Most()(token, warp_reduce(mine_last, Most()));
+        from += __shfl_sync(kFull, incl, 31);
+    }
+    if (lane == 0) a.tokens[row] = token;
+}
+
+template <typename T>
+cudaError_t launch(const SampleArgs &a, int B, int ctas, cudaStream_t st) {
+    static_assert(sizeof(Shared) <= 64 * 1024, "three CTAs per SM");
+    const cudaError_t raised = cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared));
+    if (raised != cudaSuccess) return raised;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)B * ctas), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = sizeof(Shared), cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, k_sample<T>, a);
 }
 
 }  // namespace
@@ -173,12 +671,22 @@ extern "C" int adacode_sample_tokens(const void *logits, int64_t row_stride, int
                                      const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
                                      int64_t *tokens, void *stream) {
     if (B < 0 || V <= 0 || (B > 0 && (!logits || !uniforms || !temperature || !tokens))) return ADACODE_ERR_INVALID_ARG;
+    if (dtype != ADACODE_BF16 && dtype != ADACODE_FP16 && dtype != ADACODE_FP32) return ADACODE_ERR_INVALID_ARG;
+    if (V > 1 << 30 || B > 1 << 27) return ADACODE_ERR_TOO_LARGE;
     if (B == 0) return ADACODE_OK;
-    const SampleArgs a{logits, row_stride, V, uniforms, temperature, top_p, min_p, top_k, tokens};
+    const int size = dtype == ADACODE_FP32 ? 4 : 2;
+    const bool wide = ((uintptr_t)logits & 15) == 0 && (row_stride * size) % 16 == 0;
+    const SampleArgs a{logits, row_stride, V, wide, uniforms, temperature, top_p, min_p, top_k, tokens};
+    // As many CTAs per row as keep the GPU's 148 SMs busy, three on each, and leave every warp a step or more of the vocabulary.
+    int ctas = 1;
+    while (ctas < kMostCtas && (int64_t)B * ctas < 2 * 148 && V > 2 * ctas * kWarps * kStep / 2) ctas *= 2;
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == ADACODE_BF16) k_sample<__nv_bfloat16><<<B, kThreads, 0, st>>>(a);
-    else if (dtype == ADACODE_FP16) k_sample<__half><<<B, kThreads, 0, st>>>(a);
-    else if (dtype == ADACODE_FP32) k_sample<float><<<B, kThreads, 0, st>>>(a);
-    else return ADACODE_ERR_INVALID_ARG;
-    return cudaGetLastError() == cudaSuccess ? ADACODE_OK : ADACODE_ERR_CUDA;
+    const cudaError_t e = dtype == ADACODE_BF16 ? launch<__nv_bfloat16>(a, B, ctas, st)
+                          : dtype == ADACODE_FP16 ? launch<__half>(a, B, ctas, st)
+                                                  : launch<float>(a, B, ctas, st);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return ADACODE_ERR_CUDA;
+    }
+    return ADACODE_OK;
 }
