@@ -39,7 +39,10 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 128;               // cached positions per tile, rows per stream
-constexpr int kAttnThreads = 320;
+constexpr int kAttnThreads = 384;         // two warpgroups of softmax, one of which two warps work
+// Registers per thread: 384 x 168 at the launch, which the softmax (whose rows are held whole) takes from the others.
+constexpr int kRegsRows = 216, kRegsRest = 72;
+static_assert(256 * kRegsRows + 128 * kRegsRest <= 384 * 168, "a split of what the launch has");
 constexpr int kPieces = 4;               // pieces that the loading warp is ahead at most
 constexpr float kLag = 8.f;              // how far (powers of two) a maximum may be behind
 
@@ -54,6 +57,7 @@ struct PagedArgs {
     uint32_t negate;
     int box_rows;             // rows per tensor copy
     int room;                 // positions that the table has
+    Quotient by_page;
     float *part_o, *part_ml;  // [2 CTAs][rows][D], [2 CTAs][rows][2]
     struct Cut *cuts;         // [CTAs]
     int32_t *status;
@@ -166,6 +170,80 @@ __device__ __forceinline__ uint32_t pack_two<__half>(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+
+// Two floats in one register pair, for the packed instructions.
+using Two = unsigned long long;
+__device__ __forceinline__ Two two(float lo, float hi) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void parts(Two v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ Two fma_two(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ Two add_two(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float most_of(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2**y of two numbers (at least 2**-126) on the FMA pipe: y rounded to a whole number n, the power of the rest by a polynomial
+// (least relative error on [-1/2, 1/2], found by weighted least squares: 7.5e-5 of degree 3 for bf16, whose rounding is up to
+// 3.9e-3, 2.6e-6 of degree 4 for fp16), n added to the exponent.
+template <typename T>
+__device__ __forceinline__ void exp2_two(Two y, float &p0, float &p1) {
+    constexpr float kShift = 12582912.f;                      // 1.5 x 2**23
+    float y0, y1;
+    parts(y, y0, y1);
+    y = two(fmaxf(y0, -126.f), fmaxf(y1, -126.f));
+    const Two t = add_two(y, two(kShift, kShift)), r = fma_two(add_two(t, two(-kShift, -kShift)), two(-1.f, -1.f), y);
+    Two p;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        p = fma_two(r, two(0.05517167f, 0.05517167f), two(0.24261113f, 0.24261113f));
+        p = fma_two(p, r, two(0.69326097f, 0.69326097f));
+        p = fma_two(p, r, two(0.99992806f, 0.99992806f));
+    } else {
+        p = fma_two(r, two(0.0095701022f, 0.0095701022f), two(0.05591786f, 0.05591786f));
+        p = fma_two(p, r, two(0.24024744f, 0.24024744f));
+        p = fma_two(p, r, two(0.69312179f, 0.69312179f));
+        p = fma_two(p, r, two(0.99999928f, 0.99999928f));
+    }
+    float t0, t1;
+    parts(t, t0, t1);
+    parts(p, p0, p1);
+    p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+    p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
+// The weights of 32 scores: summed up, rounded, stored to 16 columns of TMEM.  POLY of every eight pairs take the polynomial, the others the
+// special function unit, which alone would take as long as the products.
+template <typename T, int POLY>
+__device__ __forceinline__ void weigh(const uint32_t (&x)[32], Two c, Two base, Two (&sum)[2], uint32_t at) {
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const Two y = fma_two(two(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c, base);
+        float p0, p1;
+        if (e % 8 < POLY) {
+            exp2_two<T>(y, p0, p1);
+        } else {
+            parts(y, p0, p1);
+            p0 = exp2_fast(p0), p1 = exp2_fast(p1);
+        }
+        sum[e & 1] = add_two(sum[e & 1], two(p0, p1));
+        w[e] = pack_two<T>(p0, p1);
+    }
+    tmem_st16(w, at);
+}
+constexpr int kByPolynomial = 3;
 
 // ---------------------------------------------------------------------------------------
 // units
@@ -378,24 +456,34 @@ __device__ __forceinline__ bool load_pieces(const PagedArgs &a, Shared<D, SOLO> 
                 if (len > a.room) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
             }
             pr.next();
-            // keys of a tile come one tile (SOLO: two) before its values
+            // Keys of a tile come one tile (SOLO: two) before its values.  A lane has one page (of box_rows slots) and 64 columns; the table is
+            // read one tile ahead, so that its latency hides behind the copies.
             constexpr int kAhead = SOLO ? 2 : 1;
             const int part = lane / (D / 64), half = lane - part * (D / 64);
+            const auto boxes_of = [&](int j) {                                        // pages of tile j that hold tokens
+                const int valid = len - (j0 + j) * kTile;
+                return j >= tiles || valid <= 0 ? 0 : valid >= kTile ? kTile / a.box_rows : (valid + a.box_rows - 1) / a.box_rows;
+            };
+            const auto look_up = [&](int j, int &slot_in) {
+                if (part >= boxes_of(j)) return -1;
+                const int at = (j0 + j) * kTile + part * a.box_rows, entry = (int)((uint32_t)at / a.by_page);
+                slot_in = at - entry * c.page_size;
+                return entry < c.table_width ? c.block_table[b * c.table_stride + entry] : -1;
+            };
+            int page[kAhead + 1], slot_in[kAhead + 1], next_slot = 0;
+            int next_page = look_up(0, next_slot);
             for (int i = 0; ok && i < tiles + kAhead; ++i) {
+#pragma unroll
+                for (int k = kAhead; k > 0; --k) page[k] = page[k - 1], slot_in[k] = slot_in[k - 1];
+                page[0] = next_page, slot_in[0] = next_slot;
+                next_page = look_up(i + 1, next_slot);
 #pragma unroll
                 for (int which = 0; which < 2; ++which) {
                     const int j = which ? i - kAhead : i;
                     if (j < 0 || j >= tiles) continue;
                     Ring &r = which ? vr : kr;
                     uint64_t *full = which ? &s.v_full[r.at] : &s.k_full[r.at];
-                    const int at = (j0 + j) * kTile, valid = len - at < kTile ? (len - at > 0 ? len - at : 0) : kTile;
-                    const int boxes = (valid + a.box_rows - 1) / a.box_rows;
-                    int page = c.n_pages, slot_in = 0;                                // (a page behind the pool reads as zeros)
-                    if (part < boxes) {
-                        const int p = page_of(c, b, at + part * a.box_rows, slot_in);
-                        if (p >= 0) page = p;
-                        else atomicOr(a.status, ADACODE_STATUS_BAD_PAGE), slot_in = 0;
-                    }
+                    const int boxes = boxes_of(j);
                     ok = warp_wait(which ? &s.v_empty[r.at] : &s.k_empty[r.at], r.phase ^ 1, a.status);
                     if (!ok) break;
                     if (lane == 0) {
@@ -403,12 +491,18 @@ __device__ __forceinline__ bool load_pieces(const PagedArgs &a, Shared<D, SOLO> 
                         else mbar_arrive(full);
                     }
                     __syncwarp();
-                    if (part < boxes)
+                    if (part < boxes) {
+                        int from = page[which ? kAhead : 0], first_slot = slot_in[which ? kAhead : 0];
+                        if (from < 0 || from >= c.n_pages) {                          // (a page behind the pool reads as zeros)
+                            from = c.n_pages, first_slot = 0;
+                            atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
+                        }
                         asm volatile(
                             "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
                                 smem_u32((which ? s.v[r.at] : s.k[r.at]) + half * S::kHalf + part * a.box_rows * 128)),
-                            "l"(which ? &vm : &km), "r"(half * 64), "r"(slot_in), "r"(h), "r"(page), "r"(smem_u32(full))
+                            "l"(which ? &vm : &km), "r"(half * 64), "r"(first_slot), "r"(h), "r"(from), "r"(smem_u32(full))
                             : "memory");
+                    }
                     r.next();
                     ++held;
                 }
@@ -583,9 +677,9 @@ __device__ __forceinline__ bool soften_pieces(const PagedArgs &a, Shared<D, SOLO
                 float top[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    top[k] = __uint_as_float(x[k][0]);
+                    top[k] = fmaxf(__uint_as_float(x[k][0]), __uint_as_float(x[k][1]));
 #pragma unroll
-                    for (int e = 1; e < 32; ++e) top[k] = fmaxf(top[k], __uint_as_float(x[k][e]));
+                    for (int e = 2; e < 32; e += 2) top[k] = most_of(top[k], __uint_as_float(x[k][e]), __uint_as_float(x[k][e + 1]));
                 }
                 const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 if (n < (SOLO ? 2 : 1)) {
@@ -610,20 +704,20 @@ __device__ __forceinline__ bool soften_pieces(const PagedArgs &a, Shared<D, SOLO
                     }
                 }
                 const float base = m == -INFINITY ? 0.f : m * c;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const Two c2 = two(c, c), base2 = two(-base, -base);
+                // (the polynomial's smallest power is 2**-126, not 0: not where positions may be hidden)
+                const bool plain = warp_lo > j || warp_hi < j + kTile || __any_sync(kFull, m == -INFINITY);
+                Two sum[2] = {two(0.f, 0.f), two(0.f, 0.f)};
+                if (plain) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    uint32_t w[16];
+                    for (int k = 0; k < 4; ++k) weigh<T, 0>(x[k], c2, base2, sum, s_at + 16 * k);
+                } else {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float p0 = exp2_fast(fmaf(__uint_as_float(x[k][2 * e]), c, -base));
-                        const float p1 = exp2_fast(fmaf(__uint_as_float(x[k][2 * e + 1]), c, -base));
-                        sum[e & 1] += p0, sum[2 + (e & 1)] += p1;
-                        w[e] = pack_two<T>(p0, p1);
-                    }
-                    tmem_st16(w, s_at + 16 * k);
+                    for (int k = 0; k < 4; ++k) weigh<T, kByPolynomial>(x[k], c2, base2, sum, s_at + 16 * k);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                float sums[4];
+                parts(sum[0], sums[0], sums[1]), parts(sum[1], sums[2], sums[3]);
+                l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
                 tmem_wait_st();
             }
             tmem_fence_before();
@@ -743,16 +837,18 @@ __global__ void __launch_bounds__(kAttnThreads, 1) k_paged_attn(const __grid_con
     tmem_fence_after();
     const uint32_t tmem = s.tmem;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (warp == 9) {
-        load_pieces<D, SOLO>(a, s, keys, values);
-    } else if (warp == 8) {
-        if (!multiply_pieces<T, D, SOLO>(a, s, tmem)) {
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsRows));
+        soften_pieces<T, D, SOLO>(a, s, tmem, warp >> 2);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
+        if (warp == 9) {
+            load_pieces<D, SOLO>(a, s, keys, values);
+        } else if (warp == 8 && !multiply_pieces<T, D, SOLO>(a, s, tmem)) {
             // (given up: products may still be running)
             if ((threadIdx.x & 31) == 0) mma_commit(&s.done);
             mbar_wait(&s.done, 0, a.status, 1u << 16);
         }
-    } else {
-        soften_pieces<T, D, SOLO>(a, s, tmem, warp >> 2);
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __syncwarp();
@@ -934,6 +1030,7 @@ int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int6
     a.part_o = (float *)workspace, a.part_ml = a.part_o + rows * D, a.cuts = (Cut *)(a.part_ml + rows * 2);
     const long long room = (long long)cache->table_width * cache->page_size;
     a.room = room < 1 << 30 ? (int)room : 1 << 30;
+    a.by_page = quotient_by(cache->page_size);
     a.status = status;
     CUtensorMap keys, values;
     if (!map_pages(keys, cache->key_pages, *cache, cache->key_page, cache->key_head, cache->key_slot, a.box_rows) ||
