@@ -124,20 +124,30 @@ __device__ __forceinline__ void tmem_st16(const uint32_t (&r)[16], uint32_t at) 
         "r"(at)
         : "memory");
 }
-// D[128 x N] (+)= A B, both operands in shared memory, or A (16-bit pairs along its columns) in TMEM
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-                 "r"((uint32_t)add)
-                 : "memory");
+// D[128 x N] (+)= A B, both operands in shared memory, or A (16-bit pairs along its columns) in TMEM.  Issued by one lane by a predicate, not
+// in a branch: operands that a branch on the lane makes look different per lane are moved one by one before every product (100 cycles
+// each; the product takes 64).
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader)
+        : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
-                 "r"((uint32_t)add)
-                 : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader)
+        : "memory");
 }
 // the barrier counts one arrival when all products issued so far are done
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void mma_commit(uint32_t leader, uint64_t *bar) {
+    asm volatile(
+        "{\n.reg .pred q;\nsetp.ne.b32 q, %1, 0;\n"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar)),
+        "r"(leader)
+        : "memory");
 }
 // Operands in shared memory are stacks of 8 rows of 128 bytes, their 16-byte pieces permuted by the row (128-byte swizzle); 64 columns
 // of all rows come before the next 64.  Rows of queries and keys are the product's rows (its sum runs along the columns); rows of
@@ -243,7 +253,7 @@ __device__ __forceinline__ void weigh(const uint32_t (&x)[32], Two c, Two base, 
     }
     tmem_st16(w, at);
 }
-constexpr int kByPolynomial = 3;
+constexpr int kByPolynomial = 0;
 
 // ---------------------------------------------------------------------------------------
 // units
@@ -545,29 +555,26 @@ __device__ __forceinline__ bool multiply_pieces(const PagedArgs &a, Shared<D, SO
     using S = Shape<D, SOLO>;
     constexpr uint32_t kScores = instruction<T>(kTile, false), kOut = instruction<T>(D, true);
     const int lane = threadIdx.x & 31;
+    const uint32_t leader = lane == 0;
     Ring kr(S::kKeys), vr(S::kValues), pr(kPieces);
     uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+    const uint64_t q_at = operand(smem_u32(s.q), 16), k_at = operand(smem_u32(s.k), 16), v_at = operand(smem_u32(s.v), S::kHalf);
     const auto scores = [&](int i) {         // stream i's next tile of keys, which has arrived
-        if (lane == 0) {
+        const uint64_t q = q_at + (SOLO ? 0 : i * (S::kBytes >> 4)), keys = k_at + kr.at * (S::kBytes >> 4);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                const uint32_t off = (k / 4) * S::kHalf + (k % 4) * 32;
-                mma_ss(tmem + i * 128, operand(smem_u32(s.q[SOLO ? 0 : i]) + off, 16), operand(smem_u32(s.k[kr.at]) + off, 16), kScores, k > 0);
-            }
-            mma_commit(&s.s_full[i]);
+        for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = ((k / 4) * S::kHalf + (k % 4) * 32) >> 4;
+            mma_ss(leader, tmem + i * 128, q + off, keys + off, kScores, k > 0);
         }
+        mma_commit(leader, &s.s_full[i]);
     };
     const auto output = [&](int i, bool add) {
-        if (lane == 0) {
+        const uint64_t values = v_at + vr.at * (S::kBytes >> 4);
 #pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
-                mma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, operand(smem_u32(s.v[vr.at]) + k * 2048, S::kHalf), kOut, add || k > 0);
-        }
+        for (int k = 0; k < kTile / 16; ++k)
+            mma_ts(leader, tmem + 256 + i * D, tmem + i * 128 + k * 8, values + k * (2048 >> 4), kOut, k > 0 ? 1u : (uint32_t)add);
     };
-    const auto release = [&](uint64_t *bar) {
-        if (lane == 0) mma_commit(bar);
-        __syncwarp();
-    };
+    const auto release = [&](uint64_t *bar) { mma_commit(leader, bar); };
     for (;;) {
         if (!warp_wait(&s.piece_full[pr.at], pr.phase, a.status)) return false;
         const Piece p = s.piece[pr.at];
@@ -835,7 +842,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) k_paged_attn(const __grid_con
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = s.tmem;
+    const uint32_t tmem = __shfl_sync(kFull, s.tmem, 0);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsRows));
@@ -846,7 +853,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) k_paged_attn(const __grid_con
             load_pieces<D, SOLO>(a, s, keys, values);
         } else if (warp == 8 && !multiply_pieces<T, D, SOLO>(a, s, tmem)) {
             // (given up: products may still be running)
-            if ((threadIdx.x & 31) == 0) mma_commit(&s.done);
+            mma_commit((threadIdx.x & 31) == 0, &s.done);
             mbar_wait(&s.done, 0, a.status, 1u << 16);
         }
     }
