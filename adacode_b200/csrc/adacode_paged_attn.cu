@@ -7,8 +7,8 @@
 // partial results (numerator, maximum, sum per row) that a second kernel merges.  Lengths lie on the device: every
 // CTA finds its run by itself.
 //
-// One CTA: warp 9 finds the pieces and loads (one tensor copy per page and 64 columns), warp 8 issues the products, two
-// warpgroups do the softmax, one row per thread.  S = Q K^T goes to TMEM, the weights go back to where S was, and
+// One CTA: warp 9 finds the pieces and loads (one tensor copy per page and 64 columns), warp 8 issues the products of both streams (a warp
+// for each made them interleave, and took a third longer), two warpgroups do the softmax, one row per thread.  S = Q K^T goes to TMEM, the weights go back to where S was, and
 // O += P V takes them from there.  Two streams of S, P and O let one's softmax run while the other's products do:
 //   PAIR  a unit has 256 rows, stream i the rows 128 i ..; every tile is used by both.
 //   SOLO  a unit has 128 rows; stream i takes every second tile, and the two meet at the end of the piece.  For few rows, where
@@ -41,7 +41,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 128;               // cached positions per tile, rows per stream
 constexpr int kAttnThreads = 384;         // two warpgroups of softmax, one of which two warps work
 // Registers per thread: 384 x 168 at the launch, which the softmax (whose rows are held whole) takes from the others.
-constexpr int kRegsRows = 216, kRegsRest = 72;
+constexpr int kRegsRows = 224, kRegsRest = 56;
 static_assert(256 * kRegsRows + 128 * kRegsRest <= 384 * 168, "a split of what the launch has");
 constexpr int kPieces = 4;               // pieces that the loading warp is ahead at most
 constexpr float kLag = 8.f;              // how far (powers of two) a maximum may be behind
@@ -205,55 +205,24 @@ __device__ __forceinline__ float most_of(float a, float b, float c) {
     return r;
 }
 
-// 2**y of two numbers (at least 2**-126) on the FMA pipe: y rounded to a whole number n, the power of the rest by a polynomial
-// (least relative error on [-1/2, 1/2], found by weighted least squares: 7.5e-5 of degree 3 for bf16, whose rounding is up to
-// 3.9e-3, 2.6e-6 of degree 4 for fp16), n added to the exponent.
+// The weights of 32 scores: summed up, rounded, stored to 16 columns of TMEM.  The special function unit takes eight cycles for a warp's
+// powers of two, 1024 for a tile, as long as the tile's products.  (A polynomial of degree 3 on the FMA pipe for a quarter to a half of them
+// made the two chunks of 2048 tokens behind 16384 slower, 652 us -> 674 and 694: what counts is a warp's own chain of
+// instructions, while the unit is idle half of the time.)
 template <typename T>
-__device__ __forceinline__ void exp2_two(Two y, float &p0, float &p1) {
-    constexpr float kShift = 12582912.f;                      // 1.5 x 2**23
-    float y0, y1;
-    parts(y, y0, y1);
-    y = two(fmaxf(y0, -126.f), fmaxf(y1, -126.f));
-    const Two t = add_two(y, two(kShift, kShift)), r = fma_two(add_two(t, two(-kShift, -kShift)), two(-1.f, -1.f), y);
-    Two p;
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        p = fma_two(r, two(0.05517167f, 0.05517167f), two(0.24261113f, 0.24261113f));
-        p = fma_two(p, r, two(0.69326097f, 0.69326097f));
-        p = fma_two(p, r, two(0.99992806f, 0.99992806f));
-    } else {
-        p = fma_two(r, two(0.0095701022f, 0.0095701022f), two(0.05591786f, 0.05591786f));
-        p = fma_two(p, r, two(0.24024744f, 0.24024744f));
-        p = fma_two(p, r, two(0.69312179f, 0.69312179f));
-        p = fma_two(p, r, two(0.99999928f, 0.99999928f));
-    }
-    float t0, t1;
-    parts(t, t0, t1);
-    parts(p, p0, p1);
-    p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-    p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
-}
-
-// The weights of 32 scores: summed up, rounded, stored to 16 columns of TMEM.  POLY of every eight pairs take the polynomial, the others the
-// special function unit, which alone would take as long as the products.
-template <typename T, int POLY>
 __device__ __forceinline__ void weigh(const uint32_t (&x)[32], Two c, Two base, Two (&sum)[2], uint32_t at) {
     uint32_t w[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         const Two y = fma_two(two(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c, base);
         float p0, p1;
-        if (e % 8 < POLY) {
-            exp2_two<T>(y, p0, p1);
-        } else {
-            parts(y, p0, p1);
-            p0 = exp2_fast(p0), p1 = exp2_fast(p1);
-        }
+        parts(y, p0, p1);
+        p0 = exp2_fast(p0), p1 = exp2_fast(p1);
         sum[e & 1] = add_two(sum[e & 1], two(p0, p1));
         w[e] = pack_two<T>(p0, p1);
     }
     tmem_st16(w, at);
 }
-constexpr int kByPolynomial = 0;
 
 // ---------------------------------------------------------------------------------------
 // units
@@ -292,19 +261,19 @@ __device__ __forceinline__ void sequence(const PagedArgs &a, int b, int &q0, int
 }
 // Tiles of all units of one head of sequence b.
 template <int ROWS>
-__device__ __forceinline__ long long head_tiles(const PagedArgs &a, int b) {
+__device__ __forceinline__ uint32_t head_tiles(const PagedArgs &a, int b) {
     int q0, fresh, len, start, first;
     sequence(a, b, q0, fresh, len, start);
     const int rows = fresh * a.G;
-    long long n = 0;
+    uint32_t n = 0;
     for (int r = 0; r < rows; r += ROWS) n += unit_tiles(a, r, r + ROWS < rows ? r + ROWS : rows, fresh, len, start, first);
     return n;
 }
-__device__ __forceinline__ long long warp_scan(long long v) {
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const long long u = __shfl_up_sync(kFull, v, d);
+        const uint32_t u = __shfl_up_sync(kFull, v, d);
         if (lane >= d) v += u;
     }
     return v;
@@ -399,71 +368,81 @@ struct Ring {
     }
 };
 
+// Finds where the run of CTA `cta` begins: the unit (its row0, sequence and head in `p`) and how many of its tiles come before.  Returns the run's
+// length; `ctas`: how many CTAs have runs (no CTA between two of a unit goes without a tile), `total`: all tiles.
+template <int ROWS>
+__device__ __forceinline__ int find_run(const PagedArgs &a, int cta, Piece &p, int &skipped, int &ctas, uint32_t &total) {
+    const adacode_paged_cache &c = a.cache;
+    const int lane = threadIdx.x & 31;
+    uint32_t mine = 0;
+    for (int b = lane; b < c.B; b += 32) mine += head_tiles<ROWS>(a, b);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(kFull, mine, d);
+    total = mine * c.Hkv;
+    ctas = total < gridDim.x ? (int)total : (int)gridDim.x;
+    if (cta >= ctas) return 0;
+    const uint32_t x = (uint32_t)((uint64_t)total * cta / ctas), end = (uint32_t)((uint64_t)total * (cta + 1) / ctas);
+    uint32_t from = 0, per_head = 0;
+    for (int b0 = 0;; b0 += 32) {
+        const uint32_t w = b0 + lane < c.B ? head_tiles<ROWS>(a, b0 + lane) : 0;
+        const uint32_t upto = from + warp_scan(w * c.Hkv);
+        const unsigned later = __ballot_sync(kFull, upto > x);
+        if (later || b0 + 32 >= c.B) {
+            const int l = later ? __ffs(later) - 1 : 31;
+            p.b = b0 + l;
+            per_head = __shfl_sync(kFull, w, l);
+            from = __shfl_sync(kFull, upto, l) - per_head * c.Hkv;
+            break;
+        }
+        from = __shfl_sync(kFull, upto, 31);
+    }
+    sequence(a, p.b, p.q0, p.fresh, p.len, p.start);
+    p.h = (int)((x - from) / per_head);
+    from += p.h * per_head;
+    for (p.row0 = 0;; p.row0 += ROWS) {
+        p.rows = p.fresh * a.G - p.row0 < ROWS ? p.fresh * a.G - p.row0 : ROWS;
+        const uint32_t n = unit_tiles(a, p.row0, p.row0 + p.rows, p.fresh, p.len, p.start, p.j0);
+        if (x < from + n) break;
+        from += n;
+    }
+    skipped = (int)(x - from);
+    return (int)(end - x);
+}
+
 // Loads: one lane per page and 64 columns of a tile.
 template <int D, bool SOLO>
 __device__ __forceinline__ bool load_pieces(const PagedArgs &a, Shared<D, SOLO> &s, const CUtensorMap &km, const CUtensorMap &vm) {
     using S = Shape<D, SOLO>;
     const adacode_paged_cache &c = a.cache;
-    const int lane = threadIdx.x & 31, cta = blockIdx.x;
-    // all tiles, and the sequence in which this CTA's run begins
-    long long total = 0;
-    for (int b = lane; b < c.B; b += 32) total += head_tiles<S::kRows>(a, b);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(kFull, total, d);
-    total *= c.Hkv;
-    // (no CTA between two of a unit goes without a tile)
-    const int ctas = total < gridDim.x ? (int)total : (int)gridDim.x;
-    long long x = cta < ctas ? total * cta / ctas : total;
-    const long long end = cta < ctas ? total * (cta + 1) / ctas : total;
-    Cut cut;
-    cut.n = 0;
+    const int lane = threadIdx.x & 31;
     Ring kr(S::kKeys), vr(S::kValues), pr(kPieces);
     bool ok = true;
-    int held = 0;                        // copies in flight at most, should the launch be given up
-    if (x < end) {
-        int b = 0;
-        long long from = 0, per_head = 0;
-        for (int b0 = 0; b0 < c.B; b0 += 32) {
-            const long long w = b0 + lane < c.B ? head_tiles<S::kRows>(a, b0 + lane) : 0;
-            const long long upto = from + warp_scan(w * c.Hkv);
-            const unsigned later = __ballot_sync(kFull, upto > x);
-            if (later) {
-                const int l = __ffs(later) - 1;
-                b = b0 + l;
-                per_head = __shfl_sync(kFull, w, l);
-                from = __shfl_sync(kFull, upto, l) - per_head * c.Hkv;
-                break;
-            }
-            from = __shfl_sync(kFull, upto, 31);
-        }
-        int q0, fresh, len, start;
-        sequence(a, b, q0, fresh, len, start);
-        int h = (int)((x - from) / per_head), row0 = 0, first = 0;
-        from += h * per_head;
-        int n = 0;
-        for (;; row0 += S::kRows) {
-            const int row1 = row0 + S::kRows < fresh * a.G ? row0 + S::kRows : fresh * a.G;
-            n = unit_tiles(a, row0, row1, fresh, len, start, first);
-            if (x < from + n) break;
-            from += n;
-        }
-        // one piece after the other
-        while (ok && x < end) {
-            const int rows = fresh * a.G, row1 = row0 + S::kRows < rows ? row0 + S::kRows : rows;
-            const long long upto = from + n < end ? from + n : end;
-            const int j0 = first + (int)(x - from), tiles = (int)(upto - x);
-            const bool begins = x == from, ends = upto == from + n;
-            const int slot = begins && ends ? -1 : begins ? 2 * cta + 1 : 2 * cta;
+    if (lane == 0) a.cuts[blockIdx.x].n = 0;
+    {
+        Piece p;
+        int skipped = 0, ctas;
+        uint32_t total;
+        int left = find_run<S::kRows>(a, blockIdx.x, p, skipped, ctas, total);
+        while (left > 0) {
+            // the next piece
+            int first;
+            const int all = unit_tiles(a, p.row0, p.row0 + p.rows, p.fresh, p.len, p.start, first);
+            const bool whole = all - skipped <= left;
+            p.j0 = first + skipped;
+            p.n = whole ? all - skipped : left;
+            p.slot = skipped > 0 ? 2 * blockIdx.x : whole ? -1 : 2 * blockIdx.x + 1;
             ok = warp_wait(&s.piece_empty[pr.at], pr.phase ^ 1, a.status);
             if (!ok) break;
-            if (begins && !ends) {
-                const int last = (int)(((from + n) * ctas - 1) / total);              // CTA of the unit's last tile
-                cut = {last - cta + 1, row1 - row0, row0, b, h, q0, fresh, len, start};
-            }
             if (lane == 0) {
-                s.piece[pr.at] = {tiles, j0, row1 - row0, row0, b, h, q0, fresh, len, start, slot};
+                if (skipped == 0 && !whole) {
+                    // CTA of the unit's last tile (which is left - all tiles behind this run's end)
+                    const uint32_t end = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / ctas);
+                    const int last = (int)(((uint64_t)(end + (all - left)) * ctas - 1) / total);
+                    a.cuts[blockIdx.x] = {last - (int)blockIdx.x + 1, p.rows, p.row0, p.b, p.h, p.q0, p.fresh, p.len, p.start};
+                }
+                s.piece[pr.at] = p;
                 mbar_arrive(&s.piece_full[pr.at]);
-                if (len > a.room) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
+                if (p.len > a.room) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
             }
             pr.next();
             // Keys of a tile come one tile (SOLO: two) before its values.  A lane has one page (of box_rows slots) and 64 columns; the table is
@@ -471,30 +450,29 @@ __device__ __forceinline__ bool load_pieces(const PagedArgs &a, Shared<D, SOLO> 
             constexpr int kAhead = SOLO ? 2 : 1;
             const int part = lane / (D / 64), half = lane - part * (D / 64);
             const auto boxes_of = [&](int j) {                                        // pages of tile j that hold tokens
-                const int valid = len - (j0 + j) * kTile;
-                return j >= tiles || valid <= 0 ? 0 : valid >= kTile ? kTile / a.box_rows : (valid + a.box_rows - 1) / a.box_rows;
+                const int valid = p.len - (p.j0 + j) * kTile;
+                return j >= p.n || valid <= 0 ? 0 : valid >= kTile ? kTile / a.box_rows : (valid + a.box_rows - 1) / a.box_rows;
             };
             const auto look_up = [&](int j, int &slot_in) {
                 if (part >= boxes_of(j)) return -1;
-                const int at = (j0 + j) * kTile + part * a.box_rows, entry = (int)((uint32_t)at / a.by_page);
+                const int at = (p.j0 + j) * kTile + part * a.box_rows, entry = (int)((uint32_t)at / a.by_page);
                 slot_in = at - entry * c.page_size;
-                return entry < c.table_width ? c.block_table[b * c.table_stride + entry] : -1;
+                return entry < c.table_width ? c.block_table[p.b * c.table_stride + entry] : -1;
             };
             int page[kAhead + 1], slot_in[kAhead + 1], next_slot = 0;
             int next_page = look_up(0, next_slot);
-            for (int i = 0; ok && i < tiles + kAhead; ++i) {
+            for (int i = 0; ok && i < p.n + kAhead; ++i) {
 #pragma unroll
                 for (int k = kAhead; k > 0; --k) page[k] = page[k - 1], slot_in[k] = slot_in[k - 1];
                 page[0] = next_page, slot_in[0] = next_slot;
                 next_page = look_up(i + 1, next_slot);
-#pragma unroll
+#pragma unroll 1
                 for (int which = 0; which < 2; ++which) {
                     const int j = which ? i - kAhead : i;
-                    if (j < 0 || j >= tiles) continue;
-                    Ring &r = which ? vr : kr;
-                    uint64_t *full = which ? &s.v_full[r.at] : &s.k_full[r.at];
+                    if (j < 0 || j >= p.n) continue;
+                    uint64_t *full = which ? &s.v_full[vr.at] : &s.k_full[kr.at], *empty = which ? &s.v_empty[vr.at] : &s.k_empty[kr.at];
                     const int boxes = boxes_of(j);
-                    ok = warp_wait(which ? &s.v_empty[r.at] : &s.k_empty[r.at], r.phase ^ 1, a.status);
+                    ok = warp_wait(empty, (which ? vr.phase : kr.phase) ^ 1, a.status);
                     if (!ok) break;
                     if (lane == 0) {
                         if (boxes) mbar_arrive_expect_tx(full, boxes * a.box_rows * D * 2);
@@ -502,44 +480,43 @@ __device__ __forceinline__ bool load_pieces(const PagedArgs &a, Shared<D, SOLO> 
                     }
                     __syncwarp();
                     if (part < boxes) {
-                        int from = page[which ? kAhead : 0], first_slot = slot_in[which ? kAhead : 0];
+                        int from = which ? page[kAhead] : page[0], first_slot = which ? slot_in[kAhead] : slot_in[0];
                         if (from < 0 || from >= c.n_pages) {                          // (a page behind the pool reads as zeros)
                             from = c.n_pages, first_slot = 0;
                             atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
                         }
                         asm volatile(
                             "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-                                smem_u32((which ? s.v[r.at] : s.k[r.at]) + half * S::kHalf + part * a.box_rows * 128)),
-                            "l"(which ? &vm : &km), "r"(half * 64), "r"(first_slot), "r"(h), "r"(from), "r"(smem_u32(full))
+                                smem_u32((which ? s.v[vr.at] : s.k[kr.at]) + half * S::kHalf + part * a.box_rows * 128)),
+                            "l"(which ? &vm : &km), "r"(half * 64), "r"(first_slot), "r"(p.h), "r"(from), "r"(smem_u32(full))
                             : "memory");
                     }
-                    r.next();
-                    ++held;
+                    if (which) vr.next();
+                    else kr.next();
                 }
             }
             // the next unit
-            x = upto;
-            from += n;
-            if (!ends || x >= end) break;
-            row0 += S::kRows;
-            if (row0 >= rows) {
-                row0 = 0;
-                if (++h == c.Hkv) {
-                    h = 0;
-                    do sequence(a, ++b, q0, fresh, len, start);
-                    while (fresh == 0 && b + 1 < c.B);
+            left -= p.n;
+            skipped = 0;
+            if (!ok || left == 0) break;
+            p.row0 += S::kRows;
+            if (p.row0 >= p.fresh * a.G) {
+                p.row0 = 0;
+                if (++p.h == c.Hkv) {
+                    p.h = 0;
+                    do sequence(a, ++p.b, p.q0, p.fresh, p.len, p.start);
+                    while (p.fresh == 0 && p.b + 1 < c.B);
                 }
             }
-            n = unit_tiles(a, row0, row0 + S::kRows < fresh * a.G ? row0 + S::kRows : fresh * a.G, fresh, len, start, first);
+            p.rows = p.fresh * a.G - p.row0 < S::kRows ? p.fresh * a.G - p.row0 : S::kRows;
         }
     }
-    if (lane == 0) a.cuts[cta] = cut;
     if (ok) ok = warp_wait(&s.piece_empty[pr.at], pr.phase ^ 1, a.status);
     if (ok && lane == 0) {
         s.piece[pr.at].n = 0;
         mbar_arrive(&s.piece_full[pr.at]);
     }
-    if (!ok && held)                     // do not leave while a copy may be in flight
+    if (!ok)                             // do not leave while a copy may be in flight
         for (int i = 0; i < S::kKeys + S::kValues; ++i) {
             Ring &r = i < S::kKeys ? kr : vr;
             if (r.at == 0) r.at = r.n, r.phase ^= 1;
@@ -557,7 +534,7 @@ __device__ __forceinline__ bool multiply_pieces(const PagedArgs &a, Shared<D, SO
     const int lane = threadIdx.x & 31;
     const uint32_t leader = lane == 0;
     Ring kr(S::kKeys), vr(S::kValues), pr(kPieces);
-    uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+    uint32_t q_phase = 0, p_phase = 0;       // (a bit per stream)
     const uint64_t q_at = operand(smem_u32(s.q), 16), k_at = operand(smem_u32(s.k), 16), v_at = operand(smem_u32(s.v), S::kHalf);
     const auto scores = [&](int i) {         // stream i's next tile of keys, which has arrived
         const uint64_t q = q_at + (SOLO ? 0 : i * (S::kBytes >> 4)), keys = k_at + kr.at * (S::kBytes >> 4);
@@ -577,25 +554,27 @@ __device__ __forceinline__ bool multiply_pieces(const PagedArgs &a, Shared<D, SO
     const auto release = [&](uint64_t *bar) { mma_commit(leader, bar); };
     for (;;) {
         if (!warp_wait(&s.piece_full[pr.at], pr.phase, a.status)) return false;
-        const Piece p = s.piece[pr.at];
+        const int tiles = s.piece[pr.at].n, rows = s.piece[pr.at].rows, held = s.piece[pr.at].len - s.piece[pr.at].j0 * kTile;
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.piece_empty[pr.at]);
         pr.next();
-        if (p.n == 0) return true;
-        const int streams = SOLO ? (p.n > 1 ? 2 : 1) : (p.rows > kTile ? 2 : 1);
+        if (tiles == 0) return true;
+        const int streams = SOLO ? (tiles > 1 ? 2 : 1) : (rows > kTile ? 2 : 1);
+#pragma unroll 1
         for (int i = 0; i < (SOLO ? 1 : streams); ++i) {
-            if (!warp_wait(&s.q_full[i], q_phase[i], a.status)) return false;
-            q_phase[i] ^= 1;
+            if (!warp_wait(&s.q_full[i], q_phase >> i & 1, a.status)) return false;
+            q_phase ^= 1u << i;
         }
+#pragma unroll 1
         for (int i = 0; i < streams; ++i) {
             if ((SOLO || i == 0) && !warp_wait(&s.k_full[kr.at], kr.phase, a.status)) return false;
             tmem_fence_after();
             scores(i);
             if (SOLO || i == streams - 1) release(&s.k_empty[kr.at]), kr.next();
         }
-        for (int t = 0; t < p.n; ++t) {
+        for (int t = 0; t < tiles; ++t) {
             if (!warp_wait(&s.v_full[vr.at], vr.phase, a.status)) return false;
-            const int valid = p.len - (p.j0 + t) * kTile;
+            const int valid = held - t * kTile;
             if (valid < kTile) {             // rows behind the sequence's end are cleared
                 for (int x = (valid > 0 ? valid : 0) * (D / 8) + lane; x < kTile * (D / 8); x += 32) {
                     const int row = x / (D / 8), col = x - row * (D / 8);
@@ -605,14 +584,15 @@ __device__ __forceinline__ bool multiply_pieces(const PagedArgs &a, Shared<D, SO
                 __syncwarp();
             }
             const int last = t + (SOLO ? 2 : 1);          // the tile whose scores follow
+            if (last < tiles && !warp_wait(&s.k_full[kr.at], kr.phase, a.status)) return false;
+#pragma unroll 1
             for (int i = SOLO ? (t & 1) : 0; i < (SOLO ? (t & 1) + 1 : streams); ++i) {
-                if (!warp_wait(&s.p_full[i], p_phase[i], a.status)) return false;
-                p_phase[i] ^= 1;
+                if (!warp_wait(&s.p_full[i], p_phase >> i & 1, a.status)) return false;
+                p_phase ^= 1u << i;
                 tmem_fence_after();
                 output(i, t >= (SOLO ? 2 : 1));
                 if (SOLO || i == streams - 1) release(&s.v_empty[vr.at]), vr.next();
-                if (last < p.n) {
-                    if ((SOLO || i == 0) && !warp_wait(&s.k_full[kr.at], kr.phase, a.status)) return false;
+                if (last < tiles) {
                     scores(i);
                     if (SOLO || i == streams - 1) release(&s.k_empty[kr.at]), kr.next();
                 } else {
@@ -712,16 +692,9 @@ __device__ __forceinline__ bool soften_pieces(const PagedArgs &a, Shared<D, SOLO
                 }
                 const float base = m == -INFINITY ? 0.f : m * c;
                 const Two c2 = two(c, c), base2 = two(-base, -base);
-                // (the polynomial's smallest power is 2**-126, not 0: not where positions may be hidden)
-                const bool plain = warp_lo > j || warp_hi < j + kTile || __any_sync(kFull, m == -INFINITY);
                 Two sum[2] = {two(0.f, 0.f), two(0.f, 0.f)};
-                if (plain) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) weigh<T, 0>(x[k], c2, base2, sum, s_at + 16 * k);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) weigh<T, kByPolynomial>(x[k], c2, base2, sum, s_at + 16 * k);
-                }
+                for (int k = 0; k < 4; ++k) weigh<T>(x[k], c2, base2, sum, s_at + 16 * k);
                 float sums[4];
                 parts(sum[0], sums[0], sums[1]), parts(sum[1], sums[2], sums[3]);
                 l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
