@@ -7,8 +7,8 @@
 // partial results (numerator, maximum, sum per row) that a second kernel merges.  Lengths lie on the device: every
 // CTA finds its run by itself.
 //
-// One CTA: warp 9 finds the pieces and loads (one tensor copy per page and 64 columns), warp 8 issues the products of both streams (a warp
-// for each made them interleave, and took a third longer), two warpgroups do the softmax, one row per thread.  S = Q K^T goes to TMEM, the weights go back to where S was, and
+// One CTA: warp 9 finds the pieces and loads the keys, warp 10 the values (one tensor copy per page and 64 columns), warp 8 issues the products
+// of both streams (a warp for each made them interleave, and took a third longer), two warpgroups do the softmax, one row per thread.  S = Q K^T goes to TMEM, the weights go back to where S was, and
 // O += P V takes them from there.  Two streams of S, P and O let one's softmax run while the other's products do:
 //   PAIR  a unit has 256 rows, stream i the rows 128 i ..; every tile is used by both.
 //   SOLO  a unit has 128 rows; stream i takes every second tile, and the two meet at the end of the piece.  For few rows, where
@@ -57,7 +57,7 @@ struct PagedArgs {
     uint32_t negate;
     int box_rows;             // rows per tensor copy
     int room;                 // positions that the table has
-    Quotient by_page;
+    Quotient by_page, by_group;
     float *part_o, *part_ml;  // [2 CTAs][rows][D], [2 CTAs][rows][2]
     struct Cut *cuts;         // [CTAs]
     int32_t *status;
@@ -239,8 +239,8 @@ __device__ __forceinline__ void seen_by(const PagedArgs &a, int t, int fresh, in
 // Tiles of the unit of rows row0 .. row1 - 1 (one, of hidden positions, if it sees none).
 __device__ __forceinline__ int unit_tiles(const PagedArgs &a, int row0, int row1, int fresh, int len, int start, int &first) {
     int lo, hi, other;
-    seen_by(a, row0 / a.G, fresh, len, start, lo, other);
-    seen_by(a, (row1 - 1) / a.G, fresh, len, start, other, hi);
+    seen_by(a, (uint32_t)row0 / a.by_group, fresh, len, start, lo, other);
+    seen_by(a, (uint32_t)(row1 - 1) / a.by_group, fresh, len, start, other, hi);
     first = lo / kTile;
     const int n = (hi > 0 ? (hi - 1) / kTile + 1 : 0) - first;
     if (n <= 0) first = 0;
@@ -366,7 +366,16 @@ struct Ring {
     __device__ __forceinline__ void next() {
         if (++at == n) at = 0, phase ^= 1;
     }
+    __device__ __forceinline__ void back() {
+        if (at == 0) at = n, phase ^= 1;
+        --at;
+    }
 };
+
+// a x / n, where a < n
+__device__ __forceinline__ uint32_t share_of(uint32_t x, uint32_t a, uint32_t n) {
+    return x < 1u << 22 && n < 1u << 10 ? x * a / n : (uint32_t)((uint64_t)x * a / n);
+}
 
 // Finds where the run of CTA `cta` begins: the unit (its row0, sequence and head in `p`) and how many of its tiles come before.  Returns the run's
 // length; `ctas`: how many CTAs have runs (no CTA between two of a unit goes without a tile), `total`: all tiles.
@@ -374,17 +383,18 @@ template <int ROWS>
 __device__ __forceinline__ int find_run(const PagedArgs &a, int cta, Piece &p, int &skipped, int &ctas, uint32_t &total) {
     const adacode_paged_cache &c = a.cache;
     const int lane = threadIdx.x & 31;
-    uint32_t mine = 0;
-    for (int b = lane; b < c.B; b += 32) mine += head_tiles<ROWS>(a, b);
+    const uint32_t mine = lane < c.B ? head_tiles<ROWS>(a, lane) : 0;
+    total = mine;
+    for (int b = lane + 32; b < c.B; b += 32) total += head_tiles<ROWS>(a, b);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(kFull, mine, d);
-    total = mine * c.Hkv;
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(kFull, total, d);
+    total *= c.Hkv;
     ctas = total < gridDim.x ? (int)total : (int)gridDim.x;
     if (cta >= ctas) return 0;
-    const uint32_t x = (uint32_t)((uint64_t)total * cta / ctas), end = (uint32_t)((uint64_t)total * (cta + 1) / ctas);
+    const uint32_t x = share_of(total, cta, ctas), end = share_of(total, cta + 1, ctas);
     uint32_t from = 0, per_head = 0;
     for (int b0 = 0;; b0 += 32) {
-        const uint32_t w = b0 + lane < c.B ? head_tiles<ROWS>(a, b0 + lane) : 0;
+        const uint32_t w = b0 == 0 ? mine : b0 + lane < c.B ? head_tiles<ROWS>(a, b0 + lane) : 0;
         const uint32_t upto = from + warp_scan(w * c.Hkv);
         const unsigned later = __ballot_sync(kFull, upto > x);
         if (later || b0 + 32 >= c.B) {
@@ -409,121 +419,141 @@ __device__ __forceinline__ int find_run(const PagedArgs &a, int cta, Piece &p, i
     return (int)(end - x);
 }
 
-// Loads: one lane per page and 64 columns of a tile.
+// Loads the keys or the values of a piece.  Lane i has the i-th page (of box_rows slots) of a tile; the table is read one tile ahead, so that its
+// latency hides behind the copies.  One lane issues all of them, by a predicate: each lane its own took a hundred cycles per copy, 5000 for a tile
+// of pages of 16.
+template <int D, int STAGES>
+__device__ __forceinline__ bool load_tiles(const PagedArgs &a, const Piece &p, const CUtensorMap &map, Ring &r, uint8_t (*stage)[kTile * D * 2],
+                                           uint64_t *full, uint64_t *empty) {
+    const adacode_paged_cache &c = a.cache;
+    const int lane = threadIdx.x & 31;
+    const uint32_t leader = lane == 0;
+    const int tiles = p.n, h = p.h, held = p.len - p.j0 * kTile, at0 = p.j0 * kTile + lane * a.box_rows;
+    const int32_t *table = c.block_table + p.b * c.table_stride;
+    const auto boxes_of = [&](int j) {                        // pages of tile j that hold tokens
+        const int valid = held - j * kTile;
+        return j >= tiles || valid <= 0 ? 0 : valid >= kTile ? kTile / a.box_rows : (valid + a.box_rows - 1) / a.box_rows;
+    };
+    int next_boxes = boxes_of(0), next_page = -1, next_slot = 0;
+    const auto look_up = [&](int j) {
+        if (lane < next_boxes) {
+            const int at = at0 + j * kTile, entry = (int)((uint32_t)at / a.by_page);
+            next_slot = at - entry * c.page_size;
+            next_page = entry < c.table_width ? table[entry] : -1;
+        }
+    };
+    look_up(0);
+    for (int j = 0; j < tiles; ++j) {
+        const int boxes = next_boxes;
+        int page = next_page, slot = next_slot;
+        if (lane < boxes && (page < 0 || page >= c.n_pages)) {        // (a page behind the pool reads as zeros)
+            page = c.n_pages, slot = 0;
+            atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
+        }
+        next_boxes = boxes_of(j + 1);
+        look_up(j + 1);
+        if (!warp_wait(&empty[r.at], r.phase ^ 1, a.status)) return false;
+        const uint32_t bar = smem_u32(&full[r.at]), to = smem_u32(stage[r.at]);
+        if (leader) {
+            if (boxes) mbar_arrive_expect_tx(&full[r.at], boxes * a.box_rows * D * 2);
+            else mbar_arrive(&full[r.at]);
+        }
+        __syncwarp();
+        {
+            const int i = lane / (D / 64), half = lane % (D / 64);
+            const int from = __shfl_sync(kFull, page, i), first = __shfl_sync(kFull, slot, i);
+            if (i < boxes)
+                    asm volatile(
+                        "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+                            to + half * (kTile * 128) + i * a.box_rows * 128),
+                        "l"(&map), "r"(half * 64), "r"(first), "r"(h), "r"(from), "r"(bar)
+                        : "memory");
+        }
+        r.next();
+    }
+    return true;
+}
+// Given up: do not leave while a copy may be in flight.
+template <int STAGES>
+__device__ __forceinline__ void drain(Ring &r, uint64_t *full, int32_t *status) {
+    for (int i = 0; i < STAGES; ++i) {
+        r.back();
+        mbar_wait(&full[r.at], r.phase, status, 1u << 16);
+    }
+}
+
+// Finds the pieces and loads the keys.
 template <int D, bool SOLO>
-__device__ __forceinline__ bool load_pieces(const PagedArgs &a, Shared<D, SOLO> &s, const CUtensorMap &km, const CUtensorMap &vm) {
+__device__ __forceinline__ void load_keys(const PagedArgs &a, Shared<D, SOLO> &s, const CUtensorMap &map) {
     using S = Shape<D, SOLO>;
     const adacode_paged_cache &c = a.cache;
     const int lane = threadIdx.x & 31;
-    Ring kr(S::kKeys), vr(S::kValues), pr(kPieces);
+    Ring r(S::kKeys), pr(kPieces);
     bool ok = true;
-    if (lane == 0) a.cuts[blockIdx.x].n = 0;
-    {
-        Piece p;
-        int skipped = 0, ctas;
-        uint32_t total;
-        int left = find_run<S::kRows>(a, blockIdx.x, p, skipped, ctas, total);
-        while (left > 0) {
-            // the next piece
-            int first;
-            const int all = unit_tiles(a, p.row0, p.row0 + p.rows, p.fresh, p.len, p.start, first);
-            const bool whole = all - skipped <= left;
-            p.j0 = first + skipped;
-            p.n = whole ? all - skipped : left;
-            p.slot = skipped > 0 ? 2 * blockIdx.x : whole ? -1 : 2 * blockIdx.x + 1;
-            ok = warp_wait(&s.piece_empty[pr.at], pr.phase ^ 1, a.status);
-            if (!ok) break;
-            if (lane == 0) {
-                if (skipped == 0 && !whole) {
-                    // CTA of the unit's last tile (which is left - all tiles behind this run's end)
-                    const uint32_t end = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / ctas);
-                    const int last = (int)(((uint64_t)(end + (all - left)) * ctas - 1) / total);
-                    a.cuts[blockIdx.x] = {last - (int)blockIdx.x + 1, p.rows, p.row0, p.b, p.h, p.q0, p.fresh, p.len, p.start};
-                }
-                s.piece[pr.at] = p;
-                mbar_arrive(&s.piece_full[pr.at]);
-                if (p.len > a.room) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
-            }
-            pr.next();
-            // Keys of a tile come one tile (SOLO: two) before its values.  A lane has one page (of box_rows slots) and 64 columns; the table is
-            // read one tile ahead, so that its latency hides behind the copies.
-            constexpr int kAhead = SOLO ? 2 : 1;
-            const int part = lane / (D / 64), half = lane - part * (D / 64);
-            const auto boxes_of = [&](int j) {                                        // pages of tile j that hold tokens
-                const int valid = p.len - (p.j0 + j) * kTile;
-                return j >= p.n || valid <= 0 ? 0 : valid >= kTile ? kTile / a.box_rows : (valid + a.box_rows - 1) / a.box_rows;
-            };
-            const auto look_up = [&](int j, int &slot_in) {
-                if (part >= boxes_of(j)) return -1;
-                const int at = (p.j0 + j) * kTile + part * a.box_rows, entry = (int)((uint32_t)at / a.by_page);
-                slot_in = at - entry * c.page_size;
-                return entry < c.table_width ? c.block_table[p.b * c.table_stride + entry] : -1;
-            };
-            int page[kAhead + 1], slot_in[kAhead + 1], next_slot = 0;
-            int next_page = look_up(0, next_slot);
-            for (int i = 0; ok && i < p.n + kAhead; ++i) {
-#pragma unroll
-                for (int k = kAhead; k > 0; --k) page[k] = page[k - 1], slot_in[k] = slot_in[k - 1];
-                page[0] = next_page, slot_in[0] = next_slot;
-                next_page = look_up(i + 1, next_slot);
-#pragma unroll 1
-                for (int which = 0; which < 2; ++which) {
-                    const int j = which ? i - kAhead : i;
-                    if (j < 0 || j >= p.n) continue;
-                    uint64_t *full = which ? &s.v_full[vr.at] : &s.k_full[kr.at], *empty = which ? &s.v_empty[vr.at] : &s.k_empty[kr.at];
-                    const int boxes = boxes_of(j);
-                    ok = warp_wait(empty, (which ? vr.phase : kr.phase) ^ 1, a.status);
-                    if (!ok) break;
-                    if (lane == 0) {
-                        if (boxes) mbar_arrive_expect_tx(full, boxes * a.box_rows * D * 2);
-                        else mbar_arrive(full);
-                    }
-                    __syncwarp();
-                    if (part < boxes) {
-                        int from = which ? page[kAhead] : page[0], first_slot = which ? slot_in[kAhead] : slot_in[0];
-                        if (from < 0 || from >= c.n_pages) {                          // (a page behind the pool reads as zeros)
-                            from = c.n_pages, first_slot = 0;
-                            atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
-                        }
-                        asm volatile(
-                            "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-                                smem_u32((which ? s.v[vr.at] : s.k[kr.at]) + half * S::kHalf + part * a.box_rows * 128)),
-                            "l"(which ? &vm : &km), "r"(half * 64), "r"(first_slot), "r"(p.h), "r"(from), "r"(smem_u32(full))
-                            : "memory");
-                    }
-                    if (which) vr.next();
-                    else kr.next();
-                }
-            }
-            // the next unit
-            left -= p.n;
-            skipped = 0;
-            if (!ok || left == 0) break;
-            p.row0 += S::kRows;
-            if (p.row0 >= p.fresh * a.G) {
-                p.row0 = 0;
-                if (++p.h == c.Hkv) {
-                    p.h = 0;
-                    do sequence(a, ++p.b, p.q0, p.fresh, p.len, p.start);
-                    while (p.fresh == 0 && p.b + 1 < c.B);
-                }
-            }
-            p.rows = p.fresh * a.G - p.row0 < S::kRows ? p.fresh * a.G - p.row0 : S::kRows;
+    Piece p;
+    int skipped = 0, ctas;
+    uint32_t total;
+    int left = find_run<S::kRows>(a, blockIdx.x, p, skipped, ctas, total);
+    Cut cut;
+    cut.n = 0;
+    while (left > 0) {
+        int first;
+        const int all = unit_tiles(a, p.row0, p.row0 + p.rows, p.fresh, p.len, p.start, first);
+        const bool whole = all - skipped <= left;
+        p.j0 = first + skipped;
+        p.n = whole ? all - skipped : left;
+        p.slot = skipped > 0 ? 2 * blockIdx.x : whole ? -1 : 2 * blockIdx.x + 1;
+        ok = warp_wait(&s.piece_empty[pr.at], pr.phase ^ 1, a.status);
+        if (!ok) break;
+        if (lane == 0) {
+            s.piece[pr.at] = p;
+            mbar_arrive(&s.piece_full[pr.at]);
         }
+        pr.next();
+        ok = load_tiles<D, S::kKeys>(a, p, map, r, s.k, s.k_full, s.k_empty);
+        if (p.len > a.room && lane == 0) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
+        if (!ok) break;
+        left -= p.n;
+        if (skipped == 0 && !whole) {
+            // the unit goes on behind this run: its last tile is all - p.n tiles further on
+            const uint32_t end = share_of(total, blockIdx.x + 1, ctas);
+            const int last = (int)(((uint64_t)(end + (all - p.n)) * ctas - 1) / total);
+            cut = {last - (int)blockIdx.x + 1, p.rows, p.row0, p.b, p.h, p.q0, p.fresh, p.len, p.start};
+        }
+        skipped = 0;
+        if (left == 0) break;
+        p.row0 += S::kRows;
+        if (p.row0 >= p.fresh * a.G) {
+            p.row0 = 0;
+            if (++p.h == c.Hkv) {
+                p.h = 0;
+                do sequence(a, ++p.b, p.q0, p.fresh, p.len, p.start);
+                while (p.fresh == 0 && p.b + 1 < c.B);
+            }
+        }
+        p.rows = p.fresh * a.G - p.row0 < S::kRows ? p.fresh * a.G - p.row0 : S::kRows;
     }
+    if (lane == 0) a.cuts[blockIdx.x] = cut;
     if (ok) ok = warp_wait(&s.piece_empty[pr.at], pr.phase ^ 1, a.status);
     if (ok && lane == 0) {
         s.piece[pr.at].n = 0;
         mbar_arrive(&s.piece_full[pr.at]);
     }
-    if (!ok)                             // do not leave while a copy may be in flight
-        for (int i = 0; i < S::kKeys + S::kValues; ++i) {
-            Ring &r = i < S::kKeys ? kr : vr;
-            if (r.at == 0) r.at = r.n, r.phase ^= 1;
-            --r.at;
-            mbar_wait(i < S::kKeys ? &s.k_full[r.at] : &s.v_full[r.at], r.phase, a.status, 1u << 16);
-        }
-    return ok;
+    if (!ok) drain<S::kKeys>(r, s.k_full, a.status);
+}
+template <int D, bool SOLO>
+__device__ __forceinline__ void load_values(const PagedArgs &a, Shared<D, SOLO> &s, const CUtensorMap &map) {
+    using S = Shape<D, SOLO>;
+    Ring r(S::kValues), pr(kPieces);
+    for (;;) {
+        if (!warp_wait(&s.piece_full[pr.at], pr.phase, a.status)) break;
+        if (s.piece[pr.at].n == 0) return;
+        if (!load_tiles<D, S::kValues>(a, s.piece[pr.at], map, r, s.v, s.v_full, s.v_empty)) break;
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&s.piece_empty[pr.at]);
+        pr.next();
+    }
+    drain<S::kValues>(r, s.v_full, a.status);
 }
 
 // Products.
@@ -622,7 +652,7 @@ __device__ __forceinline__ bool soften_pieces(const PagedArgs &a, Shared<D, SOLO
         const int row = (SOLO ? 0 : stream * kTile) + r;      // within the unit
         const bool mine = row < p.rows;
         if (!SOLO && p.rows <= stream * kTile) continue;
-        const int t = (p.row0 + row) / a.G, head = p.h * a.G + p.row0 + row - t * a.G;
+        const int t = (int)((uint32_t)(p.row0 + row) / a.by_group), head = p.h * a.G + p.row0 + row - t * a.G;
         int lo = 0, hi = INT32_MAX;
         if (mine) seen_by(a, t, p.fresh, p.len, p.start, lo, hi);
         // queries (of SOLO, half of the columns per warpgroup)
@@ -808,7 +838,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) k_paged_attn(const __grid_con
         for (int i = 0; i < S::kKeys; ++i) mbar_init(&s.k_full[i], 1), mbar_init(&s.k_empty[i], 1);
         for (int i = 0; i < S::kValues; ++i) mbar_init(&s.v_full[i], 1), mbar_init(&s.v_empty[i], 1);
         for (int i = 0; i < 2; ++i) mbar_init(&s.q_full[i], SOLO ? 8 : 4), mbar_init(&s.s_full[i], 1), mbar_init(&s.p_full[i], 4), mbar_init(&s.o_full[i], 1);
-        for (int i = 0; i < kPieces; ++i) mbar_init(&s.piece_full[i], 1), mbar_init(&s.piece_empty[i], 9);
+        for (int i = 0; i < kPieces; ++i) mbar_init(&s.piece_full[i], 1), mbar_init(&s.piece_empty[i], 8 + 2);
         mbar_init(&s.sums, 8), mbar_init(&s.read, 8), mbar_init(&s.done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -823,7 +853,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1) k_paged_attn(const __grid_con
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
         if (warp == 9) {
-            load_pieces<D, SOLO>(a, s, keys, values);
+            load_keys<D, SOLO>(a, s, keys);
+        } else if (warp == 10) {
+            load_values<D, SOLO>(a, s, values);
         } else if (warp == 8 && !multiply_pieces<T, D, SOLO>(a, s, tmem)) {
             // (given up: products may still be running)
             mma_commit((threadIdx.x & 31) == 0, &s.done);
@@ -854,6 +886,7 @@ __global__ void __launch_bounds__(256) k_paged_merge(const __grid_constant__ Pag
     float l = 0.f, o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 4
     for (int i = 0; i < cut.n; ++i) {
         const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + piece(i) * 2);
         if (ml.x == -INFINITY) {
@@ -878,7 +911,7 @@ __global__ void __launch_bounds__(256) k_paged_merge(const __grid_constant__ Pag
         repair_row<T, D>(a, cut.b, cut.h, cut.q0, cut.fresh, cut.len, cut.start, cut.row0 + row, 0, D);
         return;
     }
-    const int t = (cut.row0 + row) / a.G, head = cut.h * a.G + cut.row0 + row - t * a.G;
+    const int t = (int)((uint32_t)(cut.row0 + row) / a.by_group), head = cut.h * a.G + cut.row0 + row - t * a.G;
     T *out = reinterpret_cast<T *>(a.out) + (long long)(cut.q0 + t) * a.o_n + head * a.o_h + lane * E;
     const float share = l == 0.f ? 0.f : 1.f / l;
     uint32_t w[E / 2];
@@ -1010,7 +1043,7 @@ int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int6
     a.part_o = (float *)workspace, a.part_ml = a.part_o + rows * D, a.cuts = (Cut *)(a.part_ml + rows * 2);
     const long long room = (long long)cache->table_width * cache->page_size;
     a.room = room < 1 << 30 ? (int)room : 1 << 30;
-    a.by_page = quotient_by(cache->page_size);
+    a.by_page = quotient_by(cache->page_size), a.by_group = quotient_by(G);
     a.status = status;
     CUtensorMap keys, values;
     if (!map_pages(keys, cache->key_pages, *cache, cache->key_page, cache->key_head, cache->key_slot, a.box_rows) ||
