@@ -179,7 +179,8 @@ def lib() -> ctypes.CDLL:
     L.adacode_paged_attn.restype = i32
     L.adacode_paged_attn.argtypes = [vp, vp, i64, i64, i32, vp, i64, i64, vp, i32, ctypes.c_float, i32, i32, vp, sz, vp, vp]
     L.adacode_sample_tokens.restype = i32
-    L.adacode_sample_tokens.argtypes = [vp, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp]
+    f32 = ctypes.c_float
+    L.adacode_sample_tokens.argtypes = [vp, i64, i32, i32, i32, vp, vp, f32, vp, i32, vp, f32, vp, f32, vp, vp]
     _lib = L
     return L
 

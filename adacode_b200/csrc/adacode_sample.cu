@@ -42,6 +42,8 @@ struct SampleArgs {
     const float *uniforms, *temperature, *top_p, *min_p;
     const int32_t *top_k;
     int64_t *tokens;
+    float temperature_all, top_p_all, min_p_all;
+    int top_k_all;
 };
 
 __device__ __forceinline__ float widen(float v) { return v; }
@@ -163,7 +165,7 @@ __device__ void sort_places(uint64_t *list, int n) {
 
 // The smallest weight that stays; the largest weight, 1, always does.
 __device__ __forceinline__ double least_of(const SampleArgs &a, int row) {
-    const float p = a.min_p ? a.min_p[row] : 0.f;
+    const float p = a.min_p ? a.min_p[row] : a.min_p_all;
     return p > 0.f ? fminf(p, 1.f) : 0.f;
 }
 
@@ -191,7 +193,7 @@ __device__ void sample_slowly(const SampleArgs &a, Shared &s, const T *x, int ro
     unsigned long long *s_u = reinterpret_cast<unsigned long long *>(s.best);
     uint32_t cut = 1;
     long long ties = V;
-    const int k = a.top_k ? a.top_k[row] : 0;
+    const int k = a.top_k ? a.top_k[row] : a.top_k_all;
     if (k > 0 && k < V) {
         // the largest key that at least k tokens reach
         uint32_t lo = 1, hi = top;
@@ -207,7 +209,7 @@ __device__ void sample_slowly(const SampleArgs &a, Shared &s, const T *x, int ro
         cut = lo;
         ties = k - above;
     }
-    const float p = a.top_p ? a.top_p[row] : 1.f;
+    const float p = a.top_p ? a.top_p[row] : a.top_p_all;
     if (p < 1.f) {
         const auto total = [&](uint32_t from) {           // weight of the tokens of keys from `from` on, inside the cut
             double w = 0.0;
@@ -311,7 +313,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
     cluster.sync();
     uint64_t best = 0;
     for (int r = 0; r < ctas; ++r) best = Most()(best, cluster.map_shared_rank(&s, r)->cta_best);
-    const float t = a.temperature[row];
+    const float t = a.temperature ? a.temperature[row] : a.temperature_all;
     if (best == 0 || !(t > 0.f)) {
         if (rank == 0 && tid == 0) a.tokens[row] = best == 0 ? -1 : token_of(best);
         cluster.sync();
@@ -319,8 +321,8 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
     }
     const float top = value_of((uint32_t)(best >> 32));
     const double largest = top, scale = 1.4426950408889634074 / (double)t, least = least_of(a, row);
-    const int k = a.top_k ? a.top_k[row] : 0;
-    const float p = a.top_p ? a.top_p[row] : 1.f;
+    const int k = a.top_k ? a.top_k[row] : a.top_k_all;
+    const float p = a.top_p ? a.top_p[row] : a.top_p_all;
     const bool use_k = k > 0 && k < V, use_p = p < 1.f;
     bool slow = use_k && k > kMostK;
 
@@ -668,15 +670,15 @@ cudaError_t launch(const SampleArgs &a, int B, int ctas, cudaStream_t st) {
 }  // namespace
 
 extern "C" int adacode_sample_tokens(const void *logits, int64_t row_stride, int dtype, int B, int V, const float *uniforms,
-                                     const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
-                                     int64_t *tokens, void *stream) {
-    if (B < 0 || V <= 0 || (B > 0 && (!logits || !uniforms || !temperature || !tokens))) return ADACODE_ERR_INVALID_ARG;
+                                     const float *temperature, float temperature_all, const int32_t *top_k, int top_k_all, const float *top_p,
+                                     float top_p_all, const float *min_p, float min_p_all, int64_t *tokens, void *stream) {
+    if (B < 0 || V <= 0 || (B > 0 && (!logits || !uniforms || !tokens))) return ADACODE_ERR_INVALID_ARG;
     if (dtype != ADACODE_BF16 && dtype != ADACODE_FP16 && dtype != ADACODE_FP32) return ADACODE_ERR_INVALID_ARG;
     if (V > 1 << 30 || B > 1 << 27) return ADACODE_ERR_TOO_LARGE;
     if (B == 0) return ADACODE_OK;
     const int size = dtype == ADACODE_FP32 ? 4 : 2;
     const bool wide = ((uintptr_t)logits & 15) == 0 && (row_stride * size) % 16 == 0;
-    const SampleArgs a{logits, row_stride, V, wide, uniforms, temperature, top_p, min_p, top_k, tokens};
+    const SampleArgs a{logits, row_stride, V, wide, uniforms, temperature, top_p, min_p, top_k, tokens, temperature_all, top_p_all, min_p_all, top_k_all};
     // As many CTAs per row as keep the GPU's 148 SMs busy, three on each, and leave every warp a step or more of the vocabulary.
     int ctas = 1;
     while (ctas < kMostCtas && (int64_t)B * ctas < 2 * 148 && V > 2 * ctas * kWarps * kStep / 2) ctas *= 2;

@@ -398,7 +398,226 @@ PyObject *dense_view(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// An argument of the paged operators and of the sampler: a tensor (None where it may be left out) that is what torch makes it look like, on
+// one GPU with the others, and that no gradient is asked of.
+struct Arg {
+    const Tensor *t = nullptr;
+    bool given() const { return t != nullptr; }
+    const Tensor *operator->() const { return t; }
+    const void *at() const { return t ? t->const_data_ptr() : nullptr; }
+    int64_t stride(int d) const { return t ? t->stride(d) : 0; }
+};
+struct Args {
+    bool ok = !at::impl::torch_function_mode_enabled() && !torch::autograd::ForwardADLevel::try_get_by_idx(0);
+    const Tensor *device_of = nullptr;
+    Arg take(PyObject *o, bool optional = false, bool to_write = false) {
+        Arg a;
+        if (o == Py_None && optional) return a;
+        constexpr auto wrappers = c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                                       c10::DispatchKey::Functionalize, c10::DispatchKey::Python,
+                                                       c10::DispatchKey::Conjugate, c10::DispatchKey::Negative});
+        if (!ok || !THPVariable_CheckExact(o)) {
+            ok = false;
+            return a;
+        }
+        const Tensor &t = THPVariable_Unpack(o);
+        if (!device_of) device_of = &t;
+        ok = t.is_cuda() && t.layout() == at::kStrided && t.device() == device_of->device() && !t.key_set().has_any(wrappers) &&
+             !(c10::GradMode::is_enabled() && t.requires_grad()) && !(to_write && t.is_inference() && !c10::InferenceMode::is_enabled());
+        a.t = &t;
+        return a;
+    }
+};
+bool whole_number(PyObject *o, int64_t lo, int64_t hi, int64_t &v) {
+    if (!PyLong_Check(o)) return false;
+    int over = 0;
+    v = PyLong_AsLongLongAndOverflow(o, &over);
+    return !over && v >= lo && v <= hi;
+}
+bool is_shape(const Arg &a, at::IntArrayRef shape) { return a->sizes() == shape; }
+int element_type(const Tensor &t) {
+    switch (t.scalar_type()) {
+        case at::kBFloat16: return ADACODE_BF16;
+        case at::kHalf: return ADACODE_FP16;
+        case at::kFloat: return ADACODE_FP32;
+        default: return -1;
+    }
+}
+void count_write(const Tensor &t) {
+    if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+
+// The checked cache of a call with N new tokens (what paged._describe_cache refuses, this does too).
+bool describe_cache(const Arg &keys, const Arg &values, const Arg &table, const Arg &lens, const Arg &cu, int64_t N, adacode_paged_cache &c) {
+    if (keys->dim() != 4 || values->sizes() != keys->sizes() || table->dim() != 2 || table->scalar_type() != at::kInt || lens->scalar_type() != at::kInt)
+        return false;
+    const int type = element_type(*keys.t);
+    if ((type != ADACODE_BF16 && type != ADACODE_FP16) || values->scalar_type() != keys->scalar_type()) return false;
+    const int64_t P = keys->size(0), H = keys->size(1), page = keys->size(2), D = keys->size(3), B = table->size(0), W = table->size(1);
+    constexpr int64_t kMost = INT32_MAX;
+    if (B <= 0 || W <= 0 || keys->numel() == 0 || P >= kMost || H > kMost || page > kMost || B > kMost || W > kMost || N > kMost) return false;
+    if (D > 1 && (keys->stride(3) != 1 || values->stride(3) != 1)) return false;
+    if ((W > 1 && table->stride(1) != 1) || !is_shape(lens, {B}) || !lens->is_contiguous()) return false;
+    if (cu.given() ? cu->scalar_type() != at::kInt || !is_shape(cu, {B + 1}) || !cu->is_contiguous() : N % B != 0) return false;
+    c = {const_cast<void *>(keys.at()), const_cast<void *>(values.at()), keys.stride(0), keys.stride(1), keys.stride(2), values.stride(0), values.stride(1),
+         values.stride(2), (const int32_t *)table.at(), table.stride(0), (const int32_t *)lens.at(), (const int32_t *)cu.at(),
+         (int32_t)W, (int32_t)B, (int32_t)P, (int32_t)page, (int32_t)H, (int32_t)D, type, (int32_t)N};
+    return true;
+}
+// queries, keys, values or an output of N tokens
+bool is_states(const Arg &a, int64_t N, int64_t heads, const Arg &pages) {
+    const int64_t D = pages->size(3);
+    return a->scalar_type() == pages->scalar_type() && is_shape(a, {N, heads, D}) && (D == 1 || a->stride(2) == 1);
+}
+bool on_sixteen_bytes(const Arg &a) {
+    if ((uintptr_t)a.at() & 15) return false;
+    for (int d = 0; d + 1 < a->dim(); ++d)
+        if (a->size(d) > 1 && (a->stride(d) & 7)) return false;
+    return true;
+}
+
+// append_rotary(key, value, cos, sin, key_pages, value_pages, block_table, seq_lens, query, cu_seqlens, sections, interleaved, out, status)
+//   -> what adacode_b200.append_rotary returns, or False, and nothing done, where it has to look closer
+PyObject *append_rotary(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n_args == 14, "append_rotary: arguments");
+    Args in;
+    const Arg keys = in.take(args[4], false, true), values = in.take(args[5], false, true), key = in.take(args[0]), value = in.take(args[1]),
+              cos = in.take(args[2]), sin = in.take(args[3]), table = in.take(args[6]), lens = in.take(args[7]), query = in.take(args[8], true),
+              cu = in.take(args[9], true), given = in.take(args[12], true, true), status = in.take(args[13], false, true);
+    if (!in.ok || key->dim() != 3) Py_RETURN_FALSE;
+    const int64_t N = key->size(0);
+    adacode_paged_cache c;
+    if (!describe_cache(keys, values, table, lens, cu, N, c) || !is_states(key, N, c.Hkv, keys) || !is_states(value, N, c.Hkv, keys)) Py_RETURN_FALSE;
+    if (c.D % 2 != 0 || c.D > 512) Py_RETURN_FALSE;
+    const int type = element_type(*cos.t);
+    if (sin->sizes() != cos->sizes() || sin->strides() != cos->strides() || sin->scalar_type() != cos->scalar_type() || (type != ADACODE_FP32 && type != c.dtype) ||
+        (cos->dim() != 2 && cos->dim() != 3))
+        Py_RETURN_FALSE;
+    const int a0 = cos->dim() - 2;
+    adacode_rotary r = {};
+    const int64_t axes = a0 ? cos->size(0) : 1, half = cos->size(a0 + 1);
+    if (axes < 1 || axes > 4 || cos->size(a0) != N || 2 * half > c.D || (half > 1 && cos->stride(a0 + 1) != 1)) Py_RETURN_FALSE;
+    r.cos = cos.at(), r.sin = sin.at(), r.axis_stride = a0 ? cos.stride(0) : 0, r.token_stride = cos.stride(a0);
+    r.axes = (int32_t)axes, r.half = (int32_t)half, r.interleaved = args[11] == Py_True, r.dtype = type;
+    if (args[10] == Py_None) {
+        if (axes != 1) Py_RETURN_FALSE;
+        r.section[0] = (int32_t)half;
+    } else {
+        if (!PyTuple_Check(args[10]) || PyTuple_GET_SIZE(args[10]) != axes) Py_RETURN_FALSE;
+        int64_t sum = 0, n = 0;
+        for (int x = 0; x < axes; ++x) {
+            if (!whole_number(PyTuple_GET_ITEM(args[10], x), 0, half, n)) Py_RETURN_FALSE;
+            r.section[x] = (int32_t)n, sum += n;
+        }
+        if (sum != half) Py_RETURN_FALSE;
+    }
+    int64_t Hq = 0;
+    if (query.given()) {
+        if (query->dim() != 3) Py_RETURN_FALSE;
+        Hq = query->size(1);
+        if (!is_states(query, N, Hq, keys) || Hq > INT32_MAX || (given.given() && !is_states(given, N, Hq, keys))) Py_RETURN_FALSE;
+    } else if (given.given()) {
+        Py_RETURN_FALSE;
+    }
+    const c10::cuda::CUDAGuard on(keys->device());
+    Tensor out;
+    if (query.given()) out = given.given() ? *given.t : at::empty({N, Hq, c.D}, keys->options());
+    check(adacode_append_rotary(&c, &r, query.at(), query.stride(0), query.stride(1), (int)Hq, Hq ? out.mutable_data_ptr() : nullptr,
+                                Hq ? out.stride(0) : 0, Hq ? out.stride(1) : 0, key.at(), key.stride(0), key.stride(1), value.at(), value.stride(0),
+                                value.stride(1), (int32_t *)const_cast<void *>(status.at()), c10::cuda::getCurrentCUDAStream(keys->device().index()).stream()),
+          "adacode_append_rotary");
+    count_write(*keys.t), count_write(*values.t);
+    if (!query.given()) Py_RETURN_NONE;
+    count_write(out);
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(query, key_pages, value_pages, block_table, seq_lens, cu_seqlens, max_query_len, scale, causal, window, seq_starts, out, status)
+//   -> what adacode_b200.paged_attention returns, or False, and nothing done, where it has to look closer
+PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n_args == 13, "paged_attention: arguments");
+    Args in;
+    const Arg keys = in.take(args[1]), values = in.take(args[2]), query = in.take(args[0]), table = in.take(args[3]), lens = in.take(args[4]),
+              cu = in.take(args[5], true), starts = in.take(args[10], true), given = in.take(args[11], true, true), status = in.take(args[12], false, true);
+    if (!in.ok || query->dim() != 3) Py_RETURN_FALSE;
+    const int64_t N = query->size(0), Hq = query->size(1);
+    adacode_paged_cache c;
+    if (!describe_cache(keys, values, table, lens, cu, N, c) || !is_states(query, N, Hq, keys) || (c.D != 64 && c.D != 128)) Py_RETURN_FALSE;
+    if (Hq <= 0 || Hq > INT32_MAX || Hq % c.Hkv != 0) Py_RETURN_FALSE;
+    if (c.table_width > 1 && c.page_size % 128 != 0 && c.page_size != 16 && c.page_size != 32 && c.page_size != 64) Py_RETURN_FALSE;
+    if (starts.given() && (starts->scalar_type() != at::kInt || starts->sizes() != lens->sizes() || !starts->is_contiguous())) Py_RETURN_FALSE;
+    if (given.given() && !is_states(given, N, Hq, keys)) Py_RETURN_FALSE;
+    int64_t longest = cu.given() ? N : N / c.B, window = 0;
+    if ((args[6] != Py_None && !whole_number(args[6], 0, INT32_MAX, longest)) || !whole_number(args[9], 0, INT32_MAX, window)) Py_RETURN_FALSE;
+    double scale = c.D == 64 ? 0.125 : 0.08838834764831845;
+    if (args[7] != Py_None) {
+        if (!PyFloat_Check(args[7])) Py_RETURN_FALSE;
+        scale = PyFloat_AS_DOUBLE(args[7]);
+    }
+    if (!on_sixteen_bytes(keys) || !on_sixteen_bytes(values) || !on_sixteen_bytes(query) || (given.given() && !on_sixteen_bytes(given))) Py_RETURN_FALSE;
+    const c10::cuda::CUDAGuard on(keys->device());
+    const Tensor out = given.given() ? *given.t : at::empty({N, Hq, c.D}, query->options());
+    const Tensor ws = at::empty({(int64_t)adacode_paged_attn_workspace_bytes((int)longest, (int)Hq, c.Hkv, c.D)}, keys->options().dtype(at::kByte));
+    check(adacode_paged_attn(&c, query.at(), query.stride(0), query.stride(1), (int)Hq, out.mutable_data_ptr(), out.stride(0), out.stride(1),
+                             (const int32_t *)starts.at(), (int)longest, (float)scale, args[8] == Py_True, (int)window, ws.mutable_data_ptr(), ws.nbytes(),
+                             (int32_t *)const_cast<void *>(status.at()), c10::cuda::getCurrentCUDAStream(keys->device().index()).stream()),
+          "adacode_paged_attn");
+    count_write(out);
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p, out) -> what adacode_b200.sample_tokens returns, or False, and nothing done,
+// where it has to look closer
+PyObject *sample_tokens(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n_args == 7, "sample_tokens: arguments");
+    Args in;
+    const Arg logits = in.take(args[0]), uniforms = in.take(args[1]), given = in.take(args[6], true, true);
+    if (!in.ok || logits->dim() != 2 || uniforms->scalar_type() != at::kFloat) Py_RETURN_FALSE;
+    const int64_t B = logits->size(0), V = logits->size(1);
+    const int type = element_type(*logits.t);
+    if (type < 0 || V < 1 || V > 1 << 30 || B > 1 << 27 || (V > 1 && logits->stride(1) != 1) || !is_shape(uniforms, {B}) || !uniforms->is_contiguous())
+        Py_RETURN_FALSE;
+    // settings: one number for all rows, or one per row
+    Arg per_row[4];
+    double all[4] = {0, 0, 0, 0};
+    for (int i = 0; i < 4; ++i) {
+        PyObject *o = args[2 + i];
+        if (PyFloat_Check(o)) {
+            all[i] = PyFloat_AS_DOUBLE(o);
+            if (i == 1) Py_RETURN_FALSE;
+        } else if (PyLong_Check(o)) {
+            int64_t n;
+            if (!whole_number(o, -1, INT32_MAX, n)) Py_RETURN_FALSE;
+            all[i] = (double)n;
+        } else {
+            per_row[i] = in.take(o);
+            if (!in.ok || per_row[i]->scalar_type() != (i == 1 ? at::kInt : at::kFloat) || !is_shape(per_row[i], {B}) || !per_row[i]->is_contiguous())
+                Py_RETURN_FALSE;
+        }
+        if (all[i] != all[i]) Py_RETURN_FALSE;
+    }
+    if (given.given() && (given->scalar_type() != at::kLong || !is_shape(given, {B}) || !given->is_contiguous())) Py_RETURN_FALSE;
+    const c10::cuda::CUDAGuard on(logits->device());
+    const Tensor out = given.given() ? *given.t : at::empty({B}, logits->options().dtype(at::kLong));
+    check(adacode_sample_tokens(logits.at(), logits.stride(0), type, (int)B, (int)V, (const float *)uniforms.at(), (const float *)per_row[0].at(), (float)all[0],
+                                (const int32_t *)per_row[1].at(), (int)all[1], (const float *)per_row[2].at(), (float)all[2],
+                                (const float *)per_row[3].at(), (float)all[3], out.mutable_data_ptr<int64_t>(),
+                                c10::cuda::getCurrentCUDAStream(logits->device().index()).stream()),
+          "adacode_sample_tokens");
+    count_write(out);
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
+    {"append_rotary", (PyCFunction)(void (*)(void))append_rotary, METH_FASTCALL, nullptr},
+    {"paged_attention", (PyCFunction)(void (*)(void))paged_attention, METH_FASTCALL, nullptr},
+    {"sample_tokens", (PyCFunction)(void (*)(void))sample_tokens, METH_FASTCALL, nullptr},
     {"pack", (PyCFunction)(void (*)(void))pack, METH_FASTCALL, nullptr},
     {"pack_flat", (PyCFunction)(void (*)(void))pack_flat, METH_FASTCALL, nullptr},
     {"append", (PyCFunction)(void (*)(void))append, METH_FASTCALL, nullptr},

@@ -24,8 +24,8 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from .codec import _scratch_for
-from .rows import increment_version, on_device, stream_ptr
+from .codec import _scratch_for, device_status
+from .rows import on_device, stream_ptr, written
 
 _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
 _ANGLES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.FP32}
@@ -75,9 +75,11 @@ def _states(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype) -> tor
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _refuse_gradients(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _refuse_autograd(what: str, read: tuple, written_to: tuple) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*read, *written_to)):
         raise RuntimeError(f'{what} has no backward pass: call it under torch.no_grad()')
+    if not torch.is_inference_mode_enabled() and any(t is not None and t.is_inference() for t in written_to):
+        raise RuntimeError(f'{what}: inference tensors are written to in inference mode only')
 
 
 def append_rotary(key: torch.Tensor, value: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, key_pages: torch.Tensor,
@@ -96,6 +98,13 @@ def append_rotary(key: torch.Tensor, value: torch.Tensor, cos: torch.Tensor, sin
     Keys (rotated, in 32 bits and rounded once) and values are written to the last tokens of their sequences.  Returns the rotated
     queries, in ``out`` if given (which may be ``query``), or None without ``query``.
     """
+    if key_pages.is_cuda:
+        got = _lib.native().append_rotary(key, value, cos, sin, key_pages, value_pages, block_table, seq_lens, query, cu_seqlens,
+                                          None if sections is None else tuple(sections),
+                                          bool(interleaved), out, device_status(key_pages.device))
+        if got is not False:
+            return got
+    # (what is left: a call to refuse, or one whose tensors have to be laid out first)
     if key.dim() != 3 or key_pages.dim() != 4:
         raise ValueError('key must be [N, Hkv, D] and the pages [pages, Hkv, page_size, D]')
     N, dtype = key.shape[0], key_pages.dtype
@@ -134,7 +143,7 @@ def append_rotary(key: torch.Tensor, value: torch.Tensor, cos: torch.Tensor, sin
             raise ValueError(f'out must be {dtype} {[N, Hq, D]} with unit stride along D')
     elif out is not None:
         raise ValueError('out without query')
-    _refuse_gradients('append_rotary', key, value, cos, sin, query, key_pages, value_pages, out)
+    _refuse_autograd('append_rotary', (key, value, cos, sin, query), (key_pages, value_pages, out))
     dev = key_pages.device
     sc = _scratch_for(dev)
     _same_device(dev, key=key, value=value, cos=cos, sin=sin, value_pages=value_pages, block_table=block_table, seq_lens=seq_lens, query=query,
@@ -147,7 +156,7 @@ def append_rotary(key: torch.Tensor, value: torch.Tensor, cos: torch.Tensor, sin
             out.data_ptr() if Hq else None, *(out.stride()[:2] if Hq else (0, 0)), key.data_ptr(), *key.stride()[:2],
             value.data_ptr(), *value.stride()[:2], sc.status.data_ptr(), stream_ptr(dev))
     _lib.check(rc, 'adacode_append_rotary')
-    increment_version([key_pages, value_pages] if out is None else [key_pages, value_pages, out])
+    written(key_pages, value_pages, out)
     return out
 
 
@@ -167,6 +176,12 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     Scores and sums are of 32 bits; the softmax weights are rounded to the pages' type for their product with the values.
     Returns ``[N, Hq, D]``, ``out`` if given.
     """
+    if key_pages.is_cuda:
+        got = _lib.native().paged_attention(query, key_pages, value_pages, block_table, seq_lens, cu_seqlens, max_query_len, scale, bool(causal),
+                                            window, seq_starts, out, device_status(key_pages.device))
+        if got is not False:
+            return got
+    # (what is left: a call to refuse, or one whose tensors have to be laid out first)
     if query.dim() != 3:
         raise ValueError('query must be [N, Hq, D]')
     N, Hq, D = query.shape
@@ -191,7 +206,7 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
         max_query_len = N // cache.B if cu_seqlens is None else N
     elif max_query_len < 0:
         raise ValueError('max_query_len must not be negative')
-    _refuse_gradients('paged_attention', query, key_pages, value_pages, out)
+    _refuse_autograd('paged_attention', (query, key_pages, value_pages), (out,))
     dev = key_pages.device
     sc = _scratch_for(dev)
     _same_device(dev, query=query, value_pages=value_pages, block_table=block_table, seq_lens=seq_lens, cu_seqlens=cu_seqlens,
@@ -201,15 +216,12 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     if scale is None:
         scale = D ** -0.5
     with on_device(dev):
-        stream = stream_ptr(dev)
-        need = int(_lib.lib().adacode_paged_attn_workspace_bytes(max_query_len, Hq, cache.Hkv, D))
-        # (a captured graph runs on other streams than the one that it is captured on: it has memory of its own)
-        ws = (torch.empty(need, dtype=torch.uint8, device=dev) if torch.cuda.is_current_stream_capturing()
-              else sc.partials.get(stream, need))
+        # (memory of every call's own: calls of other streams, and graphs that were captured, share nothing)
+        ws = torch.empty(int(_lib.lib().adacode_paged_attn_workspace_bytes(max_query_len, Hq, cache.Hkv, D)), dtype=torch.uint8, device=dev)
         rc = _lib.lib().adacode_paged_attn(
             ctypes.byref(cache), query.data_ptr(), *query.stride()[:2], Hq, out.data_ptr(), *out.stride()[:2],
             None if seq_starts is None else seq_starts.data_ptr(), int(max_query_len), float(scale), int(bool(causal)), int(window),
-            ws.data_ptr(), ws.numel(), sc.status.data_ptr(), stream)
+            ws.data_ptr(), ws.numel(), sc.status.data_ptr(), stream_ptr(dev))
     _lib.check(rc, 'adacode_paged_attn')
-    increment_version([out])
+    written(out)
     return out

@@ -29,6 +29,11 @@ def on_device(device: torch.device):
     return _HERE if index is None or index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
+def written(*tensors: torch.Tensor) -> None:
+    """Tensors that a launch has written to count it (inference tensors count nothing)."""
+    increment_version([t for t in tensors if t is not None and not t.is_inference()])
+
+
 def row_record(src: torch.Tensor, dst: torch.Tensor, rows: Optional[int] = None, at: int = 0) -> Optional[tuple]:
     """``dst[:, :, at: at + rows].copy_(src[:, :, :rows])`` (all of both without ``rows``) as a record of the row-copy
     kernel, or None if it is not one: it takes plain bf16 CUDA tensors [B, H, T, D] on one device, rows on 16-byte

@@ -13,29 +13,26 @@ import torch
 
 from . import _lib
 from .codec import _scratch_for
-from .rows import increment_version, on_device, stream_ptr
+from .rows import on_device, stream_ptr, written
 
 _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.FP32}
 Setting = Union[float, int, torch.Tensor]
+_MOST_TOKENS = 1 << 30
 
 
-def _setting(name: str, value: Optional[Setting], off, B: int, dtype: torch.dtype, device: torch.device) -> Optional[torch.Tensor]:
-    """A setting as one entry per row, or None where it is off for all."""
-    if value is None:
-        return None
+def _setting(name: str, value: Setting, B: int, dtype: torch.dtype, device: torch.device) -> tuple:
+    """A setting as (tensor of one entry per row or None, number for all rows)."""
     if isinstance(value, numbers.Real):
         if value != value:
             raise ValueError(f'{name} is not a number')
-        if off is not None and off(value):
-            return None
-        return torch.full((B,), value, dtype=dtype, device=device)
-    if value.shape != (B,) or value.dtype != dtype or value.device != device:
-        raise ValueError(f'{name} must be a number or {dtype} [{B}] on {device}: got {value.dtype} {list(value.shape)} on {value.device}')
-    return value.contiguous()
+        return None, value
+    if not isinstance(value, torch.Tensor) or value.shape != (B,) or value.dtype != dtype or value.device != device:
+        raise ValueError(f'{name} must be a number or {dtype} [{B}] on {device}: got {value!r}')
+    return value.contiguous(), 0
 
 
-def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Setting = 1.0, top_k: Optional[Setting] = 0,
-                  top_p: Optional[Setting] = 1.0, min_p: Optional[Setting] = 0.0, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Setting = 1.0, top_k: Setting = 0,
+                  top_p: Setting = 1.0, min_p: Setting = 0.0, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Draw one token of every row of ``logits`` ``[B, V]`` (bf16, fp16 or fp32) with the row's entry of ``uniforms``, fp32 ``[B]`` in [0, 1).
 
     Tokens are ordered by descending logit, the lower token first among equals.  The first ``top_k`` stay (0: all); of those, each whose
@@ -46,18 +43,20 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Set
 
     The settings are numbers for all rows or tensors of one entry per row (fp32, ``top_k`` int32).  Returns int64 ``[B]``, ``out`` if given.
     """
-    if logits.dim() != 2 or logits.dtype not in _DTYPES or logits.shape[1] == 0 or logits.shape[1] >= 2 ** 31:
-        raise ValueError(f'logits must be bf16, fp16 or fp32 [B, V]: got {logits.dtype} {list(logits.shape)}')
+    if logits.is_cuda:
+        got = _lib.native().sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p, out)
+        if got is not False:
+            return got
+    # (what is left: a call to refuse, or one whose tensors have to be laid out first)
+    if logits.dim() != 2 or logits.dtype not in _DTYPES or logits.shape[1] == 0 or logits.shape[1] > _MOST_TOKENS:
+        raise ValueError(f'logits must be bf16, fp16 or fp32 [B, V], V at most {_MOST_TOKENS}: got {logits.dtype} {list(logits.shape)}')
     B, V = logits.shape
     dev = logits.device
     if uniforms.dtype != torch.float32 or uniforms.shape != (B,) or uniforms.device != dev:
         raise ValueError(f'uniforms must be fp32 [{B}] on {dev}: got {uniforms.dtype} {list(uniforms.shape)} on {uniforms.device}')
-    temperature = _setting('temperature', temperature, None, B, torch.float32, dev)
-    if temperature is None:
-        raise ValueError('temperature must be given (0: the largest logit)')
-    top_k = _setting('top_k', top_k, lambda v: v <= 0 or v >= V, B, torch.int32, dev)
-    top_p = _setting('top_p', top_p, lambda v: v >= 1, B, torch.float32, dev)
-    min_p = _setting('min_p', min_p, lambda v: v <= 0, B, torch.float32, dev)
+    settings = [_setting(name, value, B, dtype, dev) for name, value, dtype in (
+        ('temperature', temperature, torch.float32), ('top_k', top_k, torch.int32), ('top_p', top_p, torch.float32),
+        ('min_p', min_p, torch.float32))]
     if out is None:
         out = torch.empty(B, dtype=torch.int64, device=dev)
     elif out.dtype != torch.int64 or out.shape != (B,) or not out.is_contiguous() or out.device != dev:
@@ -66,11 +65,12 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Set
         logits = logits.contiguous()
     uniforms = uniforms.contiguous()
     _scratch_for(dev)
+    (t, t_all), (k, k_all), (p, p_all), (m, m_all) = settings
     with on_device(dev):
         rc = _lib.lib().adacode_sample_tokens(
-            logits.data_ptr(), logits.stride(0), _DTYPES[logits.dtype], B, V, uniforms.data_ptr(), temperature.data_ptr(),
-            None if top_k is None else top_k.data_ptr(), None if top_p is None else top_p.data_ptr(),
-            None if min_p is None else min_p.data_ptr(), out.data_ptr(), stream_ptr(dev))
+            logits.data_ptr(), logits.stride(0), _DTYPES[logits.dtype], B, V, uniforms.data_ptr(), None if t is None else t.data_ptr(), t_all,
+            None if k is None else k.data_ptr(), max(-1, min(int(k_all), 2 ** 31 - 1)), None if p is None else p.data_ptr(), p_all,
+            None if m is None else m.data_ptr(), m_all, out.data_ptr(), stream_ptr(dev))
     _lib.check(rc, 'adacode_sample_tokens')
-    increment_version([out])
+    written(out)
     return out

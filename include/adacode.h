@@ -459,10 +459,11 @@ int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int6
  * at least min_p times the largest.  The token drawn is the first, in the order of the vocabulary, at which the running sum of what stays exceeds
  * uniform times its total.  temperature <= 0: the first token of the largest logit.  Minus infinity and NaN are never drawn, plus infinity counts as
  * the largest finite number; a row without a token to draw gives -1.  Weights and sums are of 64 bits.
- * temperature, top_p, min_p (fp32) and top_k (int32) are device arrays of B entries; each but temperature may be NULL (off).
+ * Settings are device arrays of B entries, or NULL: then the number behind it holds for all rows.
  */
 int adacode_sample_tokens(const void *logits, int64_t row_stride, int dtype, int B, int V, const float *uniforms, const float *temperature,
-                          const int32_t *top_k, const float *top_p, const float *min_p, int64_t *tokens, void *stream);
+                          float temperature_all, const int32_t *top_k, int top_k_all, const float *top_p, float top_p_all, const float *min_p,
+                          float min_p_all, int64_t *tokens, void *stream);
 
 #ifdef __cplusplus
 }

@@ -104,6 +104,6 @@ def test_entry_points_refuse_without_a_gpu():
     assert attend(N=0) == _lib.OK
     c, r = _lib.PagedCache(**fine), _lib.Rotary(at, at, 0, 32, 1, (ctypes.c_int32 * 4)(31), 32, 0, 2)
     assert L.adacode_append_rotary(ctypes.byref(c), ctypes.byref(r), None, 0, 0, 0, None, 0, 0, at, 64, 64, at, 64, 64, at, None) == _lib.ERR_INVALID_ARG
-    assert L.adacode_sample_tokens(at, 4, 7, 1, 4, at, at, None, None, None, at, None) == _lib.ERR_INVALID_ARG
-    assert L.adacode_sample_tokens(at, 4, 0, 1, 0, at, at, None, None, None, at, None) == _lib.ERR_INVALID_ARG
-    assert L.adacode_sample_tokens(at, 4, 0, 0, 4, at, at, None, None, None, at, None) == _lib.OK
+    assert L.adacode_sample_tokens(at, 4, 7, 1, 4, at, at, 1.0, None, 0, None, 1.0, None, 0.0, at, None) == _lib.ERR_INVALID_ARG
+    assert L.adacode_sample_tokens(at, 4, 0, 1, 0, at, at, 1.0, None, 0, None, 1.0, None, 0.0, at, None) == _lib.ERR_INVALID_ARG
+    assert L.adacode_sample_tokens(at, 4, 0, 0, 4, at, at, 1.0, None, 0, None, 1.0, None, 0.0, at, None) == _lib.OK
