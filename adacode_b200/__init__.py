@@ -24,11 +24,11 @@ from .mla_float_cache_utils import MLAFloat11Cache, MLALatentFloat11DenseRopeLay
 from .manager import convert_model
 from .model_configs import model_config_map
 from .paged import append_rotary, paged_attention
-from .sampling import sample_tokens
+from .sampling import FusedSampler, sample_tokens
 
 __all__ = [
     'Float11Cache', 'float11Layer', 'MLAFloat11Cache', 'MLALatentFloat11DenseRopeLayer',
     'TiledCompressedTensor', 'compress_tiled_tensor', 'materialize_tiled_state',
     'export_initial_compress_parameters', 'model_config_map', 'decode_attention', 'CompressorBitMap',
-    'convert_model', 'append_rotary', 'paged_attention', 'sample_tokens',
+    'convert_model', 'append_rotary', 'paged_attention', 'sample_tokens', 'FusedSampler',
 ]

@@ -283,34 +283,40 @@ __device__ __forceinline__ uint32_t warp_scan(uint32_t v) {
 // rows that hidden infinities have spoilt
 // ---------------------------------------------------------------------------------------
 
-// Columns c0 .. c1 - 1 of one row by the whole warp, in 32 bits, first the weights' sum and then the values, of which hidden ones and those of
-// weight 0 are not read.  A position without a page counts as zeros.
+// Columns c0 .. c1 - 1 of one row by the whole warp, in 32 bits, 32 positions at a time: first the weights' sum and then the values, of which hidden
+// ones and those of weight 0 are not read.  A position without a page counts as zeros.
 template <typename T, int D>
 __device__ __noinline__ void repair_row(const PagedArgs &a, int b, int h, int q0, int fresh, int len, int start, int row, int c0, int c1) {
     constexpr int E = D / 32;
     const adacode_paged_cache &c = a.cache;
-    const int lane = threadIdx.x & 31, t = row / a.G, head = h * a.G + row - t * a.G;
+    const int lane = threadIdx.x & 31, t = (int)((uint32_t)row / a.by_group), head = h * a.G + row - t * a.G;
     int lo, hi;
     seen_by(a, t, fresh, len, start, lo, hi);
-    const T *q = reinterpret_cast<const T *>(a.query) + (q0 + t) * a.q_n + head * a.q_h + lane * E;
-    float x[E], acc[E], m = -INFINITY, l = 0.f;
+    const T *q = reinterpret_cast<const T *>(a.query) + (q0 + t) * a.q_n + head * a.q_h;
+    const float scale = a.negate ? -a.scale : a.scale;
+    float acc[E], m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = widen(q[e]) * (a.negate ? -a.scale : a.scale), acc[e] = 0.f;
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
         const float base = m == -INFINITY ? 0.f : m, share = pass ? 1.f / l : 0.f;
 #pragma unroll 1
-        for (int j = lo; j < hi; ++j) {
-            int slot;
-            const int page = page_of(c, b, j, slot);
-            float s = 0.f;
+        for (int j0 = lo; j0 < hi; j0 += 32) {
+            // a position's score per lane
+            int slot = 0;
+            const int page = j0 + lane < hi ? page_of(c, b, j0 + lane, slot) : -1;
+            float s = j0 + lane < hi ? 0.f : -INFINITY;
             if (page >= 0) {
-                const T *k = reinterpret_cast<const T *>(c.key_pages) + page * c.key_page + h * c.key_head + slot * c.key_slot + lane * E;
+                const T *k = reinterpret_cast<const T *>(c.key_pages) + page * c.key_page + h * c.key_head + slot * c.key_slot;
+#pragma unroll 4
+                for (int d = 0; d < D; d += 8) {
+                    const uint4 kw = *reinterpret_cast<const uint4 *>(k + d), qw = *reinterpret_cast<const uint4 *>(q + d);
+                    const T *ke = reinterpret_cast<const T *>(&kw), *qe = reinterpret_cast<const T *>(&qw);
 #pragma unroll
-                for (int e = 0; e < E; ++e) s = fmaf(x[e], widen(k[e]), s);
+                    for (int e = 0; e < 8; ++e) s = fmaf(widen(qe[e]), widen(ke[e]), s);
+                }
+                s *= scale;
             }
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(kFull, s, d);
             if (pass == 0) {
                 const float top = fmaxf(m, s), from = top == -INFINITY ? 0.f : top;
                 l = l * exp2f(m - from) + exp2f(s - from);
@@ -318,12 +324,28 @@ __device__ __noinline__ void repair_row(const PagedArgs &a, int b, int h, int q0
                 continue;
             }
             const float p = exp2f(s - base) * share;
-            if (p == 0.f || page < 0) continue;
-            const T *v = reinterpret_cast<const T *>(c.value_pages) + page * c.value_page + h * c.value_head + slot * c.value_slot + lane * E;
+            const long long at = page * c.value_page + slot * c.value_slot;
+            unsigned seen = __ballot_sync(kFull, page >= 0 && p != 0.f);
+            while (seen) {
+                const int i = __ffs(seen) - 1;
+                seen &= seen - 1;
+                const float w = __shfl_sync(kFull, p, i);
+                const T *v = reinterpret_cast<const T *>(c.value_pages) + __shfl_sync(kFull, at, i) + h * c.value_head + lane * E;
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(p, widen(v[e]), acc[e]);
+                for (int e = 0; e < E; ++e) acc[e] = fmaf(w, widen(v[e]), acc[e]);
+            }
         }
-        if (l == 0.f) break;
+        if (pass == 0) {
+            // the lanes' maxima and sums put together
+            float top = m;
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+            l = m == -INFINITY ? l : l * exp2f(m - top);
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(kFull, l, d);
+            m = top;
+            if (l == 0.f) break;
+        }
     }
     T *out = reinterpret_cast<T *>(a.out) + (q0 + t) * a.o_n + head * a.o_h;
 #pragma unroll

@@ -34,7 +34,7 @@ import torch
 from transformers import Cache
 from transformers.cache_utils import DynamicLayer
 
-from . import _lib, codec
+from . import _lib, codec, paged
 from .codec import SegmentRef, TiledCompressedTensor, check_one_shape
 
 _SUPPORTED_LAYOUTS = ('segmented_tiled', 'legacy', 'tiled')
@@ -130,6 +130,13 @@ class _Residual:
         _copy_tokens(self.buf, self.length, states)
         self.length += q
 
+    def extend(self, like: torch.Tensor, block: int) -> torch.Tensor:
+        """Room for ``like``'s tokens behind the others, counted but not yet written: the buffer."""
+        q = int(like.shape[-2])
+        self._reserve(like, self.length + q, block)
+        self.length += q
+        return self.buf
+
     def drop_front(self, count: int) -> None:
         """Forget the first ``count`` tokens, moving what follows to the front."""
         count = int(count)
@@ -144,6 +151,53 @@ class _Residual:
     def clear(self) -> None:
         self.buf = None
         self.length = 0
+
+
+def _dense_pages(B: int, total: int, device: torch.device) -> tuple:
+    """(block table, lengths) of a dense ``[B, H, T, D]`` tensor as pages: one per sequence, ``total`` tokens of each."""
+    return (torch.arange(B, dtype=torch.int32, device=device)[:, None], torch.full((B,), total, dtype=torch.int32, device=device))
+
+
+class _Rotary:
+    """The rotation of one call's new tokens on their way into a cache (``paged.append_rotary``): the queries, the angles, and where the rotated
+    queries go."""
+
+    def __init__(self, query: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, sections, interleaved: bool):
+        if query.dim() != 4:
+            raise ValueError('query must be [B, Hq, T, D]')
+        B, Hq, T, D = query.shape
+        if cos.shape != sin.shape or cos.dim() not in (3, 4) or cos.shape[-2] != T or cos.shape[-3] not in (1, B):
+            raise ValueError(f'cos and sin must be [B or 1, T, R] or [axes, B or 1, T, R] for B = {B}, T = {T}: got {list(cos.shape)} and {list(sin.shape)}')
+        R = cos.shape[-1]
+        if R % 2 != 0 or R > D:
+            raise ValueError(f'cos and sin must have an even number of columns, at most {D}: got {R}')
+        # (a model's position embeddings hold every angle twice: in halves, or next to each other)
+        angles = slice(0, R, 2) if interleaved else slice(0, R // 2)
+        self.cos, self.sin = (x[..., angles].expand(*x.shape[:-3], B, T, R // 2).reshape(*x.shape[:-3], B * T, R // 2) for x in (cos, sin))
+        if self.cos.dtype not in (torch.bfloat16, torch.float32):
+            self.cos, self.sin = self.cos.float(), self.sin.float()
+        self.query = query.to(torch.bfloat16).transpose(1, 2).reshape(B * T, Hq, D)
+        self.shape = (B, T, Hq, D)
+        self.sections, self.interleaved, self.out = sections, interleaved, None
+
+    def append(self, key_states, value_states, key_buf, value_buf, total: int) -> None:
+        """Rotated keys, and values, to the tokens of the ``[B, H, capacity, D]`` buffers that end at ``total``."""
+        B, H, T, D = key_states.shape
+        if (B, T) != self.shape[:2]:
+            raise ValueError(f'queries of {self.shape[:2]} sequences and tokens, keys of {(B, T)}')
+        key, value = (x.transpose(1, 2).reshape(B * T, x.shape[1], x.shape[3]) for x in (key_states, value_states))
+        self.out = paged.append_rotary(key, value, self.cos, self.sin, key_buf, value_buf, *_dense_pages(B, total, key_buf.device),
+                                       query=self.query, sections=self.sections, interleaved=self.interleaved)
+
+    def rotated(self, key_states, value_states) -> tuple:
+        """Rotated keys, and values, as new ``[B, H, T, D]`` tensors."""
+        key_buf, value_buf = (torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) for x in (key_states, value_states))
+        self.append(key_states, value_states, key_buf, value_buf, key_states.shape[2])
+        return key_buf, value_buf
+
+    def queries(self) -> torch.Tensor:
+        """The rotated queries, ``[B, Hq, T, D]``."""
+        return self.out.view(self.shape).transpose(1, 2)
 
 
 class float11Layer(DynamicLayer):
@@ -350,7 +404,12 @@ class float11Layer(DynamicLayer):
     def _active_residual_tensors(self):
         return self._res_k.tensor(), self._res_v.tensor()
 
-    def _append_residual(self, key_states: torch.Tensor, value_states: torch.Tensor) -> None:
+    def _append_residual(self, key_states: torch.Tensor, value_states: torch.Tensor, rotary: Optional['_Rotary'] = None) -> None:
+        if rotary is not None and key_states.shape[-2] > 0:
+            # the residual's buffers are the pages: one per sequence, the new tokens are its last
+            key_buf, value_buf = self._res_k.extend(key_states, self.block_size), self._res_v.extend(value_states, self.block_size)
+            rotary.append(key_states, value_states, key_buf, value_buf, self._res_k.length)
+            return
         self._res_k.append(key_states, self.block_size)
         self._res_v.append(value_states, self.block_size)
 
@@ -719,6 +778,26 @@ class float11Layer(DynamicLayer):
             key_table=self._segment_table('k', ks) if ks else None,
             value_table=self._segment_table('v', vs) if vs else None)
 
+    def chunk_attention(self, query: torch.Tensor, scale: Optional[float] = None, seq_starts: Optional[torch.Tensor] = None,
+                        window: int = 0) -> torch.Tensor:
+        """Causal attention of a chunk of queries ``[B, Hq, T, D]``, those of the last T tokens that this layer caches, over all that it
+        caches: drafted tokens that are verified, the next turn of a conversation, a chunk of a prompt.  ``seq_starts`` (int32 ``[B]``)
+        hides the left padding in front of each sequence, ``window`` all but the last tokens before each query.  The dense view is made as for
+        ``update`` (the packed planes are decoded once, whatever T is) and read by ``paged_attention``, one page per sequence."""
+        if query.dim() != 4:
+            raise ValueError('query must be [B, Hq, T, D]')
+        B, Hq, T, D = query.shape
+        keys, values = self.materialize_dense()
+        if keys is None or keys.dim() != 4:
+            raise ValueError('the cache is empty')
+        total = int(keys.shape[2])
+        if keys.shape[0] != B or T > total:
+            raise ValueError(f'{T} queries of {B} sequences, and {total} cached tokens of {keys.shape[0]}')
+        tokens = query.transpose(1, 2).reshape(B * T, Hq, D)
+        out = paged.paged_attention(tokens, keys, values, *_dense_pages(B, total, keys.device), scale=scale, window=window,
+                                    seq_starts=seq_starts)
+        return out.view(B, T, Hq, D).transpose(1, 2)
+
     def _empty_states(self):
         if self.cache_device is None:
             return None
@@ -895,6 +974,11 @@ class float11Layer(DynamicLayer):
             key_states = key_states.to(torch.bfloat16)
         if value_states.dtype != torch.bfloat16:
             value_states = value_states.to(torch.bfloat16)
+        rotary = None if cache_kwargs is None else cache_kwargs.get('float11_rotary')
+        if rotary is not None and prefill_fastpath:
+            # (blocks are packed from where the rotated keys lie)
+            key_states, value_states = rotary.rotated(key_states, value_states)
+            rotary = None
 
         if prefill_fastpath and self._res_k.length == 0:
             # all full blocks go from the projection output to packed planes in one launch;
@@ -914,7 +998,7 @@ class float11Layer(DynamicLayer):
             if n_full < q_len:
                 self._append_residual(key_states[:, :, n_full:], value_states[:, :, n_full:])
         else:
-            self._append_residual(key_states, value_states)
+            self._append_residual(key_states, value_states, rotary)
             keys_exp_count, values_exp_count, flushed_any = self._flush_ready_blocks(
                 need_adjust=need_adjust,
                 delay_segmented_block=segmented and not prefill_fastpath,
@@ -1017,6 +1101,7 @@ class Float11Cache(Cache):
         self._init_adjust_schedule(need_adjust, update_steps, block_size, layout)
         self.peak_mem = 0
         self._fused_decode = False         # set by hf_attention.fused_decode
+        self._fused_chunks = False         # also for more than one token at a time
         self.layout = layout
         self.seq_tile_size = seq_tile_size if seq_tile_size is not None else block_size
         self.auto_init_compress_params = auto_init_compress_params
@@ -1063,7 +1148,8 @@ class Float11Cache(Cache):
             elif layer.has_pending_dense_block() and not layer.has_pending_adjust_work():
                 layer.apply_pending_dense_block_if_needed()
         need_adjust = self.need_adjust and self.steps % self.update_steps == 0
-        fused = getattr(self, '_fused_decode', False) and key_states.shape[-2] == 1 and layer.is_initialized
+        fused = (getattr(self, '_fused_decode', False) and layer.is_initialized
+                 and (key_states.shape[-2] == 1 or getattr(self, '_fused_chunks', False)))
         if fused:
             # hf_attention.fused_decode: the step's attention reads the packed planes itself
             cache_kwargs = dict(cache_kwargs or {}, float11_skip_materialize=True)
@@ -1091,6 +1177,24 @@ class Float11Cache(Cache):
             raise ValueError('decode_attention appends exactly one token per sequence; use update() for prefill')
         self.update(key_states, value_states, layer_idx, {'float11_skip_materialize': True})
         return self.layers[layer_idx].decode_attention(query, scale=scale, n_splits=n_splits)
+
+    def chunk_attention(self, query: torch.Tensor, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int,
+                        scale: Optional[float] = None, seq_starts: Optional[torch.Tensor] = None, window: int = 0) -> torch.Tensor:
+        """``decode_attention`` for T >= 1 new tokens per sequence: append ``key_states`` / ``value_states`` ([B, Hkv, T, D]) as
+        ``update`` does, then return the causal attention of ``query`` ([B, Hq, T, D]) over the whole cache (``float11Layer.chunk_attention``)."""
+        self.update(key_states, value_states, layer_idx, {'float11_skip_materialize': True})
+        return self.layers[layer_idx].chunk_attention(query, scale=scale, seq_starts=seq_starts, window=window)
+
+    def update_rotary(self, query: torch.Tensor, key_states: torch.Tensor, value_states: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                      layer_idx: int, cache_kwargs: Optional[dict] = None, sections=None, interleaved: bool = False) -> tuple:
+        """``update`` for queries and keys that have not been rotated yet: both are, and keys and values written to the cache, in one
+        launch (``append_rotary``).  ``cos`` and ``sin`` are a HF model's position embeddings ``[B or 1, T, R]``, with ``sections`` ``[axes, B or 1,
+        T, R]``.  Returns the rotated queries and what ``update`` returns."""
+        if type(self.layers[layer_idx]).update is not float11Layer.update:
+            raise NotImplementedError('update_rotary needs keys and values with heads; this layer caches something else')
+        rotary = _Rotary(query, cos, sin, sections, interleaved)
+        keys, values = self.update(key_states, value_states, layer_idx, dict(cache_kwargs or {}, float11_rotary=rotary))
+        return rotary.queries(), keys, values
 
     def get_layer_cache_view(self, layer_idx: int):
         return self.layers[layer_idx].get_cache_view()

@@ -13,6 +13,11 @@ the dense tensors, as before.
     with fused_decode(cache):
         out = model.generate(ids, past_key_values=cache, ...)
 
+With ``fused_decode(cache, model, chunks=True)`` updates of several tokens behind the prefill (drafted tokens of assisted generation, the next
+turn of a conversation, a chunk of a prompt) go the same way: the chunk's attention is computed by ``paged_attention`` over the dense view,
+without the model's mask in memory.  Left-padded batches are served too, in chunks and single steps: the mask is read once per
+forward pass and has to be causal behind each sequence's padding.
+
 Limits: every cached token is attended to, head_dim 64 or 128.  A step whose attention mask hides
 any cached position (left-padded batches) or whose layer uses a sliding window cannot be served by
 the kernel; such a step raises instead of attending to the wrong tokens, and ``fused_decode``
@@ -35,8 +40,16 @@ def float11_fused_attention(module, query, key, value, attention_mask, dropout: 
                             scaling: Optional[float] = None, **kwargs):
     """Attention function with the ``AttentionInterface`` signature."""
     cache = _active_cache
-    if cache is not None and query.shape[2] == 1 and getattr(cache, '_fused_decode', False):
+    chunks = cache is not None and getattr(cache, '_fused_chunks', False)
+    if cache is not None and (query.shape[2] == 1 or (chunks and key.shape[2] == query.shape[2] and _behind_prefill(cache, module, query))) and \
+            getattr(cache, '_fused_decode', False):
         layer = cache.layers[module.layer_idx]
+        if chunks:
+            starts = None if attention_mask is None else _left_padding(cache, attention_mask, layer.get_seq_length())
+            window = getattr(module, 'sliding_window', None) or 0
+            if query.shape[2] > 1 or starts is not None or window:
+                return layer.chunk_attention(query, scale=scaling, seq_starts=starts, window=window).transpose(1, 2).contiguous(), None
+            return layer.decode_attention(query, scale=scaling).transpose(1, 2).contiguous(), None
         if getattr(module, 'sliding_window', None):
             raise NotImplementedError('float11_fused attention has no sliding window; use the materialising path')
         if attention_mask is not None and not _mask_shows_everything(cache, attention_mask):
@@ -60,16 +73,44 @@ def _mask_shows_everything(cache, mask: torch.Tensor) -> bool:
     return ok
 
 
+def _behind_prefill(cache, module, query: torch.Tensor) -> bool:
+    """Whether the layer held tokens before this chunk (its first update is attended to by SDPA on the model's own tensors)."""
+    return cache.layers[module.layer_idx].get_seq_length() > query.shape[2]
+
+
+def _left_padding(cache, mask: torch.Tensor, total: int) -> Optional[torch.Tensor]:
+    """First visible position of every sequence (int32 [B]) of a mask that is causal behind left padding; None where nothing is
+    padded.  All layers of a forward pass get the same mask object, so the (synchronising) check runs once per pass."""
+    seen = getattr(cache, '_fused_mask_seen', None)
+    if seen is not None and seen[0] is mask:
+        return seen[1]
+    visible = mask if mask.dtype == torch.bool else mask == 0
+    B, T = visible.shape[0], visible.shape[2]
+    if visible.shape[3] != total:
+        raise NotImplementedError(f'float11_fused attention: a mask of {visible.shape[3]} positions for {total} cached tokens')
+    j = torch.arange(total, device=mask.device)
+    starts = visible[:, 0, -1].to(torch.int8).argmax(-1)
+    causal = (j >= starts[:, None, None]) & (j <= torch.arange(total - T, total, device=mask.device)[:, None])
+    if not bool((visible == causal[:, None]).all()):
+        raise NotImplementedError('float11_fused attention takes masks that are causal behind left padding; use the materialising path')
+    out = starts.to(torch.int32) if bool((starts > 0).any()) else None
+    cache._fused_mask_seen = (mask, out)
+    return out
+
+
 def register() -> str:
-    """Register the attention function with transformers; returns its name."""
+    """Register the attention function with transformers, and SDPA's masks for it (without them a padded batch would come without
+    any); returns its name."""
     from transformers import AttentionInterface
+    from transformers.masking_utils import AttentionMaskInterface, sdpa_mask
+    AttentionMaskInterface.register(ATTENTION_NAME, sdpa_mask)
     AttentionInterface.register(ATTENTION_NAME, float11_fused_attention)
     return ATTENTION_NAME
 
 
 @contextlib.contextmanager
-def fused_decode(cache, model=None):
-    """Single-token updates of ``cache`` skip the dense rebuild while this context is active.
+def fused_decode(cache, model=None, chunks: bool = False):
+    """Single-token updates of ``cache`` skip the dense rebuild while this context is active, with ``chunks`` all updates behind the prefill.
     Pass the model (or its config) to have its attention implementation checked: with any other
     implementation the model's own attention would run on the one token ``update`` returns."""
     global _active_cache
@@ -81,10 +122,10 @@ def fused_decode(cache, model=None):
                                f'(call hf_attention.register() and set it); found {impl!r}')
     previous = _active_cache
     _active_cache = cache
-    cache._fused_decode = True
+    cache._fused_decode, cache._fused_chunks = True, bool(chunks)
     try:
         yield cache
     finally:
-        cache._fused_decode = False
+        cache._fused_decode = cache._fused_chunks = False
         cache._fused_mask_seen = None
         _active_cache = previous

@@ -206,6 +206,15 @@ def get_parse() -> argparse.ArgumentParser:
     p.add_argument('--random_init_layers', type=int, default=None, help='fewer decoder layers (smoke runs)')
     p.add_argument('--fused_decode', action='store_true',
                    help='float11 only: decode steps through the fused unpack + attention kernel')
+    p.add_argument('--fused_chunks', action='store_true',
+                   help='with --fused_decode: updates of several tokens behind the prefill, and left-padded batches, too')
+    p.add_argument('--fused_sample', action='store_true',
+                   help='with --do_sample: tokens are drawn by the fused sampler, with the four settings below')
+    p.add_argument('--temperature', type=float, default=1.0)
+    p.add_argument('--top_k', type=int, default=50)
+    p.add_argument('--top_p', type=float, default=1.0)
+    p.add_argument('--min_p', type=float, default=0.0)
+    p.add_argument('--sample_seed', type=int, default=0)
     return p
 
 
@@ -258,6 +267,14 @@ def run(args) -> dict:
         from . import hf_attention
         model.config._attn_implementation = hf_attention.register()
 
+    sampler = None
+    if args.fused_sample:
+        if not args.do_sample:
+            raise ValueError('--fused_sample needs --do_sample')
+        from transformers import LogitsProcessorList
+        from .sampling import FusedSampler
+        sampler = LogitsProcessorList([FusedSampler(args.temperature, args.top_k, args.top_p, args.min_p, args.sample_seed)])
+
     dn = 'synthetic'
     all_info_lists[dn] = []
     mini = max(1, int(args.batch_size))
@@ -277,6 +294,8 @@ def run(args) -> dict:
                 if kv_cache_impl in ('float11', 'mla_float11'):
                     info.update(float11_layout=args.float11_layout, float11_need_adjust=bool(args.float11_need_adjust),
                                 float11_update_steps=int(args.float11_update_steps))
+                if sampler is not None:
+                    info['fused_sample'] = dict(zip(('temperature', 'top_k', 'top_p', 'min_p'), sampler[0].settings))
                 if kv_cache_impl == 'float11':
                     info['fused_decode'] = fused
                 if kv_cache_impl == 'mla_float11':
@@ -292,10 +311,10 @@ def run(args) -> dict:
                 info['total_input_tokens'] = input_lengths.sum().item()
                 info['input_mean_len'] = input_lengths.mean().item()
                 generation_config = GenerationConfig(
-                    max_new_tokens=max_new_tokens, min_new_tokens=args.min_new_tokens, do_sample=bool(args.do_sample),
+                    max_new_tokens=max_new_tokens, min_new_tokens=args.min_new_tokens, do_sample=bool(args.do_sample) and sampler is None,
                     return_dict_in_generate=True, output_scores=False, output_attentions=False,
                     output_hidden_states=False, pad_token_id=pad_id, eos_token_id=eos_id)
-                if not args.do_sample:
+                if not generation_config.do_sample:
                     generation_config.temperature = None
                     generation_config.top_p = None
                     generation_config.top_k = None
@@ -303,12 +322,12 @@ def run(args) -> dict:
                 begin = time.time()
                 if fused:
                     from . import hf_attention
-                    with hf_attention.fused_decode(prompt_cache):
+                    with hf_attention.fused_decode(prompt_cache, chunks=bool(args.fused_chunks)):
                         outputs = model.generate(**new_inputs, past_key_values=prompt_cache,
-                                                 generation_config=generation_config)
+                                                 generation_config=generation_config, logits_processor=sampler)
                 else:
                     outputs = model.generate(**new_inputs, past_key_values=prompt_cache,
-                                             generation_config=generation_config)
+                                             generation_config=generation_config, logits_processor=sampler)
                 torch.cuda.synchronize()
                 generate_time = time.time() - begin
                 info['generate_time'] = generate_time

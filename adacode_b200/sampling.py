@@ -74,3 +74,23 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Set
     _lib.check(rc, 'adacode_sample_tokens')
     written(out)
     return out
+
+
+class FusedSampler:
+    """``sample_tokens`` inside ``model.generate``: a logits processor that leaves every row one token, which greedy decoding then takes.
+
+        model.generate(**inputs, do_sample=False, logits_processor=LogitsProcessorList([FusedSampler(0.7, top_k=50, seed=0)]))
+
+    It has to be the last processor.  The uniform numbers come from a generator of its own on the logits' device.
+    """
+
+    def __init__(self, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, seed: int = 0):
+        self.settings = (float(temperature), int(top_k), float(top_p), float(min_p))
+        self.seed, self.generator = int(seed), None
+
+    def __call__(self, input_ids: torch.Tensor, scores: torch.Tensor) -> torch.Tensor:
+        if self.generator is None or self.generator.device != scores.device:
+            self.generator = torch.Generator(scores.device).manual_seed(self.seed)
+        uniforms = torch.rand(scores.shape[0], generator=self.generator, device=scores.device)
+        tokens = sample_tokens(scores, uniforms, *self.settings)
+        return torch.full_like(scores, -torch.inf).scatter_(1, tokens.clamp(min=0)[:, None], 0.0)
