@@ -24,103 +24,111 @@ struct AppendArgs {
     long long q_n, q_h, o_n, o_h, k_n, k_h, v_n, v_h;
     int Hq;
     int32_t *status;
+    bool whole_angles;        // of one axis, on 16-byte boundaries
+    int group;
 };
 
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Chunk {
+struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Chunk {
     T v[V];
 };
 
-// A CTA has one token; a thread one pair of V-column chunks of every so manieth head, whose angles it keeps: bound by memory, and by
-// latency where tokens are few.  The chunks of a pair are rotated against each other (half-split), lie side by side (interleaved), or
-// are copied (columns that are not rotated, and values).
+// `group` threads (whole warps) have one token; a thread one pair of V-column chunks of every so manieth head, whose angles it keeps.  The chunks
+// of a pair are rotated against each other (half-split), lie side by side (interleaved), or are copied (columns that are not rotated, and
+// values).  Bound by memory where tokens are many, by the latency of finding a token's page where they are few: what does not depend on the
+// page (angles, the first head) is on its way before the page is looked for, and the next head's loads before a head is stored.
 template <typename T, typename A, int V, bool INTERLEAVED>
-__global__ void __launch_bounds__(256) k_append_rotary(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(256, 3) k_append_rotary(const __grid_constant__ AppendArgs a) {
     const adacode_paged_cache &c = a.cache;
     const adacode_rotary &r = a.rotary;
-    const int i = blockIdx.x, pairs = c.D / (2 * V), pair = threadIdx.x % pairs, first = threadIdx.x / pairs, step = blockDim.x / pairs;
+    const int tid = threadIdx.x % a.group, i = blockIdx.x * (blockDim.x / a.group) + threadIdx.x / a.group;
+    const int pairs = c.D / (2 * V), pair = tid % pairs, first = tid / pairs, step = a.group / pairs;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (i >= c.N) return;
+    const int rotated = a.Hq + c.Hkv, heads = first < step ? rotated + c.Hkv : 0;      // (threads behind the last whole set of pairs have none)
+    const bool turned = pair * V < r.half;
+    const int lo = INTERLEAVED || !turned ? pair * 2 * V : pair * V;
+    const int hi = INTERLEAVED || !turned ? lo + V : r.half + pair * V;
+    const auto load = [&](int h, Chunk<T, V> &x, Chunk<T, V> &y) {
+        const T *src = h < a.Hq     ? reinterpret_cast<const T *>(a.query) + i * a.q_n + h * a.q_h
+                       : h < rotated ? reinterpret_cast<const T *>(a.key) + i * a.k_n + (h - a.Hq) * a.k_h
+                                     : reinterpret_cast<const T *>(a.value) + i * a.v_n + (h - rotated) * a.v_h;
+        x = *reinterpret_cast<const Chunk<T, V> *>(src + lo), y = *reinterpret_cast<const Chunk<T, V> *>(src + hi);
+    };
+    Chunk<T, V> x, y;
+    if (first < heads) load(first, x, y);
+    float cs[V], sn[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) cs[j] = 1.f, sn[j] = 0.f;
+    if (turned && heads) {
+        const A *cos = reinterpret_cast<const A *>(r.cos) + i * r.token_stride, *sin = reinterpret_cast<const A *>(r.sin) + i * r.token_stride;
+        if (V > 1 && a.whole_angles) {
+            const Chunk<A, V> p = *reinterpret_cast<const Chunk<A, V> *>(cos + pair * V), q = *reinterpret_cast<const Chunk<A, V> *>(sin + pair * V);
+#pragma unroll
+            for (int j = 0; j < V; ++j) cs[j] = widen(p.v[j]), sn[j] = widen(q.v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int f = pair * V + j;
+                int axis = 0, upto = r.section[0];
+                while (axis + 1 < r.axes && f >= upto) upto += r.section[++axis];
+                cs[j] = widen(cos[axis * r.axis_stride + f]), sn[j] = widen(sin[axis * r.axis_stride + f]);
+            }
+        }
+    }
     int end = 0, slot = 0;
     const int b = sequence_of(c, i, end);
     if (b >= c.B) return;
     const int at = c.seq_lens[b] - end + i, page = page_of(c, b, at, slot);
-    if (page < 0 && threadIdx.x == 0) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
-    const bool turned = pair * V < r.half;
-    const int lo = INTERLEAVED || !turned ? pair * 2 * V : pair * V;
-    const int hi = INTERLEAVED || !turned ? lo + V : r.half + pair * V;
-    float cs[V], sn[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) cs[j] = 1.f, sn[j] = 0.f;
-    if (turned) {
-        const A *cos = reinterpret_cast<const A *>(r.cos) + i * r.token_stride, *sin = reinterpret_cast<const A *>(r.sin) + i * r.token_stride;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int f = pair * V + j;
-            int axis = 0, upto = r.section[0];
-            while (axis + 1 < r.axes && f >= upto) upto += r.section[++axis];
-            cs[j] = widen(cos[axis * r.axis_stride + f]), sn[j] = widen(sin[axis * r.axis_stride + f]);
-        }
-    }
-    const int rotated = a.Hq + c.Hkv, heads = rotated + c.Hkv;
+    if (page < 0 && tid == 0) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
     for (int h = first; h < heads; h += step) {
-        const T *src;
-        T *dst;
-        if (h < a.Hq) {
-            src = reinterpret_cast<const T *>(a.query) + i * a.q_n + h * a.q_h;
-            dst = reinterpret_cast<T *>(a.query_out) + i * a.o_n + h * a.o_h;
-        } else if (page < 0) {
-            break;
-        } else if (h < rotated) {
-            src = reinterpret_cast<const T *>(a.key) + i * a.k_n + (h - a.Hq) * a.k_h;
-            dst = reinterpret_cast<T *>(c.key_pages) + page * c.key_page + (h - a.Hq) * c.key_head + slot * c.key_slot;
-        } else {
-            src = reinterpret_cast<const T *>(a.value) + i * a.v_n + (h - rotated) * a.v_h;
-            dst = reinterpret_cast<T *>(c.value_pages) + page * c.value_page + (h - rotated) * c.value_head + slot * c.value_slot;
-        }
-        const Chunk<T, V> x = *reinterpret_cast<const Chunk<T, V> *>(src + lo), y = *reinterpret_cast<const Chunk<T, V> *>(src + hi);
         Chunk<T, V> u = x, v = y;
+        if (h + step < heads) load(h + step, x, y);
         if (turned && h < rotated) {
+            const Chunk<T, V> p = u, q = v;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                if constexpr (INTERLEAVED) {
-                    const T *from = 2 * j < V ? x.v : y.v;
-                    T *to = 2 * j < V ? u.v : v.v;
-                    const int e = 2 * j % V;
-                    if constexpr (V > 1) {
-                        const float p = widen(from[e]), q = widen(from[e + 1]);
-                        to[e] = narrow<T>(p * cs[j] - q * sn[j]), to[e + 1] = narrow<T>(q * cs[j] + p * sn[j]);
-                    } else {
-                        const float p = widen(x.v[0]), q = widen(y.v[0]);
-                        u.v[0] = narrow<T>(p * cs[0] - q * sn[0]), v.v[0] = narrow<T>(q * cs[0] + p * sn[0]);
-                    }
+                // column j of the chunks, or columns 2 j and 2 j + 1 of the two together
+                const float s = widen(INTERLEAVED && V > 1 ? (2 * j < V ? p : q).v[2 * j % V] : p.v[j]);
+                const float t = widen(INTERLEAVED && V > 1 ? (2 * j < V ? p : q).v[(2 * j + 1) % V] : q.v[j]);
+                const T first_of = narrow<T>(s * cs[j] - t * sn[j]), second_of = narrow<T>(t * cs[j] + s * sn[j]);
+                if constexpr (INTERLEAVED && V > 1) {
+                    (2 * j < V ? u : v).v[2 * j % V] = first_of;
+                    (2 * j < V ? u : v).v[(2 * j + 1) % V] = second_of;
                 } else {
-                    const float p = widen(x.v[j]), q = widen(y.v[j]);
-                    u.v[j] = narrow<T>(p * cs[j] - q * sn[j]), v.v[j] = narrow<T>(q * cs[j] + p * sn[j]);
+                    u.v[j] = first_of, v.v[j] = second_of;
                 }
             }
         }
+        if (h >= a.Hq && page < 0) continue;
+        T *dst = h < a.Hq     ? reinterpret_cast<T *>(a.query_out) + i * a.o_n + h * a.o_h
+                 : h < rotated ? reinterpret_cast<T *>(c.key_pages) + page * c.key_page + (h - a.Hq) * c.key_head + slot * c.key_slot
+                               : reinterpret_cast<T *>(c.value_pages) + page * c.value_page + (h - rotated) * c.value_head + slot * c.value_slot;
         *reinterpret_cast<Chunk<T, V> *>(dst + lo) = u;
         *reinterpret_cast<Chunk<T, V> *>(dst + hi) = v;
     }
 }
 
 template <typename T, typename A, int V>
-void launch_append(const AppendArgs &a, cudaStream_t st) {
+cudaError_t launch_append(AppendArgs &a, cudaStream_t st) {
+    // Threads per token: eight warps where tokens are few, down to one where they fill half of the GPU's threads that way.  32 tokens of 48 heads
+    // of 128: 3.1 us with eight, 8.2 with one; 3090 tokens of 20 heads: 24.8 and 8.6; 13 854 tokens of 48 heads: 108 and 68 (5.1 TB/s).
     const int pairs = a.cache.D / (2 * V);
-    const int threads = pairs * (pairs < 256 ? 256 / pairs : 1);
-    if (a.rotary.interleaved) k_append_rotary<T, A, V, true><<<a.cache.N, threads, 0, st>>>(a);
-    else k_append_rotary<T, A, V, false><<<a.cache.N, threads, 0, st>>>(a);
-}
-
-template <typename T, typename A>
-void launch_append(const AppendArgs &a, bool wide, cudaStream_t st) {
-    if (wide) launch_append<T, A, 8>(a, st);
-    else launch_append<T, A, 1>(a, st);
+    a.group = 256;
+    while (a.group > 32 && a.group / 2 >= pairs && (int64_t)a.cache.N * a.group > 148 * 1024) a.group /= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(((int64_t)a.cache.N * a.group + 255) / 256)), cfg.blockDim = dim3(256), cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    return a.rotary.interleaved ? cudaLaunchKernelEx(&cfg, k_append_rotary<T, A, V, true>, a) : cudaLaunchKernelEx(&cfg, k_append_rotary<T, A, V, false>, a);
 }
 
 template <typename T>
-void launch_append(const AppendArgs &a, bool wide, cudaStream_t st) {
-    if (a.rotary.dtype == ADACODE_FP32) launch_append<T, float>(a, wide, st);
-    else launch_append<T, T>(a, wide, st);
+cudaError_t launch_append(AppendArgs &a, bool wide, cudaStream_t st) {
+    if (a.rotary.dtype == ADACODE_FP32) return wide ? launch_append<T, float, 8>(a, st) : launch_append<T, float, 1>(a, st);
+    return wide ? launch_append<T, T, 8>(a, st) : launch_append<T, T, 1>(a, st);
 }
 
 }  // namespace
@@ -144,17 +152,21 @@ int adacode_append_rotary(const adacode_paged_cache *cache, const adacode_rotary
     }
     if (columns != r.half) return ADACODE_ERR_INVALID_ARG;
     if (cache->N == 0) return ADACODE_OK;
-    const AppendArgs a{*cache,    r,       query,    key,       value,   query_out, query_token, query_head,
-                       out_token, out_head, key_token, key_head, value_token, value_head, Hq,        status};
+    const int size = r.dtype == ADACODE_FP32 ? 4 : 2;
+    const bool whole_angles = r.axes == 1 && (((uintptr_t)r.cos | (uintptr_t)r.sin) & 15) == 0 && r.token_stride * size % 16 == 0;
+    AppendArgs a{*cache,    r,        query,     key,      value,       query_out,  query_token, query_head,   out_token,
+                 out_head,  key_token, key_head, value_token, value_head, Hq,       status,      whole_angles, 0};
     // sixteen bytes at a time where everything allows it
     const uintptr_t pointers = (uintptr_t)query | (uintptr_t)query_out | (uintptr_t)key | (uintptr_t)value | (uintptr_t)cache->key_pages |
                                (uintptr_t)cache->value_pages;
     const int64_t strides = query_token | query_head | out_token | out_head | key_token | key_head | value_token | value_head | cache->key_page |
                             cache->key_head | cache->key_slot | cache->value_page | cache->value_head | cache->value_slot;
     const bool wide = (pointers & 15) == 0 && (strides & 7) == 0 && cache->D % 16 == 0 && r.half % 8 == 0;
-    if (cache->dtype == ADACODE_BF16) launch_append<__nv_bfloat16>(a, wide, (cudaStream_t)stream);
-    else launch_append<__half>(a, wide, (cudaStream_t)stream);
-    return cudaGetLastError() == cudaSuccess ? ADACODE_OK : ADACODE_ERR_CUDA;
+    const cudaError_t e = cache->dtype == ADACODE_BF16 ? launch_append<__nv_bfloat16>(a, wide, (cudaStream_t)stream)
+                                                       : launch_append<__half>(a, wide, (cudaStream_t)stream);
+    if (e == cudaSuccess) return ADACODE_OK;
+    (void)cudaGetLastError();
+    return ADACODE_ERR_CUDA;
 }
 
 }  // extern "C"
