@@ -3,12 +3,12 @@
 // Every cut (the top_k first, the nucleus, min_p) keeps a prefix of the order (descending logit, ascending token); tokens are kept
 // as 64-bit keys of that order.  A row has a cluster of 1 to 8 CTAs, whose warps own consecutive spans of the vocabulary.  Passes over the row, which
 // after the first come from L2:
-//   1  the largest logit.
-//   top_k up to kMostK: the tokens above a border that a sample of the row says is low enough are listed (their number is checked); the
-//      list is sorted, and all else happens in it.  No weight of any other token is computed.
-//   top_p alone: 2 adds up the weights, all of them in 64 bits and per interval of the logit (2048 intervals) in about 24, which tells the
-//      interval in which the nucleus ends; 3 adds up, per span, what lies above the interval in 64 bits and lists what lies in it.
-//      The sums of 3 say exactly whether the interval was right (if not, its neighbour is next); the sorted list says where the nucleus ends.
+//   1  the largest logit, and of every thread the largest of its tokens, in two halves.
+//   top_k up to kMostK: the k-th largest of those many maxima has at least k tokens above it, and hardly more.  Threads whose maxima reach it list
+//      their tokens that do; the list is sorted, and all else happens in it.  No weight of any other token is computed.
+//   top_p alone: 2 counts tokens per interval of the logit (2048 intervals), which with the interval's middle says where the nucleus about ends;
+//      3 computes every weight once, in 64 bits, and adds up, per span, what lies above that interval, what lies below it, and lists what
+//      lies in it.  These sums say exactly whether the interval was right (if not, a neighbour is next); the sorted list says where the nucleus ends.
 //   neither: 3 alone.
 //   Then the span in which the draw falls is walked again.
 // What fits no list (thousands of equal logits at a border, a larger top_k) goes the slow way: bisection of the keys by one CTA.
@@ -30,7 +30,6 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMostCtas = 8;             // per row
 constexpr int kStep = 256;               // tokens that a warp takes at a time, eight per lane
 constexpr int kBins = 2048;
-constexpr int kSample = 4096;            // tokens that the sample has
 constexpr int kList = 4096;
 constexpr int kMostK = 1024;
 
@@ -65,18 +64,15 @@ __device__ __forceinline__ int token_of(uint64_t place) { return (int)(0xFFFFFFF
 
 struct Shared {
     double roots[32];                    // 2**(j / 32)
-    union {
-        float weight[kBins];
-        uint32_t count[kBins];
-    } bin;
+    uint32_t count[kBins];
     uint64_t list[kList];
     double line[kMostK];
     double span_all[kMostCtas * kWarps], span_kept[kMostCtas * kWarps];
     double scan[kWarps + 1];
     uint64_t best[kWarps];
     uint64_t cta_best;
-    double cta_sum;
-    float low[kWarps];
+    double cta_below;
+    float low[kWarps], cta_low;
     int scan_n[kWarps];
     int listed, found, decided;
     uint64_t border;
@@ -86,13 +82,12 @@ struct Shared {
 // term is below 1.3e-12), 32 roots of 2.  Half the time of exp() (64-bit), whose last bits no draw needs.
 __device__ __forceinline__ double weight_of(float v, double largest, double k, const double *roots) {
     const double t = ((double)v - largest) * k;
-    if (!(t > -1000.0)) return 0.0;
     constexpr double kShift = 6755399441055744.0 / 32.0;       // 1.5 x 2**52 / 32
     const double shifted = t + kShift;
     const int n = __double2loint(shifted);
     const double r = (t - (shifted - kShift)) * 0.69314718055994530942;
     const double power = fma(fma(fma(fma(r, 1.0 / 24.0, 1.0 / 6.0), r, 0.5), r, 1.0), r, 1.0) * roots[n & 31];
-    return __hiloint2double(__double2hiint(power) + ((n >> 5) << 20), __double2loint(power));
+    return t > -1000.0 ? __hiloint2double(__double2hiint(power) + ((n >> 5) << 20), __double2loint(power)) : 0.0;      // (0 of NaN too)
 }
 
 template <typename R, typename Op>
@@ -297,23 +292,37 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     // ---- 1: the largest logit, the lowest token that has it
-    float most = -INFINITY;
-    int at = -1;
+    const float p = a.top_p ? a.top_p[row] : a.top_p_all, t = a.temperature ? a.temperature[row] : a.temperature_all;
+    const int k = a.top_k ? a.top_k[row] : a.top_k_all;
+    const bool use_k = k > 0 && k < V, use_p = p < 1.f;
+    float half_most[2] = {-INFINITY, -INFINITY}, low = INFINITY;
+    int half_at[2] = {-1, -1};
     for (int i = i0 + lane * 8; i < i1; i += kStep) {
         float v[8];
-        load_eight(x, i, V, a.wide, v);
+        load_eight(x, i, i1, a.wide, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (v[j] > most) most = v[j], at = i + j;
+        for (int j = 0; j < 8; ++j) {
+            if (v[j] > half_most[j / 4]) half_most[j / 4] = v[j], half_at[j / 4] = i + j;
+            if (v[j] > -INFINITY && v[j] < low) low = v[j];
+        }
     }
+    const bool second = half_most[1] > half_most[0] || (half_most[1] == half_most[0] && half_at[1] < half_at[0]);
+    const float most = second ? half_most[1] : half_most[0];
+    const int at = second ? half_at[1] : half_at[0];
+    // (intervals reach down to the smallest finite logit, those of the top_k to the smallest of the maxima)
+    if (use_k) low = fminf(half_most[0] > -INFINITY ? half_most[0] : INFINITY, half_most[1] > -INFINITY ? half_most[1] : INFINITY);
     if (tid < 32) s.roots[tid] = exp2((double)tid / 32.0);
     if (tid == 0) s.listed = 0;
+    for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
     const uint64_t here = block_reduce(at < 0 ? (uint64_t)0 : place_of(most, at), Most(), s.best);
-    if (tid == 0) s.cta_best = here;
+    low = block_reduce(low, Least(), s.low);
+    if (tid == 0) s.cta_best = here, s.cta_low = low;
     cluster.sync();
     uint64_t best = 0;
-    for (int r = 0; r < ctas; ++r) best = Most()(best, cluster.map_shared_rank(&s, r)->cta_best);
-    const float t = a.temperature ? a.temperature[row] : a.temperature_all;
+    for (int r = 0; r < ctas; ++r) {
+        best = Most()(best, cluster.map_shared_rank(&s, r)->cta_best);
+        low = Least()(low, cluster.map_shared_rank(&s, r)->cta_low);
+    }
     if (best == 0 || !(t > 0.f)) {
         if (rank == 0 && tid == 0) a.tokens[row] = best == 0 ? -1 : token_of(best);
         cluster.sync();
@@ -321,263 +330,235 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
     }
     const float top = value_of((uint32_t)(best >> 32));
     const double largest = top, scale = 1.4426950408889634074 / (double)t, least = least_of(a, row);
-    const int k = a.top_k ? a.top_k[row] : a.top_k_all;
-    const float p = a.top_p ? a.top_p[row] : a.top_p_all;
-    const bool use_k = k > 0 && k < V, use_p = p < 1.f;
-    bool slow = use_k && k > kMostK;
-
-    // ---- intervals of the logit, from the largest one down to a sample's smallest (or to where weights vanish)
-    const int sampled = V < kSample ? V : kSample;
-    float per_bin = 0.f;
-    if (!slow && (use_k || use_p)) {
-        const double stride = (double)V / sampled;
-        float low = INFINITY;
-        float v[kSample / kThreads];
-#pragma unroll
-        for (int j = 0; j < kSample / kThreads; ++j) {
-            const int i = tid + j * kThreads;
-            v[j] = i < sampled ? clean(widen(x[(int)(i * stride)])) : NAN;
-            if (v[j] > -INFINITY && v[j] < low) low = v[j];
-        }
-        low = block_reduce(low, Least(), s.low);
-        float range = top - low;                                // (minus infinity without a finite sample)
-        if (!use_k && range > 30.f * t) range = 30.f * t;
-        per_bin = range > 0.f ? fminf(kBins / range, FLT_MAX) : 0.f;
-        for (int i = tid; i < kBins; i += kThreads) s.bin.count[i] = 0;
-        __syncthreads();
-        if (use_k) {
-#pragma unroll
-            for (int j = 0; j < kSample / kThreads; ++j)
-                if (v[j] > -INFINITY) atomicAdd(&s.bin.count[min(kBins - 1, (int)((top - v[j]) * per_bin))], 1u);
-            __syncthreads();
-        }
-    }
-    const auto bin_of = [&](float v) { return min(kBins - 1, (int)((top - v) * per_bin)); };
-
-    if (use_k && !slow) {
-        // ---- the lowest interval that is listed: what the sample says holds some hundreds more than k
-        const int need = sampled == V ? k : (int)((long long)(k + k / 2 + 400) * sampled / V) + 8;
-        uint32_t c[kBins / kThreads], sum = 0;
-#pragma unroll
-        for (int j = 0; j < kBins / kThreads; ++j) c[j] = s.bin.count[tid * (kBins / kThreads) + j], sum += c[j];
-        if (tid == 0) s.decided = kBins - 1;
-        int total;
-        int before = block_scan((int)sum, total, s.scan_n);
-#pragma unroll
-        for (int j = 0; j < kBins / kThreads; ++j) {
-            if (before < need && before + (int)c[j] >= need) s.decided = tid * (kBins / kThreads) + j;
-            before += c[j];
-        }
-        __syncthreads();
-        const int lowest = s.decided;
-        for (int i = i0 + lane * 8; i - lane * 8 < i1; i += kStep) {
-            float v[8];
-            load_eight(x, i, i1, a.wide, v);
-            unsigned in = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) in |= (v[j] > -INFINITY && bin_of(v[j]) <= lowest ? 1u : 0u) << j;
-            if (in) {
-                int n = atomicAdd(&first.listed, __popc(in));
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (in >> j & 1) {
-                        if (n < kList) first.list[n] = place_of(v[j], i + j);
-                        ++n;
-                    }
-            }
-        }
-        cluster.sync();
-        if (rank != 0) return;
-        const int n = s.listed;
-        slow = n > kList || (n < k && lowest < kBins - 1);
-        if (!slow) {
-            sort_places(s.list, n);
-            const int kept_k = n < k ? n : k;
-            // weights of the first k, two consecutive ones per thread; all cuts keep a prefix
-            double w[2], sum_w = 0.0, all;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int i = 2 * tid + j;
-                w[j] = i < kept_k ? weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots) : 0.0;
-                sum_w += w[j];
-            }
-            double before_w = block_scan(sum_w, all, s.scan);
-            int kept = 0;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int i = 2 * tid + j;
-                if (i < kept_k && (i == 0 || !use_p || before_w < (double)p * all) && w[j] >= least && w[j] > 0.0) {
-                    ++kept;
-                    s.line[i] = w[j];
-                }
-                before_w += w[j];
-            }
-            int total_kept;
-            block_scan(kept, total_kept, s.scan_n);
-            __syncthreads();
-            // in the order of the vocabulary: descending complement of the token, with the place in the sorted list
-            for (int i = tid; i < total_kept; i += kThreads) s.list[i] = s.list[i] << 32 | (uint32_t)i;
-            __syncthreads();
-            sort_places(s.list, total_kept);
-            sum_w = 0.0;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int i = 2 * tid + j;
-                w[j] = i < total_kept ? s.line[(uint32_t)s.list[i]] : 0.0;
-                sum_w += w[j];
-            }
-            before_w = block_scan(sum_w, all, s.scan);
-            const double aim = (double)a.uniforms[row] * all;
-            if (tid == 0) s.found = total_kept - 1;             // (rounding may leave no sum above the aim)
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int i = 2 * tid + j;
-                before_w += w[j];
-                if (i < total_kept && before_w > aim) atomicMin(&s.found, i);
-            }
-            __syncthreads();
-            // (a weight that counts was computed from the first token on, so there is one)
-            if (tid == 0) a.tokens[row] = (int64_t)(0xFFFFFFFFu - (uint32_t)(s.list[s.found] >> 32));
-            return;
-        }
-        sample_slowly(a, s, x, row, (uint32_t)(best >> 32), largest, scale);
-        return;
-    }
+    // (fewer maxima than tokens asked for, and too many tokens for the list: the slow way)
+    bool slow = use_k && (k > kMostK || (V > kList && k > ctas * kThreads));
     if (slow) {
         cluster.sync();
         if (rank == 0) sample_slowly(a, s, x, row, (uint32_t)(best >> 32), largest, scale);
         return;
     }
+    float range = top - low;
+    if (!use_k && range > 30.f * t) range = 30.f * t;           // (weights below e**-30 share an interval)
+    const float per_bin = range > 0.f ? fminf(kBins / range, FLT_MAX) : 0.f;
+    const auto bin_of = [&](float v) { return min(kBins - 1, (int)((top - v) * per_bin)); };
+    constexpr int kEach = kBins / kThreads;
+    // counts of all CTAs, of this thread's intervals
+    const auto gather = [&](uint32_t (&c)[kEach]) {
+        cluster.sync();
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) c[j] = 0;
+        for (int r = 0; r < ctas; ++r) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(&cluster.map_shared_rank(&s, r)->count[tid * kEach]);
+            c[0] += v.x, c[1] += v.y, c[2] += v.z, c[3] += v.w;
+        }
+        static_assert(kEach == 4, "one 16-byte load");
+    };
+    // tokens of a group of eight that are listed, with the CTA that finishes the row
+    const auto list = [&](unsigned in, const float (&v)[8], int i) {
+        if (in == 0) return;
+        int n = atomicAdd(&first.listed, __popc(in));
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (in >> j & 1) {
+                if (n < kList) first.list[n] = place_of(v[j], i + j);
+                ++n;
+            }
+    };
 
-    // ---- 2: weights, and the interval in which the nucleus ends
-    int edge = kBins;                                           // everything lies above it
-    double all = 0.0;
+    if (use_k) {
+        int lowest = kBins;                                      // the lowest interval that is listed (all, of a short row)
+        if (V > kList) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (half_at[j] >= 0) atomicAdd(&s.count[bin_of(half_most[j])], 1u);
+            uint32_t c[kEach];
+            gather(c);
+            int total, sum = 0;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) sum += c[j];
+            if (tid == 0) s.decided = kBins;
+            int before = block_scan(sum, total, s.scan_n);
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                if (before < k && before + (int)c[j] >= k) s.decided = tid * kEach + j;
+                before += c[j];
+            }
+            __syncthreads();
+            lowest = s.decided;
+        }
+        bool look = lowest == kBins;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) look |= half_at[j] >= 0 && bin_of(half_most[j]) <= lowest;
+        if (look)
+            for (int i = i0 + lane * 8; i < i1; i += kStep) {
+                float v[8];
+                load_eight(x, i, i1, a.wide, v);
+                unsigned in = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) in |= (v[j] > -INFINITY && (lowest == kBins || bin_of(v[j]) <= lowest) ? 1u : 0u) << j;
+                list(in, v, i);
+            }
+        cluster.sync();
+        if (rank != 0) return;
+        const int n = s.listed;
+        if (n > kList) {
+            sample_slowly(a, s, x, row, (uint32_t)(best >> 32), largest, scale);
+            return;
+        }
+        sort_places(s.list, n);
+        const int kept_k = n < k ? n : k;
+        // weights of the first k, two consecutive ones per thread; all cuts keep a prefix
+        double w[2], sum_w = 0.0, all;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = 2 * tid + j;
+            w[j] = i < kept_k ? weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots) : 0.0;
+            sum_w += w[j];
+        }
+        double before_w = block_scan(sum_w, all, s.scan);
+        int kept = 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = 2 * tid + j;
+            if (i < kept_k && (i == 0 || !use_p || before_w < (double)p * all) && w[j] >= least && w[j] > 0.0) {
+                ++kept;
+                s.line[i] = w[j];
+            }
+            before_w += w[j];
+        }
+        int total_kept;
+        block_scan(kept, total_kept, s.scan_n);
+        __syncthreads();
+        // in the order of the vocabulary: descending complement of the token, with the place in the sorted list
+        for (int i = tid; i < total_kept; i += kThreads) s.list[i] = s.list[i] << 32 | (uint32_t)i;
+        __syncthreads();
+        sort_places(s.list, total_kept);
+        sum_w = 0.0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = 2 * tid + j;
+            w[j] = i < total_kept ? s.line[(uint32_t)s.list[i]] : 0.0;
+            sum_w += w[j];
+        }
+        before_w = block_scan(sum_w, all, s.scan);
+        const double aim = (double)a.uniforms[row] * all;
+        if (tid == 0) s.found = total_kept - 1;                  // (rounding may leave no sum above the aim)
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = 2 * tid + j;
+            before_w += w[j];
+            if (i < total_kept && before_w > aim) atomicMin(&s.found, i);
+        }
+        __syncthreads();
+        // (the largest weight, 1, always stays, so there is one)
+        if (tid == 0) a.tokens[row] = (int64_t)(0xFFFFFFFFu - (uint32_t)(s.list[s.found] >> 32));
+        return;
+    }
+
+    // ---- 2: the interval in which the nucleus about ends
+    int edge = kBins;                                            // everything lies above it
     if (use_p) {
-        double w_sum = 0.0;
         for (int i = i0 + lane * 8; i < i1; i += kStep) {
             float v[8];
             load_eight(x, i, i1, a.wide, v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (!(v[j] > -INFINITY)) continue;
-                const double w = weight_of(v[j], largest, scale, s.roots);
-                w_sum += w;
-                atomicAdd(&s.bin.weight[bin_of(v[j])], (float)w);
-            }
+            for (int j = 0; j < 8; ++j)
+                if (v[j] > -INFINITY) atomicAdd(&s.count[bin_of(v[j])], 1u);
         }
-        w_sum = block_reduce(w_sum, Plus(), s.scan);
-        if (tid == 0) s.cta_sum = w_sum;
-        cluster.sync();
-        for (int r = 0; r < ctas; ++r) all += cluster.map_shared_rank(&s, r)->cta_sum;
-        // (every CTA adds the same numbers in the same order)
-        float c[kBins / kThreads];
-        double sum = 0.0, total;
+        uint32_t c[kEach];
+        gather(c);
+        // (every CTA finds the same from the same numbers in the same order)
+        const float step = per_bin > 0.f ? -1.442695f / (per_bin * t) : 0.f;
+        float w[kEach], sum = 0.f, total;
 #pragma unroll
-        for (int j = 0; j < kBins / kThreads; ++j) {
-            c[j] = 0.f;
-            for (int r = 0; r < ctas; ++r) c[j] += cluster.map_shared_rank(&s, r)->bin.weight[tid * (kBins / kThreads) + j];
-            sum += c[j];
-        }
+        for (int j = 0; j < kEach; ++j) w[j] = c[j] * exp2f((tid * kEach + j + 0.5f) * step), sum += w[j];
         if (tid == 0) s.decided = kBins - 1;
-        double before = block_scan(sum, total, s.scan);
-        const double aim = (double)p * all;
+        float before = block_scan(sum, total, s.low);
+        const float aim = p * total;
 #pragma unroll
-        for (int j = 0; j < kBins / kThreads; ++j) {
-            if ((before < aim || (tid == 0 && j == 0)) && before + c[j] >= aim) atomicMin(&s.decided, tid * (kBins / kThreads) + j);
-            before += c[j];
+        for (int j = 0; j < kEach; ++j) {
+            if (before + w[j] >= aim) atomicMin(&s.decided, tid * kEach + j);
+            before += w[j];
         }
         __syncthreads();
         edge = s.decided;
     }
 
-    // ---- 3: what lies above the interval, per span, and what lies in it
-    uint64_t border = 0;                                        // the last place that stays
+    // ---- 3: what lies above the interval, per span, below it, and what lies in it
+    uint64_t border = 0;                                         // the last place that stays
     for (int tries = 0;; ++tries) {
-        double above = 0.0, kept = 0.0;
+        double above = 0.0, kept = 0.0, below = 0.0;
         for (int i = i0 + lane * 8; i < i1; i += kStep) {
             float v[8];
             load_eight(x, i, i1, a.wide, v);
             unsigned in = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if (!(v[j] > -INFINITY)) continue;
-                const int bin = edge < kBins ? bin_of(v[j]) : 0;
-                if (bin < edge) {
-                    const double w = weight_of(v[j], largest, scale, s.roots);
-                    above += w;
-                    if (w >= least) kept += w;
-                } else if (bin == edge) {
-                    in |= 1u << j;
-                }
+                const double w = weight_of(v[j], largest, scale, s.roots);
+                const int bin = use_p ? bin_of(v[j]) : 0;
+                if (bin < edge) above += w;
+                if (bin < edge && w >= least) kept += w;
+                if (bin > edge) below += w;
+                in |= (v[j] > -INFINITY && bin == edge ? 1u : 0u) << j;
             }
-            if (in) {
-                int n = atomicAdd(&first.listed, __popc(in));
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (in >> j & 1) {
-                        if (n < kList) first.list[n] = place_of(v[j], i + j);
-                        ++n;
-                    }
-            }
+            list(in, v, i);
         }
         above = warp_reduce(above, Plus()), kept = warp_reduce(kept, Plus());
         if (lane == 0) first.span_all[me] = above, first.span_kept[me] = kept;
+        if (use_p) {
+            below = block_reduce(below, Plus(), s.scan);
+            if (tid == 0) s.cta_below = below;
+        }
         cluster.sync();
         if (!use_p) break;
         if (rank == 0) {
             const int n = s.listed;
-            int next = -1;                                      // -1: done, -2: the slow way, else: the interval to look at
+            int next = -1;                                       // -1: done, -2: the slow way, else: the interval to look at
             if (n > kList) {
                 next = -2;
             } else {
                 sort_places(s.list, n);
-                double over = 0.0, total, running = 0.0;
+                double over = 0.0, under = 0.0, total, running = 0.0;
                 for (int i = 0; i < spans; ++i) over += s.span_all[i];
+                for (int r = 0; r < ctas; ++r) under += cluster.map_shared_rank(&s, r)->cta_below;
                 // eight consecutive places per thread
-                constexpr int kEach = kList / kThreads;
-                double w[kEach], sum = 0.0;
-#pragma unroll
-                for (int j = 0; j < kEach; ++j) {
-                    const int i = tid * kEach + j;
-                    w[j] = i < n ? weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots) : 0.0;
-                    sum += w[j];
+                constexpr int kPlaces = kList / kThreads;
+                double sum = 0.0;
+                for (int j = 0; j < kPlaces; ++j) {
+                    const int i = tid * kPlaces + j;
+                    if (i < n) sum += weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots);
                 }
                 running = over + block_scan(sum, total, s.scan);
-                const double aim = (double)p * all;
+                const double aim = (double)p * (over + total + under);
                 if (over >= aim && edge > 0) next = edge - 1;
                 else if (over + total < aim && edge < kBins - 1) next = edge + 1;
                 if (tries == 4 && next >= 0) next = -2;
                 if (next == -1) {
                     int inside = 0, total_inside;
-#pragma unroll
-                    for (int j = 0; j < kEach; ++j) {
-                        const int i = tid * kEach + j;
-                        if (i < n && (running < aim || s.list[i] == best))
-                            ++inside;
-                        running += w[j];
+                    for (int j = 0; j < kPlaces; ++j) {
+                        const int i = tid * kPlaces + j;
+                        if (i >= n) break;
+                        inside += running < aim || s.list[i] == best;
+                        running += weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots);
                     }
                     block_scan(inside, total_inside, s.scan_n);
                     if (tid == 0) s.border = total_inside > 0 ? s.list[total_inside - 1] : 1;
-                    __syncthreads();
-                    // spans' sums in a fixed order: a warp each, over the places that stay
+                    // the weights that stay count in their spans, in a fixed order: a warp each
                     for (int sp = warp; sp < spans; sp += kWarps) {
                         double more = 0.0;
                         for (int i = lane; i < total_inside; i += 32)
                             if (token_of(s.list[i]) / span == sp) {
-                                const double v = weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots);
-                                if (v >= least) more += v;
+                                const double w = weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots);
+                                if (w >= least) more += w;
                             }
                         more = warp_reduce(more, Plus());
                         if (lane == 0) s.span_kept[sp] += more;
                     }
                 }
             }
-            if (tid == 0) {
-                s.listed = 0;
-                s.decided = next;
-            }
             __syncthreads();
+            if (tid == 0) s.listed = 0, s.decided = next;
         }
         cluster.sync();
         const int next = first.decided;
@@ -679,9 +660,14 @@ extern "C" int adacode_sample_tokens(const void *logits, int64_t row_stride, int
     const int size = dtype == ADACODE_FP32 ? 4 : 2;
     const bool wide = ((uintptr_t)logits & 15) == 0 && (row_stride * size) % 16 == 0;
     const SampleArgs a{logits, row_stride, V, wide, uniforms, temperature, top_p, min_p, top_k, tokens, temperature_all, top_p_all, min_p_all, top_k_all};
-    // As many CTAs per row as keep the GPU's 148 SMs busy, three on each, and leave every warp a step or more of the vocabulary.
+    // CTAs per row: the number that makes the rounds of two CTAs on each of 148 SMs shortest, fewer on ties, as long as every warp has a
+    // step of the vocabulary.  192 rows of 151936: three, two rounds of a third of a row each (two: two of a half).
     int ctas = 1;
-    while (ctas < kMostCtas && (int64_t)B * ctas < 2 * 148 && V > 2 * ctas * kWarps * kStep / 2) ctas *= 2;
+    double best = 1e30;
+    for (int n = 1; n <= kMostCtas && (n == 1 || (int64_t)(n - 1) * kWarps * kStep < V); ++n) {
+        const double rounds = (double)(((int64_t)B * n + 295) / 296) / n;
+        if (rounds < best * 0.95) best = rounds, ctas = n;
+    }
     cudaStream_t st = (cudaStream_t)stream;
     const cudaError_t e = dtype == ADACODE_BF16 ? launch<__nv_bfloat16>(a, B, ctas, st)
                           : dtype == ADACODE_FP16 ? launch<__half>(a, B, ctas, st)
