@@ -48,13 +48,23 @@ struct SampleArgs {
 __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
-// plus infinity counts as the largest number; NaN stays
-__device__ __forceinline__ float clean(float v) { return v > FLT_MAX ? FLT_MAX : v; }
+// plus infinity counts as the largest number
+__device__ __forceinline__ float capped(float v) { return fminf(v, FLT_MAX); }
+__device__ __forceinline__ float most_of(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));      // (passes NaN over)
+    return r;
+}
+__device__ __forceinline__ float least_of(float a, float b, float c) {
+    float r;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
 // NaN and minus infinity have key 0 (never drawn), both zeros one key.
 __device__ __forceinline__ uint32_t key_of(float v) {
     if (!(v > -INFINITY)) return 0;
-    const uint32_t u = __float_as_uint(v + 0.f);
+    const uint32_t u = __float_as_uint(capped(v) + 0.f);
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key); }
@@ -64,31 +74,39 @@ __device__ __forceinline__ int token_of(uint64_t place) { return (int)(0xFFFFFFF
 
 struct Shared {
     double roots[32];                    // 2**(j / 32)
-    uint32_t count[kBins];
+    uint32_t count[kBins];               // (later: the span of every listed token)
     uint64_t list[kList];
     double line[kMostK];
     double span_all[kMostCtas * kWarps], span_kept[kMostCtas * kWarps];
     double scan[kWarps + 1];
-    uint64_t best[kWarps];
-    uint64_t cta_best;
+    unsigned long long slow[kWarps];
     double cta_below;
-    float low[kWarps], cta_low;
+    float low[kWarps], cta_low, cta_top;
     int scan_n[kWarps];
     int listed, found, decided;
     uint64_t border;
 };
 
-// exp(x / T) = 2**(x k): x k rounded to 1/32, the rest's power by its Taylor series (degree 4, |rest ln 2| <= ln 2 / 64: the next
-// term is below 1.3e-12), 32 roots of 2.  Half the time of exp() (64-bit), whose last bits no draw needs.
-__device__ __forceinline__ double weight_of(float v, double largest, double k, const double *roots) {
-    const double t = ((double)v - largest) * k;
-    constexpr double kShift = 6755399441055744.0 / 32.0;       // 1.5 x 2**52 / 32
-    const double shifted = t + kShift;
-    const int n = __double2loint(shifted);
-    const double r = (t - (shifted - kShift)) * 0.69314718055994530942;
-    const double power = fma(fma(fma(fma(r, 1.0 / 24.0, 1.0 / 6.0), r, 0.5), r, 1.0), r, 1.0) * roots[n & 31];
-    return t > -1000.0 ? __hiloint2double(__double2hiint(power) + ((n >> 5) << 20), __double2loint(power)) : 0.0;      // (0 of NaN too)
-}
+// What turns a logit into its weight: w = exp((x - largest) / T) = 2**((x - largest) k).  Below `floor` (600 T from the largest) it is 0.
+struct Weights {
+    double largest, k;
+    float floor;
+    const double *roots;
+    __device__ Weights(float top, float t, const double *roots)
+        : largest(top), k(1.4426950408889634074 / (double)t), floor(fmaxf(top - 600.f * t, -FLT_MAX)), roots(roots) {}
+    // The exponent rounded to 1/32, the rest's power by its Taylor series (degree 4, |rest ln 2| <= ln 2 / 64: the next term is below 1.3e-12), 32 roots of
+    // 2.  Half the time of exp() (64-bit), whose last bits no draw needs.
+    __device__ __forceinline__ double operator()(float v) const {
+        const double t = ((double)capped(v) - largest) * k;
+        constexpr double kShift = 6755399441055744.0 / 32.0;       // 1.5 x 2**52 / 32
+        const double shifted = t + kShift;
+        const int n = __double2loint(shifted);
+        const double r = (t - (shifted - kShift)) * 0.69314718055994530942;
+        const double power = fma(fma(fma(fma(r, 1.0 / 24.0, 1.0 / 6.0), r, 0.5), r, 1.0), r, 1.0) * roots[n & 31];
+        const bool any = v >= floor;                               // (not NaN)
+        return __hiloint2double(any ? __double2hiint(power) + ((n >> 5) << 20) : 0, any ? __double2loint(power) : 0);
+    }
+};
 
 template <typename R, typename Op>
 __device__ __forceinline__ R warp_reduce(R v, Op op) {
@@ -141,15 +159,30 @@ __device__ R block_scan(R v, R &total, R *shared) {
     return before + (incl - v);
 }
 
-// Descending bitonic sort of n (at most kList) places, padded with zeros to a power of two.
+// Descending sort of n (at most kList) different places.  Up to kThreads by counting what is larger, all others' bitonic, padded with zeros to a
+// power of two: 300 places take 2000 cycles against 14 000.
 __device__ void sort_places(uint64_t *list, int n) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    if (n <= kThreads) {
+        const uint64_t mine = tid < n ? list[tid] : 0;
+        int larger = 0;
+        if (tid < n) {
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) larger += list[i] > mine;
+        }
+        __syncthreads();
+        if (tid < n) list[larger] = mine;
+        __syncthreads();
+        return;
+    }
     int size = 2;
     while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
+    for (int i = n + tid; i < size; i += kThreads) list[i] = 0;
     __syncthreads();
     for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+            for (int i = tid; i < size / 2; i += kThreads) {
                 const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
                 const uint64_t p = list[lo], q = list[hi];
                 if ((p < q) == ((lo & k) == 0)) list[lo] = q, list[hi] = p;
@@ -159,7 +192,7 @@ __device__ void sort_places(uint64_t *list, int n) {
 }
 
 // The smallest weight that stays; the largest weight, 1, always does.
-__device__ __forceinline__ double least_of(const SampleArgs &a, int row) {
+__device__ __forceinline__ double smallest_of(const SampleArgs &a, int row) {
     const float p = a.min_p ? a.min_p[row] : a.min_p_all;
     return p > 0.f ? fminf(p, 1.f) : 0.f;
 }
@@ -172,20 +205,31 @@ __device__ __forceinline__ void load_eight(const T *x, int i, int V, bool wide, 
 #pragma unroll
         for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4 *>(raw)[j] = __ldg(reinterpret_cast<const uint4 *>(x + i) + j);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = clean(widen(raw[j]));
+        for (int j = 0; j < 8; ++j) v[j] = widen(raw[j]);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = i + j < V ? clean(widen(x[i + j])) : NAN;
+        for (int j = 0; j < 8; ++j) v[j] = i + j < V ? widen(x[i + j]) : NAN;
+    }
+}
+
+// A warp's tokens i0 .. i1 - 1, eight per lane and step, the loads of U steps under way at a time (with one, the first pass over 58 MB took 34 us).
+template <int U, typename T, typename Use>
+__device__ __forceinline__ void each_eight(const T *x, int i0, int i1, bool wide, Use &&use) {
+    for (int i = i0 + (threadIdx.x & 31) * 8; i < i1; i += U * kStep) {
+        float v[U][8];
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_eight(x, i + u * kStep, i1, wide, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) use(v[u], i + u * kStep);
     }
 }
 
 // One CTA, bisection of the keys: (cut, ties) are a key and the number of its tokens that stay, lower tokens first.
 template <typename T>
-__device__ void sample_slowly(const SampleArgs &a, Shared &s, const T *x, int row, uint32_t top, double largest, double scale) {
+__device__ void sample_slowly(const SampleArgs &a, Shared &s, const T *x, int row, uint32_t top, const Weights &weight_of) {
     const int tid = threadIdx.x, V = a.V;
-    const auto weight = [&](uint32_t key) { return key == 0 ? 0.0 : weight_of(value_of(key), largest, scale, s.roots); };
-    const auto key_at = [&](int i) { return key_of(clean(widen(x[i]))); };
-    unsigned long long *s_u = reinterpret_cast<unsigned long long *>(s.best);
+    const auto weight = [&](uint32_t key) { return key == 0 ? 0.0 : weight_of(value_of(key)); };
+    const auto key_at = [&](int i) { return key_of(widen(x[i])); };
     uint32_t cut = 1;
     long long ties = V;
     const int k = a.top_k ? a.top_k[row] : a.top_k_all;
@@ -197,7 +241,7 @@ __device__ void sample_slowly(const SampleArgs &a, Shared &s, const T *x, int ro
             const uint32_t mid = lo + (hi - lo) / 2 + 1;
             unsigned long long n = 0;
             for (int i = tid; i < V; i += kThreads) n += key_at(i) >= mid;
-            n = block_reduce(n, Plus(), s_u);
+            n = block_reduce(n, Plus(), s.slow);
             if ((long long)n >= k) lo = mid;
             else hi = mid - 1, above = (long long)n;
         }
@@ -215,7 +259,7 @@ __device__ void sample_slowly(const SampleArgs &a, Shared &s, const T *x, int ro
                 n += key == cut;
             }
             w = block_reduce(w, Plus(), s.scan);
-            n = block_reduce(n, Plus(), s_u);
+            n = block_reduce(n, Plus(), s.slow);
             if (from <= cut && n > 0) w += (double)((long long)n < ties ? (long long)n : ties) * weight(cut);   // (no token has a NaN's key)
             return w;
         };
@@ -235,7 +279,7 @@ __device__ void sample_slowly(const SampleArgs &a, Shared &s, const T *x, int ro
         ties = lo == cut && ties < n ? ties : n;
         cut = lo;
     }
-    const double least = least_of(a, row);
+    const double least = smallest_of(a, row);
     // runs of consecutive tokens per thread: ties before it, weight before it, the token
     const int per = (V + kThreads - 1) / kThreads, i0 = min(tid * per, V), i1 = min(i0 + per, V);
     int same = 0, all_same = 0;
@@ -296,51 +340,60 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
     const int k = a.top_k ? a.top_k[row] : a.top_k_all;
     const bool use_k = k > 0 && k < V, use_p = p < 1.f;
     float half_most[2] = {-INFINITY, -INFINITY}, low = INFINITY;
-    int half_at[2] = {-1, -1};
-    for (int i = i0 + lane * 8; i < i1; i += kStep) {
-        float v[8];
-        load_eight(x, i, i1, a.wide, v);
+    each_eight<2>(x, i0, i1, a.wide, [&](const float (&v)[8], int) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (v[j] > half_most[j / 4]) half_most[j / 4] = v[j], half_at[j / 4] = i + j;
-            if (v[j] > -INFINITY && v[j] < low) low = v[j];
-        }
-    }
-    const bool second = half_most[1] > half_most[0] || (half_most[1] == half_most[0] && half_at[1] < half_at[0]);
-    const float most = second ? half_most[1] : half_most[0];
-    const int at = second ? half_at[1] : half_at[0];
+        for (int j = 0; j < 8; j += 2) half_most[j / 4] = most_of(half_most[j / 4], v[j], v[j + 1]), low = least_of(low, v[j], v[j + 1]);
+    });
     // (intervals reach down to the smallest finite logit, those of the top_k to the smallest of the maxima)
-    if (use_k) low = fminf(half_most[0] > -INFINITY ? half_most[0] : INFINITY, half_most[1] > -INFINITY ? half_most[1] : INFINITY);
-    if (tid < 32) s.roots[tid] = exp2((double)tid / 32.0);
-    if (tid == 0) s.listed = 0;
-    for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
-    const uint64_t here = block_reduce(at < 0 ? (uint64_t)0 : place_of(most, at), Most(), s.best);
-    low = block_reduce(low, Least(), s.low);
-    if (tid == 0) s.cta_best = here, s.cta_low = low;
-    cluster.sync();
-    uint64_t best = 0;
-    for (int r = 0; r < ctas; ++r) {
-        best = Most()(best, cluster.map_shared_rank(&s, r)->cta_best);
-        low = Least()(low, cluster.map_shared_rank(&s, r)->cta_low);
+    if (use_k) {
+        low = fminf(half_most[0] > -INFINITY ? half_most[0] : INFINITY, half_most[1] > -INFINITY ? half_most[1] : INFINITY);
+    } else if (__any_sync(kFull, low == -INFINITY)) {
+        low = INFINITY;
+        each_eight<1>(x, i0, i1, a.wide, [&](const float (&v)[8], int) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (v[j] > -INFINITY && v[j] < low) low = v[j];
+        });
     }
-    if (best == 0 || !(t > 0.f)) {
-        if (rank == 0 && tid == 0) a.tokens[row] = best == 0 ? -1 : token_of(best);
+    if (tid < 32) s.roots[tid] = exp2((double)tid / 32.0);
+    if (tid == 0) s.listed = 0, s.found = INT32_MAX;
+    for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
+    float top = block_reduce(fmaxf(half_most[0], half_most[1]), Most(), s.low);
+    low = block_reduce(low, Least(), s.low);
+    if (tid == 0) s.cta_top = top, s.cta_low = low;
+    cluster.sync();
+    for (int r = 0; r < ctas; ++r) {
+        top = fmaxf(top, cluster.map_shared_rank(&s, r)->cta_top);
+        low = fminf(low, cluster.map_shared_rank(&s, r)->cta_low);
+    }
+    if (!(top > -INFINITY) || !(t > 0.f)) {
+        // nothing to draw, or the first token of the largest logit
+        if (top > -INFINITY && fmaxf(half_most[0], half_most[1]) == top)
+            each_eight<1>(x, i0, i1, a.wide, [&](const float (&v)[8], int i) {
+#pragma unroll
+                for (int j = 7; j >= 0; --j)
+                    if (v[j] > -INFINITY && capped(v[j]) == capped(top)) atomicMin(&first.found, i + j);
+            });
         cluster.sync();
+        if (rank == 0 && tid == 0) a.tokens[row] = s.found == INT32_MAX ? -1 : s.found;
         return;
     }
-    const float top = value_of((uint32_t)(best >> 32));
-    const double largest = top, scale = 1.4426950408889634074 / (double)t, least = least_of(a, row);
+    top = capped(top), low = capped(low);
+    const uint32_t top_key = key_of(top);
+    const Weights weight_of(top, t, s.roots);
+    const double least = smallest_of(a, row);
     // (fewer maxima than tokens asked for, and too many tokens for the list: the slow way)
     bool slow = use_k && (k > kMostK || (V > kList && k > ctas * kThreads));
     if (slow) {
         cluster.sync();
-        if (rank == 0) sample_slowly(a, s, x, row, (uint32_t)(best >> 32), largest, scale);
+        if (rank == 0) sample_slowly(a, s, x, row, top_key, weight_of);
         return;
     }
     float range = top - low;
     if (!use_k && range > 30.f * t) range = 30.f * t;           // (weights below e**-30 share an interval)
     const float per_bin = range > 0.f ? fminf(kBins / range, FLT_MAX) : 0.f;
-    const auto bin_of = [&](float v) { return min(kBins - 1, (int)((top - v) * per_bin)); };
+    // (rounded by an addition: the conversion unit is slow; of NaN the last)
+    const auto bin_of = [&](float v) { return (int)(__float_as_uint(fminf((top - capped(v)) * per_bin, kBins - 1) + 8388608.f) & (kBins - 1)); };
     constexpr int kEach = kBins / kThreads;
     // counts of all CTAs, of this thread's intervals
     const auto gather = [&](uint32_t (&c)[kEach]) {
@@ -370,7 +423,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
         if (V > kList) {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                if (half_at[j] >= 0) atomicAdd(&s.count[bin_of(half_most[j])], 1u);
+                if (half_most[j] > -INFINITY) atomicAdd(&s.count[bin_of(half_most[j])], 1u);
             uint32_t c[kEach];
             gather(c);
             int total, sum = 0;
@@ -388,7 +441,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
         }
         bool look = lowest == kBins;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) look |= half_at[j] >= 0 && bin_of(half_most[j]) <= lowest;
+        for (int j = 0; j < 2; ++j) look |= half_most[j] > -INFINITY && bin_of(half_most[j]) <= lowest;
         if (look)
             for (int i = i0 + lane * 8; i < i1; i += kStep) {
                 float v[8];
@@ -402,7 +455,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
         if (rank != 0) return;
         const int n = s.listed;
         if (n > kList) {
-            sample_slowly(a, s, x, row, (uint32_t)(best >> 32), largest, scale);
+            sample_slowly(a, s, x, row, top_key, weight_of);
             return;
         }
         sort_places(s.list, n);
@@ -412,7 +465,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int i = 2 * tid + j;
-            w[j] = i < kept_k ? weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots) : 0.0;
+            w[j] = i < kept_k ? weight_of(value_of((uint32_t)(s.list[i] >> 32))) : 0.0;
             sum_w += w[j];
         }
         double before_w = block_scan(sum_w, all, s.scan);
@@ -459,20 +512,18 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
     // ---- 2: the interval in which the nucleus about ends
     int edge = kBins;                                            // everything lies above it
     if (use_p) {
-        for (int i = i0 + lane * 8; i < i1; i += kStep) {
-            float v[8];
-            load_eight(x, i, i1, a.wide, v);
+        each_eight<4>(x, i0, i1, a.wide, [&](const float (&v)[8], int) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (v[j] > -INFINITY) atomicAdd(&s.count[bin_of(v[j])], 1u);
-        }
+        });
         uint32_t c[kEach];
         gather(c);
         // (every CTA finds the same from the same numbers in the same order)
         const float step = per_bin > 0.f ? -1.442695f / (per_bin * t) : 0.f;
         float w[kEach], sum = 0.f, total;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) w[j] = c[j] * exp2f((tid * kEach + j + 0.5f) * step), sum += w[j];
+        for (int j = 0; j < kEach; ++j) w[j] = c[j] * exp2f((tid * kEach + j) * step), sum += w[j];
         if (tid == 0) s.decided = kBins - 1;
         float before = block_scan(sum, total, s.low);
         const float aim = p * total;
@@ -489,22 +540,20 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
     uint64_t border = 0;                                         // the last place that stays
     for (int tries = 0;; ++tries) {
         double above = 0.0, kept = 0.0, below = 0.0;
-        for (int i = i0 + lane * 8; i < i1; i += kStep) {
-            float v[8];
-            load_eight(x, i, i1, a.wide, v);
+        each_eight<2>(x, i0, i1, a.wide, [&](const float (&v)[8], int i) {
             unsigned in = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const double w = weight_of(v[j], largest, scale, s.roots);
+                const double w = weight_of(v[j]);
                 const int bin = use_p ? bin_of(v[j]) : 0;
                 if (bin < edge) above += w;
-                if (bin < edge && w >= least) kept += w;
+                if (least > 0.0 && bin < edge && w >= least) kept += w;
                 if (bin > edge) below += w;
                 in |= (v[j] > -INFINITY && bin == edge ? 1u : 0u) << j;
             }
             list(in, v, i);
-        }
-        above = warp_reduce(above, Plus()), kept = warp_reduce(kept, Plus());
+        });
+        above = warp_reduce(above, Plus()), kept = least > 0.0 ? warp_reduce(kept, Plus()) : above;
         if (lane == 0) first.span_all[me] = above, first.span_kept[me] = kept;
         if (use_p) {
             below = block_reduce(below, Plus(), s.scan);
@@ -520,14 +569,14 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
             } else {
                 sort_places(s.list, n);
                 double over = 0.0, under = 0.0, total, running = 0.0;
-                for (int i = 0; i < spans; ++i) over += s.span_all[i];
+                over = block_reduce(tid < spans ? s.span_all[tid] : 0.0, Plus(), s.scan);
                 for (int r = 0; r < ctas; ++r) under += cluster.map_shared_rank(&s, r)->cta_below;
                 // eight consecutive places per thread
                 constexpr int kPlaces = kList / kThreads;
                 double sum = 0.0;
                 for (int j = 0; j < kPlaces; ++j) {
                     const int i = tid * kPlaces + j;
-                    if (i < n) sum += weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots);
+                    if (i < n) sum += weight_of(value_of((uint32_t)(s.list[i] >> 32)));
                 }
                 running = over + block_scan(sum, total, s.scan);
                 const double aim = (double)p * (over + total + under);
@@ -539,17 +588,20 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
                     for (int j = 0; j < kPlaces; ++j) {
                         const int i = tid * kPlaces + j;
                         if (i >= n) break;
-                        inside += running < aim || s.list[i] == best;
-                        running += weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots);
+                        inside += running < aim || (edge == 0 && i == 0);       // (the very first always stays)
+                        running += weight_of(value_of((uint32_t)(s.list[i] >> 32)));
                     }
                     block_scan(inside, total_inside, s.scan_n);
                     if (tid == 0) s.border = total_inside > 0 ? s.list[total_inside - 1] : 1;
                     // the weights that stay count in their spans, in a fixed order: a warp each
+                    uint8_t *span_of = reinterpret_cast<uint8_t *>(s.count);
+                    for (int i = tid; i < total_inside; i += kThreads) span_of[i] = (uint8_t)(token_of(s.list[i]) / span);
+                    __syncthreads();
                     for (int sp = warp; sp < spans; sp += kWarps) {
                         double more = 0.0;
                         for (int i = lane; i < total_inside; i += 32)
-                            if (token_of(s.list[i]) / span == sp) {
-                                const double w = weight_of(value_of((uint32_t)(s.list[i] >> 32)), largest, scale, s.roots);
+                            if (span_of[i] == sp) {
+                                const double w = weight_of(value_of((uint32_t)(s.list[i] >> 32)));
                                 if (w >= least) more += w;
                             }
                         more = warp_reduce(more, Plus());
@@ -565,7 +617,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
         border = first.border;
         cluster.sync();
         if (next == -2) {
-            if (rank == 0) sample_slowly(a, s, x, row, (uint32_t)(best >> 32), largest, scale);
+            if (rank == 0) sample_slowly(a, s, x, row, top_key, weight_of);
             return;
         }
         if (next == -1) break;
@@ -573,63 +625,87 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
     }
     if (rank != 0) return;
 
-    // ---- the span in which the draw falls, walked by one warp
-    if (warp != 0) return;
-    double total = 0.0, from = 0.0;
-    for (int i = 0; i < spans; ++i) total += s.span_kept[i];
+    // ---- the span in which the draw falls, a step of it per warp, and then the step
+    __syncthreads();
+    double total;
+    const double mine = tid < spans ? s.span_kept[tid] : 0.0, before = block_scan(mine, total, s.scan);
     const double aim = (double)a.uniforms[row] * total;
-    int chosen = -1, last = 0;
-    double sum = 0.0;
-    for (int i = 0; i < spans; ++i) {
-        const double w = s.span_kept[i];
-        if (w > 0.0) last = i;
-        if (chosen < 0 && w > 0.0 && sum + w > aim) chosen = i, from = sum;
-        sum += w;
-    }
-    if (chosen < 0) chosen = last, from = total - s.span_kept[last];
-    int token = -1;
+    // the first part that has a weight and ends above the aim; rounding may leave none, then the last that has one
+    const auto first_above = [&](bool any, bool over, int i) {
+        if (tid == 0) s.found = INT32_MAX, s.decided = -1;
+        __syncthreads();
+        if (any) atomicMax(&s.decided, i);
+        if (any && over) atomicMin(&s.found, i);
+        __syncthreads();
+        const int r = s.found == INT32_MAX ? s.decided : s.found;
+        __syncthreads();
+        return r;
+    };
+    const int chosen = first_above(mine > 0.0, before + mine > aim, tid);
+    if (tid == chosen) s.scan[kWarps] = before;
     const int j0 = chosen * span, j1 = min(j0 + span, V);
-    for (int i = j0 + lane * 8; i - lane * 8 < j1; i += kStep) {
+    double from = 0.0;
+    // (the eight weights of a lane, those that stay)
+    const auto weights_at = [&](int i, double (&w)[8], int &last) {
         float v[8];
         load_eight(x, i, j1, a.wide, v);
-        double w[8], mine = 0.0;
-        int mine_last = -1;
+        double sum = 0.0;
+        last = -1;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            w[j] = 0.0;
-            if (v[j] > -INFINITY && place_of(v[j], i + j) >= border) w[j] = weight_of(v[j], largest, scale, s.roots);
+            w[j] = v[j] > -INFINITY && place_of(v[j], i + j) >= border ? weight_of(v[j]) : 0.0;
             if (w[j] < least) w[j] = 0.0;
-            if (w[j] > 0.0) mine_last = i + j;
-            mine += w[j];
+            if (w[j] > 0.0) last = i + j;
+            sum += w[j];
         }
-        double incl = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const double u = __shfl_up_sync(kFull, incl, d);
-            if (lane >= d) incl += u;
-        }
-        const unsigned over = __ballot_sync(kFull, mine > 0.0 && from + incl > aim);
-        if (over) {
-            const int who = __ffs(over) - 1;
-            if (lane == who) {
-                double f = from + (incl - mine);
-                token = mine_last;
-                for (int j = 0; j < 8; ++j) {
-                    f += w[j];
-                    if (w[j] > 0.0 && f > aim) {
-                        token = i + j;
-                        break;
-                    }
-                }
+        return sum;
+    };
+    // the step of the span: sums of sixteen steps at a time, the last of which has what rounding leaves over
+    int step = -1;
+    double step_from = 0.0;
+    __syncthreads();
+    from = s.scan[kWarps];
+    for (int s0 = j0; s0 < j1; s0 += kWarps * kStep) {
+        double w[8];
+        int last;
+        const double sum = warp_reduce(weights_at(s0 + warp * kStep + lane * 8, w, last), Plus());
+        __syncthreads();
+        if (lane == 0) s.span_all[warp] = sum;
+        __syncthreads();
+        bool over = false;
+        for (int i = 0; i < kWarps && !over; ++i)
+            if (s.span_all[i] > 0.0) {
+                step = s0 + i * kStep, step_from = from;
+                over = from + s.span_all[i] > aim;
+                from += s.span_all[i];
             }
-            token = __shfl_sync(kFull, token, who);
-            break;
-        }
-        // (rounding may leave no sum above the aim: then it is the last token that stays)
-        token = Most()(token, warp_reduce(mine_last, Most()));
-        from += __shfl_sync(kFull, incl, 31);
+        if (over) break;
     }
-    if (lane == 0) a.tokens[row] = token;
+    if (warp != 0) return;
+    double w[8];
+    int last;
+    const double sum = weights_at(step + lane * 8, w, last);
+    double incl = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const double u = __shfl_up_sync(kFull, incl, d);
+        if (lane >= d) incl += u;
+    }
+    const unsigned over = __ballot_sync(kFull, sum > 0.0 && step_from + incl > aim), any = __ballot_sync(kFull, sum > 0.0);
+    const int who = over ? __ffs(over) - 1 : 31 - __clz(any);
+    if (lane == who) {
+        double f = step_from + (incl - sum);
+        int token = last;
+#pragma unroll
+        for (int j = 7; j >= 0; --j) f += w[j];
+        // (backwards: the first that ends above the aim)
+#pragma unroll
+        for (int j = 7; j >= 0; --j) {
+            if (w[j] > 0.0 && f > aim) token = step + lane * 8 + j;
+            f -= w[j];
+        }
+        a.tokens[row] = token;
+    }
 }
 
 template <typename T>
