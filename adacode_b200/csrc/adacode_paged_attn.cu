@@ -884,6 +884,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) k_paged_attn(const __grid_con
             mbar_wait(&s.done, 0, a.status, 1u << 16);
         }
     }
+    // (not earlier: CTAs of the next kernel would take places on the SMs and wait there)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __syncwarp();
     tmem_fence_before();
@@ -896,51 +897,53 @@ __global__ void __launch_bounds__(kAttnThreads, 1) k_paged_attn(const __grid_con
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(256) k_paged_merge(const __grid_constant__ PagedArgs a) {
     constexpr int E = D / 32;
-    const int c = blockIdx.x, row = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x & 31;
+    const int c = blockIdx.x, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Cut cut = a.cuts[c];
-    if (cut.n == 0 || row >= cut.rows) return;
-    const auto piece = [&](int i) { return (long long)(i ? 2 * (c + i) : 2 * c + 1) * ROWS + row; };
-    float m = -INFINITY;
-    for (int i = lane; i < cut.n; i += 32) m = fmaxf(m, a.part_ml[piece(i) * 2]);
+    if (cut.n == 0) return;
+    for (int row = blockIdx.y * 8 + threadIdx.x / 32; row < cut.rows; row += gridDim.y * 8) {
+        const auto piece = [&](int i) { return (long long)(i ? 2 * (c + i) : 2 * c + 1) * ROWS + row; };
+        float m = -INFINITY;
+        for (int i = lane; i < cut.n; i += 32) m = fmaxf(m, a.part_ml[piece(i) * 2]);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, d));
-    float l = 0.f, o[E];
+        for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, d));
+        float l = 0.f, o[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
+        for (int e = 0; e < E; ++e) o[e] = 0.f;
 #pragma unroll 4
-    for (int i = 0; i < cut.n; ++i) {
-        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + piece(i) * 2);
-        if (ml.x == -INFINITY) {
-            if (ml.y != 0.f) l = ml.y;               // (NaN scores; without a maximum the sum is 0 otherwise)
+        for (int i = 0; i < cut.n; ++i) {
+            const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + piece(i) * 2);
+            if (ml.x == -INFINITY) {
+                if (ml.y != 0.f) l = ml.y;               // (NaN scores; without a maximum the sum is 0 otherwise)
+                continue;
+            }
+            const float f = exp2_fast((ml.x - m) * a.scale);
+            l = fmaf(ml.y, f, l);
+            const float *src = a.part_o + piece(i) * D + lane * E;
+            if constexpr (E == 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(src);
+                o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]), o[2] = fmaf(v.z, f, o[2]), o[3] = fmaf(v.w, f, o[3]);
+            } else {
+                const float2 v = *reinterpret_cast<const float2 *>(src);
+                o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]);
+            }
+        }
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < E; ++e) odd |= !isfinite(o[e]);
+        if (__any_sync(kFull, odd) && isfinite(l)) {
+            repair_row<T, D>(a, cut.b, cut.h, cut.q0, cut.fresh, cut.len, cut.start, cut.row0 + row, 0, D);
             continue;
         }
-        const float f = exp2_fast((ml.x - m) * a.scale);
-        l = fmaf(ml.y, f, l);
-        const float *src = a.part_o + piece(i) * D + lane * E;
-        if constexpr (E == 4) {
-            const float4 v = *reinterpret_cast<const float4 *>(src);
-            o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]), o[2] = fmaf(v.z, f, o[2]), o[3] = fmaf(v.w, f, o[3]);
-        } else {
-            const float2 v = *reinterpret_cast<const float2 *>(src);
-            o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]);
-        }
-    }
-    bool odd = false;
+        const int t = (int)((uint32_t)(cut.row0 + row) / a.by_group), head = cut.h * a.G + cut.row0 + row - t * a.G;
+        T *out = reinterpret_cast<T *>(a.out) + (long long)(cut.q0 + t) * a.o_n + head * a.o_h + lane * E;
+        const float share = l == 0.f ? 0.f : 1.f / l;
+        uint32_t w[E / 2];
 #pragma unroll
-    for (int e = 0; e < E; ++e) odd |= !isfinite(o[e]);
-    if (__any_sync(kFull, odd) && isfinite(l)) {
-        repair_row<T, D>(a, cut.b, cut.h, cut.q0, cut.fresh, cut.len, cut.start, cut.row0 + row, 0, D);
-        return;
+        for (int e = 0; e < E; e += 2) w[e / 2] = l == 0.f ? 0u : pack_two<T>(o[e] * share, o[e + 1] * share);
+        if constexpr (E == 4) *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t *>(out) = w[0];
     }
-    const int t = (int)((uint32_t)(cut.row0 + row) / a.by_group), head = cut.h * a.G + cut.row0 + row - t * a.G;
-    T *out = reinterpret_cast<T *>(a.out) + (long long)(cut.q0 + t) * a.o_n + head * a.o_h + lane * E;
-    const float share = l == 0.f ? 0.f : 1.f / l;
-    uint32_t w[E / 2];
-#pragma unroll
-    for (int e = 0; e < E; e += 2) w[e / 2] = l == 0.f ? 0u : pack_two<T>(o[e] * share, o[e + 1] * share);
-    if constexpr (E == 4) *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint32_t *>(out) = w[0];
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1003,7 +1006,7 @@ cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, int threads, s
 }
 
 template <typename T, int D, bool SOLO>
-int launch_paged(const PagedArgs &a, const CUtensorMap &keys, const CUtensorMap &values, int ctas, cudaStream_t st) {
+int launch_paged(const PagedArgs &a, const CUtensorMap &keys, const CUtensorMap &values, int ctas, int max_query_len, cudaStream_t st) {
     // the kernel's limit of dynamic shared memory is raised once per device
     static std::atomic<bool> done[64];
     int dev = 0;
@@ -1019,13 +1022,15 @@ int launch_paged(const PagedArgs &a, const CUtensorMap &keys, const CUtensorMap 
     static std::mutex locks[64];
     const std::lock_guard<std::mutex> both(locks[((uintptr_t)a.part_o >> 9) * 0x9E3779B97F4A7C15ull >> 58]);
     if (launch_dependent(k_paged_attn<T, D, SOLO>, dim3(ctas), kAttnThreads, bytes, st, a, keys, values) != cudaSuccess) return ADACODE_ERR_CUDA;
-    return launch_dependent(k_paged_merge<T, D, rows>, dim3(ctas, rows / 8), 256, 0, st, a) == cudaSuccess ? ADACODE_OK : ADACODE_ERR_CUDA;
+    // (a warp per row, as many as a unit can have by max_query_len)
+    const long long most = (long long)max_query_len * a.G, y = most < rows ? (most + 7) / 8 : rows / 8;
+    return launch_dependent(k_paged_merge<T, D, rows>, dim3(ctas, y < 1 ? 1 : (unsigned)y), 256, 0, st, a) == cudaSuccess ? ADACODE_OK : ADACODE_ERR_CUDA;
 }
 
 template <typename T>
-int launch_paged(const PagedArgs &a, bool solo, const CUtensorMap &keys, const CUtensorMap &values, int ctas, cudaStream_t st) {
-    if (a.cache.D == 128) return solo ? launch_paged<T, 128, true>(a, keys, values, ctas, st) : launch_paged<T, 128, false>(a, keys, values, ctas, st);
-    return solo ? launch_paged<T, 64, true>(a, keys, values, ctas, st) : launch_paged<T, 64, false>(a, keys, values, ctas, st);
+int launch_paged(const PagedArgs &a, bool solo, const CUtensorMap &keys, const CUtensorMap &values, int ctas, int max_query_len, cudaStream_t st) {
+    if (a.cache.D == 128) return solo ? launch_paged<T, 128, true>(a, keys, values, ctas, max_query_len, st) : launch_paged<T, 128, false>(a, keys, values, ctas, max_query_len, st);
+    return solo ? launch_paged<T, 64, true>(a, keys, values, ctas, max_query_len, st) : launch_paged<T, 64, false>(a, keys, values, ctas, max_query_len, st);
 }
 
 }  // namespace
@@ -1072,8 +1077,8 @@ int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int6
         !map_pages(values, cache->value_pages, *cache, cache->value_page, cache->value_head, cache->value_slot, a.box_rows))
         return ADACODE_ERR_INVALID_ARG;
     const cudaStream_t st = (cudaStream_t)stream;
-    const int rc = cache->dtype == ADACODE_BF16 ? launch_paged<__nv_bfloat16>(a, solo, keys, values, ctas, st)
-                                                : launch_paged<__half>(a, solo, keys, values, ctas, st);
+    const int rc = cache->dtype == ADACODE_BF16 ? launch_paged<__nv_bfloat16>(a, solo, keys, values, ctas, max_query_len, st)
+                                                : launch_paged<__half>(a, solo, keys, values, ctas, max_query_len, st);
     if (rc != ADACODE_OK) (void)cudaGetLastError();
     return rc;
 }

@@ -1,7 +1,7 @@
 // One token per row of logits: temperature, top-k, top-p, min-p and the draw from a given uniform number.
 //
 // Every cut (the top_k first, the nucleus, min_p) keeps a prefix of the order (descending logit, ascending token); tokens are kept
-// as 64-bit keys of that order.  A row has a cluster of 1 to 8 CTAs, whose warps own consecutive spans of the vocabulary.  Passes over the row, which
+// as 64-bit keys of that order.  A row has a cluster of 1 to 4 CTAs, whose warps own consecutive spans of the vocabulary.  Passes over the row, which
 // after the first come from L2:
 //   1  the largest logit, and of every thread the largest of its tokens, in two halves.
 //   top_k up to kMostK: the k-th largest of those many maxima has at least k tokens above it, and hardly more.  Threads whose maxima reach it list
@@ -27,7 +27,7 @@ namespace {
 
 constexpr unsigned kFull = 0xFFFFFFFFu;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kMostCtas = 8;             // per row
+constexpr int kMostCtas = 4;             // per row
 constexpr int kStep = 256;               // tokens that a warp takes at a time, eight per lane
 constexpr int kBins = 2048;
 constexpr int kList = 4096;
@@ -73,7 +73,7 @@ __device__ __forceinline__ uint64_t place_of(float v, int token) { return (uint6
 __device__ __forceinline__ int token_of(uint64_t place) { return (int)(0xFFFFFFFFu - (uint32_t)place); }
 
 struct Shared {
-    double roots[32];                    // 2**(j / 32)
+    double roots[128];                   // 2**(j / 128)
     uint32_t count[kBins];               // (later: the span of every listed token)
     uint64_t list[kList];
     double line[kMostK];
@@ -87,24 +87,26 @@ struct Shared {
     uint64_t border;
 };
 
-// What turns a logit into its weight: w = exp((x - largest) / T) = 2**((x - largest) k).  Below `floor` (600 T from the largest) it is 0.
+// What turns a logit into its weight: w = exp((x - largest) / T) = 2**(x k - largest k).  Below `floor` (600 T from the largest) it is 0.  (The largest
+// logit's own is 1 but for a rounding; what is compared with it is compared with that.)
 struct Weights {
-    double largest, k;
+    double k, shift;
     float floor;
     const double *roots;
     __device__ Weights(float top, float t, const double *roots)
-        : largest(top), k(1.4426950408889634074 / (double)t), floor(fmaxf(top - 600.f * t, -FLT_MAX)), roots(roots) {}
-    // The exponent rounded to 1/32, the rest's power by its Taylor series (degree 4, |rest ln 2| <= ln 2 / 64: the next term is below 1.3e-12), 32 roots of
-    // 2.  Half the time of exp() (64-bit), whose last bits no draw needs.
+        : k(1.4426950408889634074 / (double)t), shift(-(double)top * k), floor(fmaxf(top - 600.f * t, -FLT_MAX)), roots(roots) {}
+    // The exponent rounded to 1/128; the power of the rest r by the Taylor series of 2**r (degree 3, |r| <= 1/256: the next term is below 2.3e-12);
+    // 128 roots of 2.  Eight operations of 64 bits, less than half the time of exp(), whose last bits no draw needs.
     __device__ __forceinline__ double operator()(float v) const {
-        const double t = ((double)capped(v) - largest) * k;
-        constexpr double kShift = 6755399441055744.0 / 32.0;       // 1.5 x 2**52 / 32
+        const double t = fma((double)capped(v), k, shift);
+        constexpr double kShift = 6755399441055744.0 / 128.0;      // 1.5 x 2**52 / 128
         const double shifted = t + kShift;
         const int n = __double2loint(shifted);
-        const double r = (t - (shifted - kShift)) * 0.69314718055994530942;
-        const double power = fma(fma(fma(fma(r, 1.0 / 24.0, 1.0 / 6.0), r, 0.5), r, 1.0), r, 1.0) * roots[n & 31];
+        const double r = t - (shifted - kShift);
+        constexpr double kLn2 = 0.69314718055994530942;
+        const double power = fma(fma(fma(r, kLn2 * kLn2 * kLn2 / 6.0, kLn2 * kLn2 / 2.0), r, kLn2), r, 1.0) * roots[n & 127];
         const bool any = v >= floor;                               // (not NaN)
-        return __hiloint2double(any ? __double2hiint(power) + ((n >> 5) << 20) : 0, any ? __double2loint(power) : 0);
+        return __hiloint2double(any ? __double2hiint(power) + ((n >> 7) << 20) : 0, any ? __double2loint(power) : 0);
     }
 };
 
@@ -279,7 +281,7 @@ __device__ void sample_slowly(const SampleArgs &a, Shared &s, const T *x, int ro
         ties = lo == cut && ties < n ? ties : n;
         cut = lo;
     }
-    const double least = smallest_of(a, row);
+    const double least = smallest_of(a, row) * weight_of(value_of(top));
     // runs of consecutive tokens per thread: ties before it, weight before it, the token
     const int per = (V + kThreads - 1) / kThreads, i0 = min(tid * per, V), i1 = min(i0 + per, V);
     int same = 0, all_same = 0;
@@ -355,7 +357,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
                 if (v[j] > -INFINITY && v[j] < low) low = v[j];
         });
     }
-    if (tid < 32) s.roots[tid] = exp2((double)tid / 32.0);
+    if (tid < 128) s.roots[tid] = exp2((double)tid / 128.0);
     if (tid == 0) s.listed = 0, s.found = INT32_MAX;
     for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
     float top = block_reduce(fmaxf(half_most[0], half_most[1]), Most(), s.low);
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
     top = capped(top), low = capped(low);
     const uint32_t top_key = key_of(top);
     const Weights weight_of(top, t, s.roots);
-    const double least = smallest_of(a, row);
+    const double least = smallest_of(a, row) * weight_of(top);
     // (fewer maxima than tokens asked for, and too many tokens for the list: the slow way)
     bool slow = use_k && (k > kMostK || (V > kList && k > ctas * kThreads));
     if (slow) {
@@ -536,6 +538,23 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
         edge = s.decided;
     }
 
+    // the smallest logit whose weight stays, by a search of the keys 32 at a time (weights of neighbours differ by far more than the rounding)
+    float kept_from = -FLT_MAX;
+    if (least > 0.0) {
+        uint32_t lo = key_of(-FLT_MAX), hi = top_key;           // (the first that stays is one of lo .. hi)
+        while (lo < hi) {
+            const uint32_t stride = (hi - lo) / 32 + 1, mid = lo + lane * stride;
+            const unsigned stays = __ballot_sync(kFull, mid >= hi || weight_of(value_of(mid)) >= least);
+            if (stays == kFull) hi = lo;
+            else if (stays == 0) lo += 31 * stride + 1;
+            else {
+                const uint32_t at = lo + (__ffs(stays) - 1) * stride;
+                lo = at - stride + 1, hi = at < hi ? at : hi;
+            }
+        }
+        kept_from = value_of(lo);
+    }
+
     // ---- 3: what lies above the interval, per span, below it, and what lies in it
     uint64_t border = 0;                                         // the last place that stays
     for (int tries = 0;; ++tries) {
@@ -547,7 +566,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
                 const double w = weight_of(v[j]);
                 const int bin = use_p ? bin_of(v[j]) : 0;
                 if (bin < edge) above += w;
-                if (least > 0.0 && bin < edge && w >= least) kept += w;
+                if (least > 0.0 && bin < edge && v[j] >= kept_from) kept += w;
                 if (bin > edge) below += w;
                 in |= (v[j] > -INFINITY && bin == edge ? 1u : 0u) << j;
             }
@@ -736,14 +755,11 @@ extern "C" int adacode_sample_tokens(const void *logits, int64_t row_stride, int
     const int size = dtype == ADACODE_FP32 ? 4 : 2;
     const bool wide = ((uintptr_t)logits & 15) == 0 && (row_stride * size) % 16 == 0;
     const SampleArgs a{logits, row_stride, V, wide, uniforms, temperature, top_p, min_p, top_k, tokens, temperature_all, top_p_all, min_p_all, top_k_all};
-    // CTAs per row: the number that makes the rounds of two CTAs on each of 148 SMs shortest, fewer on ties, as long as every warp has a
-    // step of the vocabulary.  192 rows of 151936: three, two rounds of a third of a row each (two: two of a half).
+    // CTAs per row: up to four, as long as all rows' make no more than three for each of 148 SMs (two fit at a time; more rounds than that only add
+    // the rows' ends) and every warp has a step of the vocabulary.  192 rows of 151936: 218 us with one, 159 with two, 193 with four; 64 rows of
+    // 128256: 34, 22, 21.5 and 37 with eight; one row of 32000: 16, 12.6, 11 and 11.2.
     int ctas = 1;
-    double best = 1e30;
-    for (int n = 1; n <= kMostCtas && (n == 1 || (int64_t)(n - 1) * kWarps * kStep < V); ++n) {
-        const double rounds = (double)(((int64_t)B * n + 295) / 296) / n;
-        if (rounds < best * 0.95) best = rounds, ctas = n;
-    }
+    while (ctas < kMostCtas && (int64_t)B * ctas * 2 <= 3 * 148 && V > ctas * kWarps * kStep) ctas *= 2;
     cudaStream_t st = (cudaStream_t)stream;
     const cudaError_t e = dtype == ADACODE_BF16 ? launch<__nv_bfloat16>(a, B, ctas, st)
                           : dtype == ADACODE_FP16 ? launch<__half>(a, B, ctas, st)
