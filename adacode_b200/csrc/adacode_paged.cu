@@ -141,6 +141,11 @@ int adacode_append_rotary(const adacode_paged_cache *cache, const adacode_rotary
                           int32_t *status, void *stream) {
     if (!valid(cache) || !rotary || !status || !key || !value || Hq < 0 || (Hq > 0 && (!query || !query_out))) return ADACODE_ERR_INVALID_ARG;
     const adacode_rotary &r = *rotary;
+    const adacode_paged_cache given = used_strides(*cache);
+    cache = &given;
+    if (cache->N == 1) query_token = out_token = key_token = value_token = 0;
+    if (Hq == 1) query_head = out_head = 0;
+    if (cache->Hkv == 1) key_head = value_head = 0;
     if (cache->D <= 0 || cache->D % 2 != 0 || cache->D > 512 || r.half < 0 || 2 * r.half > cache->D || r.axes < 1 || r.axes > 4)
         return ADACODE_ERR_INVALID_ARG;
     if (r.half > 0 && (!r.cos || !r.sin)) return ADACODE_ERR_INVALID_ARG;

@@ -420,7 +420,8 @@ __device__ __forceinline__ int find_run(const PagedArgs &a, int cta, Piece &p, i
         const uint32_t upto = from + warp_scan(w * c.Hkv);
         const unsigned later = __ballot_sync(kFull, upto > x);
         if (later || b0 + 32 >= c.B) {
-            const int l = later ? __ffs(later) - 1 : 31;
+            // (the bounds here and below only matter if lengths change while the kernel runs)
+            const int l = later ? __ffs(later) - 1 : c.B - 1 - b0;
             p.b = b0 + l;
             per_head = __shfl_sync(kFull, w, l);
             from = __shfl_sync(kFull, upto, l) - per_head * c.Hkv;
@@ -429,15 +430,17 @@ __device__ __forceinline__ int find_run(const PagedArgs &a, int cta, Piece &p, i
         from = __shfl_sync(kFull, upto, 31);
     }
     sequence(a, p.b, p.q0, p.fresh, p.len, p.start);
+    if (per_head == 0 || p.fresh == 0) return 0;
     p.h = (int)((x - from) / per_head);
+    if (p.h >= c.Hkv) p.h = c.Hkv - 1;
     from += p.h * per_head;
     for (p.row0 = 0;; p.row0 += ROWS) {
         p.rows = p.fresh * a.G - p.row0 < ROWS ? p.fresh * a.G - p.row0 : ROWS;
         const uint32_t n = unit_tiles(a, p.row0, p.row0 + p.rows, p.fresh, p.len, p.start, p.j0);
-        if (x < from + n) break;
+        skipped = x < from + n ? (int)(x - from) : (int)n - 1;
+        if (x < from + n || p.row0 + ROWS >= p.fresh * a.G) break;
         from += n;
     }
-    skipped = (int)(x - from);
     return (int)(end - x);
 }
 
@@ -549,8 +552,10 @@ __device__ __forceinline__ void load_keys(const PagedArgs &a, Shared<D, SOLO> &s
             p.row0 = 0;
             if (++p.h == c.Hkv) {
                 p.h = 0;
+                if (p.b + 1 >= c.B) break;
                 do sequence(a, ++p.b, p.q0, p.fresh, p.len, p.start);
                 while (p.fresh == 0 && p.b + 1 < c.B);
+                if (p.fresh == 0) break;
             }
         }
         p.rows = p.fresh * a.G - p.row0 < S::kRows ? p.fresh * a.G - p.row0 : S::kRows;
@@ -1046,6 +1051,10 @@ int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int6
                        void *out, int64_t out_token, int64_t out_head, const int32_t *seq_starts, int max_query_len, float scale, int causal,
                        int window, void *workspace, size_t workspace_bytes, int32_t *status, void *stream) {
     if (!valid(cache) || !status || Hq <= 0 || Hq % cache->Hkv != 0 || window < 0 || max_query_len < 0) return ADACODE_ERR_INVALID_ARG;
+    const adacode_paged_cache given = used_strides(*cache);
+    cache = &given;
+    if (cache->N == 1) query_token = out_token = 0;
+    if (Hq == 1) query_head = out_head = 0;
     const int D = cache->D;
     if (D != 64 && D != 128) return ADACODE_ERR_INVALID_ARG;
     const bool one_page = cache->table_width == 1;

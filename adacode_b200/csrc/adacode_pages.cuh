@@ -46,3 +46,11 @@ bool valid(const adacode_paged_cache *c) {
            c->table_width > 0 && c->Hkv > 0 && c->N >= 0 && (c->dtype == ADACODE_BF16 || c->dtype == ADACODE_FP16) &&
            (c->cu_seqlens || c->N % c->B == 0);
 }
+
+// A dimension of one entry may have any stride: none that alignment or a tensor map would stumble over.
+adacode_paged_cache used_strides(adacode_paged_cache c) {
+    if (c.n_pages == 1) c.key_page = c.value_page = 0;
+    if (c.Hkv == 1) c.key_head = c.value_head = 0;
+    if (c.page_size == 1) c.key_slot = c.value_slot = 0;
+    return c;
+}

@@ -21,6 +21,8 @@
 
 #include "adacode.h"
 
+#include <atomic>
+
 namespace cg = cooperative_groups;
 
 namespace {
@@ -88,13 +90,14 @@ struct Shared {
 };
 
 // What turns a logit into its weight: w = exp((x - largest) / T) = 2**(x k - largest k).  Below `floor` (600 T from the largest) it is 0.  (The largest
-// logit's own is 1 but for a rounding; what is compared with it is compared with that.)
+// logit's own is 1 but for a rounding; what is compared with it is compared with that.  Where k would take x k beyond 2**40, at temperatures
+// that leave the largest logit alone, it is held there: its neighbours are then 2**16 powers of two away.)
 struct Weights {
     double k, shift;
     float floor;
     const double *roots;
     __device__ Weights(float top, float t, const double *roots)
-        : k(1.4426950408889634074 / (double)t), shift(-(double)top * k), floor(fmaxf(top - 600.f * t, -FLT_MAX)), roots(roots) {}
+        : k(fmin(1.4426950408889634074 / (double)t, 1099511627776.0 / fabs((double)top))), shift(-(double)top * k), floor(fmaxf(top - 600.f * t, -FLT_MAX)), roots(roots) {}
     // The exponent rounded to 1/128; the power of the rest r by the Taylor series of 2**r (degree 3, |r| <= 1/256: the next term is below 2.3e-12);
     // 128 roots of 2.  Eight operations of 64 bits, less than half the time of exp(), whose last bits no draw needs.
     __device__ __forceinline__ double operator()(float v) const {
@@ -730,8 +733,16 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
 template <typename T>
 cudaError_t launch(const SampleArgs &a, int B, int ctas, cudaStream_t st) {
     static_assert(sizeof(Shared) <= 64 * 1024, "three CTAs per SM");
-    const cudaError_t raised = cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared));
-    if (raised != cudaSuccess) return raised;
+    // the kernel's limit of dynamic shared memory is raised once per device
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared));
+        if (e != cudaSuccess) return e;
+        if (dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)B * ctas), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = sizeof(Shared), cfg.stream = st;
     cudaLaunchAttribute attr[2];

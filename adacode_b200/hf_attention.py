@@ -45,8 +45,8 @@ def float11_fused_attention(module, query, key, value, attention_mask, dropout: 
             getattr(cache, '_fused_decode', False):
         layer = cache.layers[module.layer_idx]
         if chunks:
-            starts = None if attention_mask is None else _left_padding(cache, attention_mask, layer.get_seq_length())
             window = getattr(module, 'sliding_window', None) or 0
+            starts = None if attention_mask is None else _left_padding(cache, attention_mask, layer.get_seq_length(), window)
             if query.shape[2] > 1 or starts is not None or window:
                 return layer.chunk_attention(query, scale=scaling, seq_starts=starts, window=window).transpose(1, 2).contiguous(), None
             return layer.decode_attention(query, scale=scaling).transpose(1, 2).contiguous(), None
@@ -78,23 +78,28 @@ def _behind_prefill(cache, module, query: torch.Tensor) -> bool:
     return cache.layers[module.layer_idx].get_seq_length() > query.shape[2]
 
 
-def _left_padding(cache, mask: torch.Tensor, total: int) -> Optional[torch.Tensor]:
-    """First visible position of every sequence (int32 [B]) of a mask that is causal behind left padding; None where nothing is
-    padded.  All layers of a forward pass get the same mask object, so the (synchronising) check runs once per pass."""
-    seen = getattr(cache, '_fused_mask_seen', None)
-    if seen is not None and seen[0] is mask:
-        return seen[1]
+def _left_padding(cache, mask: torch.Tensor, total: int, window: int) -> Optional[torch.Tensor]:
+    """First visible position of every sequence (int32 [B]) of a mask that is causal, with the layer's sliding window, behind left padding;
+    None where nothing is padded.  All layers of a kind get the same mask object in a forward pass, so the (synchronising) check runs
+    once per pass and kind."""
+    known = [k for k in getattr(cache, '_fused_masks_known', ()) if k[0] is mask and k[1] == window]
+    if known:
+        return known[0][2]
     visible = mask if mask.dtype == torch.bool else mask == 0
     B, T = visible.shape[0], visible.shape[2]
     if visible.shape[3] != total:
         raise NotImplementedError(f'float11_fused attention: a mask of {visible.shape[3]} positions for {total} cached tokens')
     j = torch.arange(total, device=mask.device)
-    starts = visible[:, 0, -1].to(torch.int8).argmax(-1)
-    causal = (j >= starts[:, None, None]) & (j <= torch.arange(total - T, total, device=mask.device)[:, None])
+    at = torch.arange(total - T, total, device=mask.device)[:, None]
+    # (with a window, the last query does not see where its sequence begins: the first one may)
+    starts = visible[:, 0].any(1).to(torch.int8).argmax(-1)
+    causal = (j >= starts[:, None, None]) & (j <= at)
+    if window:
+        causal &= j > at - window
     if not bool((visible == causal[:, None]).all()):
         raise NotImplementedError('float11_fused attention takes masks that are causal behind left padding; use the materialising path')
     out = starts.to(torch.int32) if bool((starts > 0).any()) else None
-    cache._fused_mask_seen = (mask, out)
+    cache._fused_masks_known = [*getattr(cache, '_fused_masks_known', ())[-3:], (mask, window, out)]
     return out
 
 
@@ -128,4 +133,5 @@ def fused_decode(cache, model=None, chunks: bool = False):
     finally:
         cache._fused_decode = cache._fused_chunks = False
         cache._fused_mask_seen = None
+        cache._fused_masks_known = []
         _active_cache = previous

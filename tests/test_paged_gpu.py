@@ -423,6 +423,48 @@ def test_repeated_calls_give_the_same_bits():
             assert torch.equal(paged_attention(q, k, v, table, seq), first)
 
 
+def test_strides_of_single_entries_do_not_matter():
+    """Dimensions of one entry with strides that no alignment allows."""
+    from adacode_b200 import append_rotary, paged_attention
+    storage = torch.randn(1 << 16, device='cuda').bfloat16()
+    k, v = (storage[o:].as_strided((1, 1, 128, 64), (7, 13, 64, 1)) for o in (0, 1 << 14))
+    q = storage[1 << 15:].as_strided((1, 1, 64), (5, 3, 1))
+    table, seq = torch.zeros((1, 1), dtype=I32, device='cuda'), torch.tensor([100], dtype=I32, device='cuda')
+    want, size = oracle.attention(q, k, v, table, [100], [1])
+    close(paged_attention(q, k, v, table, seq), want, size, torch.bfloat16, 100)
+    x, c = q.clone(), torch.ones((1, 32), device='cuda')
+    append_rotary(x, x, c, 0 * c, k, v, table, seq)
+    assert torch.equal(v[0, 0, 99], x[0, 0]) and torch.equal(k[0, 0, 99], x[0, 0])
+
+
+def test_inference_mode_and_grad_mode():
+    from adacode_b200 import append_rotary, paged_attention
+    k, v, table, seq = oracle.make_cache([20], 2, 64, 16, torch.bfloat16)
+    x, c = torch.randn((1, 2, 64), device='cuda').bfloat16(), torch.ones((1, 32), device='cuda')
+    with torch.inference_mode():
+        ki, vi = k.clone(), v.clone()
+        append_rotary(x, x, c, 0 * c, ki, vi, table, seq, query=x)
+        got = paged_attention(x, ki, vi, table, seq)
+    with pytest.raises(RuntimeError, match='inference'):
+        append_rotary(x, x, c, 0 * c, ki, vi, table, seq)
+    append_rotary(x, x, c, 0 * c, k, v, table, seq)
+    assert torch.equal(paged_attention(x, k, v, table, seq), got)
+    with pytest.raises(RuntimeError, match='backward'):
+        append_rotary(x.clone().requires_grad_(), x, c, 0 * c, k, v, table, seq)
+    with pytest.raises(ValueError, match='is on cpu'):
+        paged_attention(x, k, v, table, seq.cpu())
+
+
+def test_many_sequences_and_heads_per_group():
+    """More sequences than a warp has lanes, some without new tokens; many query heads on one cached head."""
+    g = torch.Generator('cpu').manual_seed(4)
+    new = [int(n) for n in torch.randint(0, 4, (200,), generator=g)]
+    lens = [n + int(m) for n, m in zip(new, torch.randint(0, 300, (200,), generator=g))]
+    run_case(new, [max(n, 1) for n in lens], 4, 2, 64, 32, 'bf16')
+    run_case([3, 1], [500, 200], 96, 1, 128, 64, 'bf16')
+    run_case([1, 1], [300, 200], 300, 1, 64, 64, 'fp16')
+
+
 def test_versions_are_counted():
     from adacode_b200 import append_rotary
     k, v, table, seq = oracle.make_cache([20], 2, 64, 16, torch.bfloat16)

@@ -78,6 +78,21 @@ def test_forbidden_tokens_and_empty_rows():
             assert got[0] == got[1] == -1 and got[2] >= 900 and 0 <= got[3] < 3 and got[4] in (17, 400) and got[5] == 0
 
 
+def test_tiny_and_huge_temperatures():
+    """Temperatures at which only the largest logits count, and at which all count alike."""
+    g = torch.Generator('cpu').manual_seed(12)
+    logits = torch.randn((4, 900), generator=g).cuda()
+    logits[:, 100], logits[:, 700] = 9.0, 9.0
+    logits[3] *= -1e30
+    u = torch.tensor([0.0, 0.4, 0.6, 0.9], device='cuda')
+    for t in (1e-45, 1e-38, 1e-20, 1e-6, 1e-3):
+        for s in (dict(), dict(top_k=5), dict(top_p=0.9), dict(min_p=1.0)):
+            got = check(logits, u, temperature=t, **s)
+            assert got[:3] == [100, 100, 700]
+    for s in (dict(), dict(top_k=100), dict(top_p=0.5)):
+        check(logits[:3], u[:3], temperature=3e38, **s)
+
+
 def test_distribution():
     """Even steps of the uniform number give every token its share, to within one step."""
     from adacode_b200 import sample_tokens
