@@ -35,10 +35,11 @@ struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Chunk {
 
 // `group` threads (whole warps) have one token; a thread one pair of V-column chunks of every so manieth head, whose angles it keeps.  The chunks
 // of a pair are rotated against each other (half-split), lie side by side (interleaved), or are copied (columns that are not rotated, and
-// values).  Bound by memory where tokens are many, by the latency of finding a token's page where they are few: what does not depend on the
-// page (angles, the first head) is on its way before the page is looked for, and the next head's loads before a head is stored.
+// values).  Bound by memory where tokens are many (13 854 tokens of 48 heads of 128 move 348 MB in 60 us, 5.8 TB/s; that takes four CTAs on an
+// SM, so 64 registers: with the next head's loads on their way early it is three and 68 us, with two more heads 82 to 159), by the
+// latency of finding a token's page where they are few.
 template <typename T, typename A, int V, bool INTERLEAVED>
-__global__ void __launch_bounds__(256, 3) k_append_rotary(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(256, 4) k_append_rotary(const __grid_constant__ AppendArgs a) {
     const adacode_paged_cache &c = a.cache;
     const adacode_rotary &r = a.rotary;
     const int tid = threadIdx.x % a.group, i = blockIdx.x * (blockDim.x / a.group) + threadIdx.x / a.group;
@@ -56,7 +57,6 @@ __global__ void __launch_bounds__(256, 3) k_append_rotary(const __grid_constant_
         x = *reinterpret_cast<const Chunk<T, V> *>(src + lo), y = *reinterpret_cast<const Chunk<T, V> *>(src + hi);
     };
     Chunk<T, V> x, y;
-    if (first < heads) load(first, x, y);
     float cs[V], sn[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) cs[j] = 1.f, sn[j] = 0.f;
@@ -82,8 +82,8 @@ __global__ void __launch_bounds__(256, 3) k_append_rotary(const __grid_constant_
     const int at = c.seq_lens[b] - end + i, page = page_of(c, b, at, slot);
     if (page < 0 && tid == 0) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
     for (int h = first; h < heads; h += step) {
+        load(h, x, y);
         Chunk<T, V> u = x, v = y;
-        if (h + step < heads) load(h + step, x, y);
         if (turned && h < rotated) {
             const Chunk<T, V> p = u, q = v;
 #pragma unroll
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(256, 3) k_append_rotary(const __grid_constant_
 template <typename T, typename A, int V>
 cudaError_t launch_append(AppendArgs &a, cudaStream_t st) {
     // Threads per token: eight warps where tokens are few, down to one where they fill half of the GPU's threads that way.  32 tokens of 48 heads
-    // of 128: 3.1 us with eight, 8.2 with one; 3090 tokens of 20 heads: 24.8 and 8.6; 13 854 tokens of 48 heads: 108 and 68 (5.1 TB/s).
+    // of 128: 2.9 us with eight, 8.2 with one; 3090 tokens of 20 heads: 24.8 and 8.1; 13 854 tokens of 48 heads: 108 and 60.
     const int pairs = a.cache.D / (2 * V);
     a.group = 256;
     while (a.group > 32 && a.group / 2 >= pairs && (int64_t)a.cache.N * a.group > 148 * 1024) a.group /= 2;
