@@ -28,6 +28,7 @@
 #include "adacode.h"
 
 #include <atomic>
+#include <cmath>
 #include <mutex>
 
 namespace {
@@ -53,7 +54,8 @@ struct PagedArgs {
     long long q_n, q_h, o_n, o_h;
     const int32_t *starts;
     int Hq, G, causal, window;
-    float scale;              // times log2 e, not negative (queries are negated where it is)
+    float scale;              // times log2 e, positive (queries are negated where it is negative; 0 is the smallest there is: hidden
+                              // scores are minus infinity, and that times 0 is no number)
     uint32_t negate;
     int box_rows;             // rows per tensor copy
     int room;                 // positions that the table has
@@ -232,7 +234,7 @@ __device__ __forceinline__ void weigh(const uint32_t (&x)[32], Two c, Two base, 
 __device__ __forceinline__ void seen_by(const PagedArgs &a, int t, int fresh, int len, int start, int &lo, int &hi) {
     const int at = len - fresh + t;
     lo = start > 0 ? start : 0;
-    if (a.window > 0 && at - lo >= a.window) lo = at - a.window + 1;
+    if (a.window > 0 && at >= 0 && at - lo >= a.window) lo = at - a.window + 1;
     hi = a.causal && at + 1 < len ? at + 1 : len;
     if (hi > a.room) hi = a.room;
 }
@@ -1050,7 +1052,7 @@ size_t adacode_paged_attn_workspace_bytes(int max_query_len, int Hq, int Hkv, in
 int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int64_t query_token, int64_t query_head, int Hq,
                        void *out, int64_t out_token, int64_t out_head, const int32_t *seq_starts, int max_query_len, float scale, int causal,
                        int window, void *workspace, size_t workspace_bytes, int32_t *status, void *stream) {
-    if (!valid(cache) || !status || Hq <= 0 || Hq % cache->Hkv != 0 || window < 0 || max_query_len < 0) return ADACODE_ERR_INVALID_ARG;
+    if (!valid(cache) || !status || Hq <= 0 || Hq % cache->Hkv != 0 || window < 0 || max_query_len < 0 || !std::isfinite(scale)) return ADACODE_ERR_INVALID_ARG;
     const adacode_paged_cache given = used_strides(*cache);
     cache = &given;
     if (cache->N == 1) query_token = out_token = 0;
@@ -1065,7 +1067,7 @@ int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int6
                             cache->value_page | cache->value_head | cache->value_slot;
     if ((pointers & 15) != 0 || (strides & 7) != 0) return ADACODE_ERR_INVALID_ARG;
     if (cache->N == 0) return ADACODE_OK;
-    if (!query || !out || !workspace || (long long)cache->N * (Hq / cache->Hkv) >= 1ll << 31 || cache->n_pages == INT32_MAX) return ADACODE_ERR_INVALID_ARG;
+    if (!query || !out || query == out || !workspace || (long long)cache->N * (Hq / cache->Hkv) >= 1ll << 31 || cache->n_pages == INT32_MAX) return ADACODE_ERR_INVALID_ARG;
     const int G = Hq / cache->Hkv, ctas = sm_count();
     const bool solo = is_solo(max_query_len, G);
     if (workspace_bytes < workspace_bytes_of(solo, D)) return ADACODE_ERR_WORKSPACE;
@@ -1073,7 +1075,7 @@ int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int6
     a.cache = *cache;
     a.query = query, a.out = out, a.q_n = query_token, a.q_h = query_head, a.o_n = out_token, a.o_h = out_head, a.starts = seq_starts;
     a.Hq = Hq, a.G = G, a.causal = causal, a.window = window;
-    a.scale = (scale < 0 ? -scale : scale) * kLog2e, a.negate = scale < 0 ? 0x80008000u : 0u;
+    a.scale = fmaxf(fabsf(scale) * kLog2e, 1.4e-45f), a.negate = scale < 0 ? 0x80008000u : 0u;
     a.box_rows = one_page || cache->page_size > kTile ? kTile : cache->page_size;
     const size_t rows = 2 * (size_t)ctas * (solo ? kTile : 2 * kTile);
     a.part_o = (float *)workspace, a.part_ml = a.part_o + rows * D, a.cuts = (Cut *)(a.part_ml + rows * 2);

@@ -556,7 +556,9 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n_args) 
     if (args[7] != Py_None) {
         if (!PyFloat_Check(args[7])) Py_RETURN_FALSE;
         scale = PyFloat_AS_DOUBLE(args[7]);
+        if (!std::isfinite((float)scale)) Py_RETURN_FALSE;
     }
+    if (given.given() && given.at() == query.at()) Py_RETURN_FALSE;
     if (!on_sixteen_bytes(keys) || !on_sixteen_bytes(values) || !on_sixteen_bytes(query) || (given.given() && !on_sixteen_bytes(given))) Py_RETURN_FALSE;
     const c10::cuda::CUDAGuard on(keys->device());
     const Tensor out = given.given() ? *given.t : at::empty({N, Hq, c.D}, query->options());

@@ -3,7 +3,7 @@
 A paged cache is two tensors of pages ``[P, Hkv, page_size, D]`` (any strides, unit stride along D) and a ``block_table``
 int32 ``[B, W]`` of page numbers: position ``p`` of sequence ``b`` is slot ``p % page_size`` of page ``block_table[b, p // page_size]``.
 A page of 128 tokens is what ``compress_tiled_tensor`` packs, and a dense cache ``[B, H, T, D]`` is one page per sequence with the table
-``arange(B)[:, None]``: that is how the caches of this package use these functions (``Float11Cache.append_rotary``,
+``arange(B)[:, None]``: that is how the caches of this package use these functions (``Float11Cache.update_rotary``,
 ``Float11Cache.chunk_attention``).
 
 ``seq_lens`` int32 ``[B]`` counts the tokens of every sequence with the new ones of the call.  New tokens lie one sequence
@@ -31,6 +31,8 @@ _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
 _ANGLES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.FP32}
 _MAX_AXES = 4
 _INT32 = torch.int32
+_MOST = 2 ** 31 - 1
+_MOST_SCALE = torch.finfo(torch.float32).max
 
 
 def _describe_cache(N: int, key_pages: torch.Tensor, value_pages: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -53,6 +55,8 @@ def _describe_cache(N: int, key_pages: torch.Tensor, value_pages: torch.Tensor, 
         raise ValueError('seq_lens must be contiguous int32 [B]')
     if B == 0 or W == 0 or key_pages.numel() == 0:
         raise ValueError('the cache has no pages or no sequences')
+    if max(N, B, W, H, page) > _MOST or P >= _MOST:
+        raise ValueError('sizes must fit in 31 bits')
     if cu_seqlens is None:
         if N % B != 0:
             raise ValueError(f'without cu_seqlens the {N} new tokens must divide evenly among {B} sequences')
@@ -174,7 +178,7 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     with one page per sequence (``block_table`` ``[B, 1]``) any number.
 
     Scores and sums are of 32 bits; the softmax weights are rounded to the pages' type for their product with the values.
-    Returns ``[N, Hq, D]``, ``out`` if given.
+    Returns ``[N, Hq, D]``, ``out`` if given, which must not overlap the queries.
     """
     if key_pages.is_cuda:
         got = _lib.native().paged_attention(query, key_pages, value_pages, block_table, seq_lens, cu_seqlens, max_query_len, scale, bool(causal),
@@ -196,12 +200,18 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
         raise ValueError(f'pages of several per sequence must hold 16, 32, 64 or a multiple of 128 tokens, got {page}')
     if window < 0:
         raise ValueError('window must be positive, or 0 for none')
+    if scale is None:
+        scale = D ** -0.5
+    if not abs(scale) <= _MOST_SCALE:
+        raise ValueError(f'scale must be finite in 32 bits, got {scale}')
     if seq_starts is not None and (seq_starts.dtype is not _INT32 or seq_starts.shape != seq_lens.shape or not seq_starts.is_contiguous()):
         raise ValueError('seq_starts must be contiguous int32 [B]')
     if out is None:
         out = torch.empty((N, Hq, D), dtype=query.dtype, device=query.device)
     elif tuple(out.shape) != (N, Hq, D) or out.dtype != query.dtype or out.stride(2) != 1:
         raise ValueError(f'out must be {query.dtype} {[N, Hq, D]} with unit stride along D')
+    elif N > 0 and out.data_ptr() == query.data_ptr():
+        raise ValueError('out must not be the queries, which are read again where a numerator is not finite')
     if max_query_len is None:
         max_query_len = N // cache.B if cu_seqlens is None else N
     elif max_query_len < 0:
@@ -213,14 +223,13 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
                  seq_starts=seq_starts, out=out)
     if any((t.data_ptr() & 15) or any(s & 7 for s, n in zip(t.stride()[:-1], t.shape) if n > 1) for t in (query, key_pages, value_pages, out)):
         raise ValueError('queries, pages and out must lie on 16-byte boundaries, with strides that are multiples of 8')
-    if scale is None:
-        scale = D ** -0.5
     with on_device(dev):
         # (memory of every call's own: calls of other streams, and graphs that were captured, share nothing)
-        ws = torch.empty(int(_lib.lib().adacode_paged_attn_workspace_bytes(max_query_len, Hq, cache.Hkv, D)), dtype=torch.uint8, device=dev)
+        most = min(int(max_query_len), _MOST)
+        ws = torch.empty(int(_lib.lib().adacode_paged_attn_workspace_bytes(most, Hq, cache.Hkv, D)), dtype=torch.uint8, device=dev)
         rc = _lib.lib().adacode_paged_attn(
             ctypes.byref(cache), query.data_ptr(), *query.stride()[:2], Hq, out.data_ptr(), *out.stride()[:2],
-            None if seq_starts is None else seq_starts.data_ptr(), int(max_query_len), float(scale), int(bool(causal)), int(window),
+            None if seq_starts is None else seq_starts.data_ptr(), most, float(scale), int(bool(causal)), min(int(window), _MOST),
             ws.data_ptr(), ws.numel(), sc.status.data_ptr(), stream_ptr(dev))
     _lib.check(rc, 'adacode_paged_attn')
     written(out)

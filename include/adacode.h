@@ -442,10 +442,11 @@ int adacode_append_rotary(const adacode_paged_cache *cache, const adacode_rotary
  * holds has no influence, infinities and NaN included; a NaN score that is seen makes its row NaN; an infinite or NaN value that is seen
  * gives its column what it has in 32-bit arithmetic.  Products of 16-bit values are summed up in 32 bits, the weights enter the
  * second product in the type of the pages, their sum in 32 bits.
- * max_query_len: the most new tokens of one sequence (an upper bound; it chooses the kernel).  D 64 or 128; pages of 16, 32, 64 or a
+ * `out` must not overlap the queries; scale finite.  max_query_len: the most new tokens of one sequence (an upper bound; it chooses the kernel).  D 64 or 128; pages of 16, 32, 64 or a
  * multiple of 128 tokens, or one page per sequence (table_width 1) of any size; pointers on 16-byte boundaries, strides
  * multiples of 8.  The workspace (on a 16-byte boundary) has adacode_paged_attn_workspace_bytes() for the current device; calls that
- * share one must be ordered on one stream.  seq_starts may be NULL.
+ * share one must be ordered on one stream.  seq_starts may be NULL.  A call has at most 2**32 - 1 tiles: the blocks of 256 rows (a query head of
+ * a new token each) of all cached heads times the 128 positions that they see.
  */
 size_t adacode_paged_attn_workspace_bytes(int max_query_len, int Hq, int Hkv, int D);
 int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int64_t query_token, int64_t query_head, int Hq,

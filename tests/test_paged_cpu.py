@@ -107,3 +107,11 @@ def test_entry_points_refuse_without_a_gpu():
     assert L.adacode_sample_tokens(at, 4, 7, 1, 4, at, at, 1.0, None, 0, None, 1.0, None, 0.0, at, None) == _lib.ERR_INVALID_ARG
     assert L.adacode_sample_tokens(at, 4, 0, 1, 0, at, at, 1.0, None, 0, None, 1.0, None, 0.0, at, None) == _lib.ERR_INVALID_ARG
     assert L.adacode_sample_tokens(at, 4, 0, 0, 4, at, at, 1.0, None, 0, None, 1.0, None, 0.0, at, None) == _lib.OK
+
+
+def test_attention_refuses_scales_and_outputs():
+    k, v, table, lens = cache()
+    q = torch.zeros(4, 4, 64, dtype=BF)
+    for more in ({'scale': float('nan')}, {'scale': float('inf')}, {'scale': -1e39}, {'out': q}):
+        with pytest.raises(ValueError, match='scale|out'):
+            paged_attention(q, k, v, table, lens, **more)

@@ -472,3 +472,29 @@ def test_versions_are_counted():
     before = k._version, v._version
     append_rotary(x, x, c, c, k, v, table, seq)
     assert k._version > before[0] and v._version > before[1]
+
+
+@pytest.mark.parametrize('T', [1, 140])
+def test_scale_zero(T):
+    """All that is seen has the same weight, and what is hidden still has none."""
+    run_case([T, T], [T + 70, T + 301], 8, 2, 128, 64, 'bf16', scale=0.0, starts=[3, 0])
+    run_case([T], [T + 301], 8, 2, 64, 64, 'fp16', scale=0.0, window=40)
+    run_case([T], [T + 301], 8, 2, 64, 64, 'bf16', scale=-0.3)
+
+
+@pytest.mark.parametrize('T', [1, 140])
+def test_windows_and_lengths_beyond_32_bits(T):
+    from adacode_b200 import codec, paged_attention
+    lens = [T + 200]
+    k, v, table, seq = oracle.make_cache(lens, 2, 64, 64, torch.bfloat16)
+    q = torch.randn((T, 4, 64), device='cuda').bfloat16()
+    want = paged_attention(q, k, v, table, seq, max_query_len=T)
+    for window in (2 ** 31 - 1, 2 ** 32 + 5):
+        assert torch.equal(paged_attention(q, k, v, table, seq, max_query_len=T, window=window), want)
+    close(paged_attention(q, k, v, table, seq, max_query_len=2 ** 32 + T), *oracle.attention(q, k, v, table, lens, [T]), torch.bfloat16, lens[0])
+    # fewer cached than new tokens, and everything left padding: nothing is seen
+    few, starts = torch.zeros_like(seq), torch.full_like(seq, 2 ** 31 - 1)
+    for window in (0, 3, 2 ** 31 - 1):
+        assert (paged_attention(q, k, v, table, few, seq_starts=starts, window=window, causal=False) == 0).all()
+        assert (paged_attention(q, k, v, table, seq, seq_starts=starts, window=window) == 0).all()
+    codec.check_device_status(q.device)
