@@ -160,17 +160,30 @@ def _dense_pages(B: int, total: int, device: torch.device) -> tuple:
 
 class _Rotary:
     """The rotation of one call's new tokens on their way into a cache (``paged.append_rotary``): the queries, the angles, and where the rotated
-    queries go."""
+    queries go.  What append_rotary would refuse is refused here, before the cache counts the tokens."""
 
-    def __init__(self, query: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, sections, interleaved: bool):
-        if query.dim() != 4:
-            raise ValueError('query must be [B, Hq, T, D]')
+    def __init__(self, query: torch.Tensor, key_states: torch.Tensor, value_states: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                 sections, interleaved: bool):
+        if query.dim() != 4 or key_states.dim() != 4 or key_states.shape != value_states.shape:
+            raise ValueError('query must be [B, Hq, T, D], keys and values [B, Hkv, T, D]')
         B, Hq, T, D = query.shape
+        if key_states.shape[0] != B or key_states.shape[2:] != (T, D):
+            raise ValueError(f'queries {list(query.shape)} and keys {list(key_states.shape)} are not of the same tokens')
+        if D % 2 != 0 or D > 512:
+            raise ValueError(f'the head size must be even and at most 512, got {D}')
+        if any(x.device != key_states.device for x in (query, value_states, cos, sin)):
+            raise ValueError('queries, keys, values and angles must be on one device')
+        if torch.is_grad_enabled() and any(x.requires_grad for x in (query, key_states, value_states, cos, sin)):
+            raise RuntimeError('update_rotary has no backward pass: call it under torch.no_grad()')
         if cos.shape != sin.shape or cos.dim() not in (3, 4) or cos.shape[-2] != T or cos.shape[-3] not in (1, B):
             raise ValueError(f'cos and sin must be [B or 1, T, R] or [axes, B or 1, T, R] for B = {B}, T = {T}: got {list(cos.shape)} and {list(sin.shape)}')
         R = cos.shape[-1]
         if R % 2 != 0 or R > D:
             raise ValueError(f'cos and sin must have an even number of columns, at most {D}: got {R}')
+        axes = cos.shape[0] if cos.dim() == 4 else 1
+        sections = [R // 2] if sections is None and axes == 1 else [] if sections is None else [int(n) for n in sections]
+        if len(sections) != axes or axes > 4 or min(sections) < 0 or sum(sections) != R // 2:
+            raise ValueError(f'sections must say how many of the {R // 2} frequencies each of the {axes} axes (at most 4) has: got {sections}')
         # (a model's position embeddings hold every angle twice: in halves, or next to each other)
         angles = slice(0, R, 2) if interleaved else slice(0, R // 2)
         self.cos, self.sin = (x[..., angles].expand(*x.shape[:-3], B, T, R // 2).reshape(*x.shape[:-3], B * T, R // 2) for x in (cos, sin))
@@ -178,14 +191,12 @@ class _Rotary:
             self.cos, self.sin = self.cos.float(), self.sin.float()
         self.query = query.to(torch.bfloat16).transpose(1, 2).reshape(B * T, Hq, D)
         self.shape = (B, T, Hq, D)
-        self.sections, self.interleaved, self.out = sections, interleaved, None
+        self.sections, self.interleaved, self.out = sections, interleaved, self.query
 
     def append(self, key_states, value_states, key_buf, value_buf, total: int) -> None:
         """Rotated keys, and values, to the tokens of the ``[B, H, capacity, D]`` buffers that end at ``total``."""
         B, H, T, D = key_states.shape
-        if (B, T) != self.shape[:2]:
-            raise ValueError(f'queries of {self.shape[:2]} sequences and tokens, keys of {(B, T)}')
-        key, value = (x.transpose(1, 2).reshape(B * T, x.shape[1], x.shape[3]) for x in (key_states, value_states))
+        key, value = (x.transpose(1, 2).reshape(B * T, H, D) for x in (key_states, value_states))
         self.out = paged.append_rotary(key, value, self.cos, self.sin, key_buf, value_buf, *_dense_pages(B, total, key_buf.device),
                                        query=self.query, sections=self.sections, interleaved=self.interleaved)
 
@@ -1189,10 +1200,11 @@ class Float11Cache(Cache):
                       layer_idx: int, cache_kwargs: Optional[dict] = None, sections=None, interleaved: bool = False) -> tuple:
         """``update`` for queries and keys that have not been rotated yet: both are, and keys and values written to the cache, in one
         launch (``append_rotary``).  ``cos`` and ``sin`` are a HF model's position embeddings ``[B or 1, T, R]``, with ``sections`` ``[axes, B or 1,
-        T, R]``.  Returns the rotated queries and what ``update`` returns."""
+        T, R]``.  Returns the rotated queries and what ``update`` returns (where ``update`` returns the keys as they came, because a fused
+        attention is to read the cache, they have not been rotated)."""
         if type(self.layers[layer_idx]).update is not float11Layer.update:
             raise NotImplementedError('update_rotary needs keys and values with heads; this layer caches something else')
-        rotary = _Rotary(query, cos, sin, sections, interleaved)
+        rotary = _Rotary(query, key_states, value_states, cos, sin, sections, interleaved)
         keys, values = self.update(key_states, value_states, layer_idx, dict(cache_kwargs or {}, float11_rotary=rotary))
         return rotary.queries(), keys, values
 

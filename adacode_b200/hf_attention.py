@@ -46,7 +46,8 @@ def float11_fused_attention(module, query, key, value, attention_mask, dropout: 
         layer = cache.layers[module.layer_idx]
         if chunks:
             window = getattr(module, 'sliding_window', None) or 0
-            starts = None if attention_mask is None else _left_padding(cache, attention_mask, layer.get_seq_length(), window)
+            starts = None if attention_mask is None else _left_padding(cache, module.layer_idx, attention_mask, query.shape[0], layer.get_seq_length(),
+                                                                       window)
             if query.shape[2] > 1 or starts is not None or window:
                 return layer.chunk_attention(query, scale=scaling, seq_starts=starts, window=window).transpose(1, 2).contiguous(), None
             return layer.decode_attention(query, scale=scaling).transpose(1, 2).contiguous(), None
@@ -78,15 +79,18 @@ def _behind_prefill(cache, module, query: torch.Tensor) -> bool:
     return cache.layers[module.layer_idx].get_seq_length() > query.shape[2]
 
 
-def _left_padding(cache, mask: torch.Tensor, total: int, window: int) -> Optional[torch.Tensor]:
+def _left_padding(cache, layer_idx: int, mask: torch.Tensor, batch: int, total: int, window: int) -> Optional[torch.Tensor]:
     """First visible position of every sequence (int32 [B]) of a mask that is causal, with the layer's sliding window, behind left padding;
     None where nothing is padded.  All layers of a kind get the same mask object in a forward pass, so the (synchronising) check runs
-    once per pass and kind."""
-    known = [k for k in getattr(cache, '_fused_masks_known', ()) if k[0] is mask and k[1] == window]
-    if known:
-        return known[0][2]
+    once per pass and kind; a layer that is not behind the last one asked for begins another pass."""
+    seen_layer, known = getattr(cache, '_fused_masks_known', (-1, ()))
+    known = [k for k in known if layer_idx > seen_layer]
+    cache._fused_masks_known = layer_idx, known
+    for k in known:
+        if k[0] is mask and k[1:3] == (window, total):
+            return k[3]
     visible = mask if mask.dtype == torch.bool else mask == 0
-    B, T = visible.shape[0], visible.shape[2]
+    T = visible.shape[2]
     if visible.shape[3] != total:
         raise NotImplementedError(f'float11_fused attention: a mask of {visible.shape[3]} positions for {total} cached tokens')
     j = torch.arange(total, device=mask.device)
@@ -98,8 +102,8 @@ def _left_padding(cache, mask: torch.Tensor, total: int, window: int) -> Optiona
         causal &= j > at - window
     if not bool((visible == causal[:, None]).all()):
         raise NotImplementedError('float11_fused attention takes masks that are causal behind left padding; use the materialising path')
-    out = starts.to(torch.int32) if bool((starts > 0).any()) else None
-    cache._fused_masks_known = [*getattr(cache, '_fused_masks_known', ())[-3:], (mask, window, out)]
+    out = starts.to(torch.int32).expand(batch).contiguous() if bool((starts > 0).any()) else None
+    known.append((mask, window, total, out))
     return out
 
 
@@ -133,5 +137,5 @@ def fused_decode(cache, model=None, chunks: bool = False):
     finally:
         cache._fused_decode = cache._fused_chunks = False
         cache._fused_mask_seen = None
-        cache._fused_masks_known = []
+        cache._fused_masks_known = -1, []
         _active_cache = previous

@@ -226,3 +226,52 @@ def test_runner_samples_and_attends_in_chunks(tmp_path, monkeypatch):
     assert record['fused_sample'] == {'temperature': 0.7, 'top_k': 20, 'top_p': 1.0, 'min_p': 0.0} and record['total_new_tokens'] == 8.0
     with pytest.raises(ValueError):
         runner.run(runner.get_parse().parse_args([a for a in args if a != '--do_sample']))
+
+
+def test_refused_rotary_updates_leave_the_cache_alone():
+    B, Hq, Hkv, D, T = 1, 2, 2, 64, 3
+    k, v = (synth.kv_tensor((B, Hkv, 40, D), seed=s).to('cuda') for s in (7, 8))
+    q = torch.randn((B, Hq, T, D), device='cuda').to(BF)
+    cos, sin = torch.ones((1, T, D), device='cuda'), torch.zeros((1, T, D), device='cuda')
+    cache = cache_of()
+    cache.update(k, v, 0)
+    good = (q, k[:, :, :T], v[:, :, :T], cos, sin, 0)
+    for i, x in ((0, q[:, :, :2]), (0, q[0]), (0, q.cpu()), (1, k[:, :, :2]), (2, v[:, :1, :T]), (3, cos[..., :63]), (4, sin[:, :2]), (3, cos.cpu())):
+        with pytest.raises(ValueError):
+            cache.update_rotary(*good[:i], x, *good[i + 1:])
+    for sections in ((16, 15), (33, -1), ()):
+        with pytest.raises(ValueError):
+            cache.update_rotary(*good, sections=sections)
+    with pytest.raises(ValueError):
+        cache.update_rotary(q, *good[1:3], *(torch.cat([x, x])[:, None] for x in (cos, sin)), 0)              # two axes without sections
+    with pytest.raises(RuntimeError):
+        cache.update_rotary(q.clone().requires_grad_(), *good[1:])
+    assert cache.get_seq_length() == 40
+    # no tokens at all, and then some
+    rotated, keys, _ = cache.update_rotary(q[:, :, :0], k[:, :, :0], v[:, :, :0], cos[:, :0], sin[:, :0], 0)
+    assert rotated.shape == (B, Hq, 0, D) and torch.equal(keys, k)
+    rotated, keys, values = cache.update_rotary(*good)
+    assert torch.equal(rotated, q) and torch.equal(keys, torch.cat([k, k[:, :, :T]], 2)) and torch.equal(values, torch.cat([v, v[:, :, :T]], 2))
+
+
+def test_masks_are_read_again_in_every_pass():
+    """A mask tensor that is written anew between passes, and one row for all sequences."""
+    from types import SimpleNamespace
+    from adacode_b200 import hf_attention
+    B, Hq, Hkv, D, T = 2, 4, 2, 64, 5
+    k, v = (synth.kv_tensor((B, Hkv, 90, D), seed=s).to('cuda') for s in (9, 10))
+    q = torch.randn((B, Hq, T, D), device='cuda').to(BF)
+    layers = [SimpleNamespace(layer_idx=i, sliding_window=None) for i in (0, 1)]
+    causal = torch.arange(90, device='cuda') <= torch.arange(85, 90, device='cuda')[:, None]
+    mask = causal.expand(1, 1, T, 90).clone()
+    cache = cache_of(2)
+    for i in (0, 1):
+        cache.update(k, v, i)
+    table = torch.arange(B, dtype=I32)[:, None]
+    with torch.no_grad(), hf_attention.fused_decode(cache, chunks=True):
+        for start in (0, 30, 7):
+            mask.copy_(causal & (torch.arange(90, device='cuda') >= start))
+            want, size = oracle.attention(q.transpose(1, 2).reshape(B * T, Hq, D), k, v, table, [90] * B, [T] * B, starts=[start] * B)
+            for layer in layers:
+                got, _ = hf_attention.float11_fused_attention(layer, q, k[:, :, -T:], v[:, :, -T:], mask)
+                near(got.reshape(B * T, Hq, D), want, size)
