@@ -6,11 +6,14 @@
 //   1  the largest logit, and of every thread the largest of its tokens, in two halves.
 //   top_k up to kMostK: the k-th largest of those many maxima has at least k tokens above it, and hardly more.  Threads whose maxima reach it list
 //      their tokens that do; the list is sorted, and all else happens in it.  No weight of any other token is computed.
-//   top_p alone: 2 counts tokens per interval of the logit (2048 intervals), which with the interval's middle says where the nucleus about ends;
-//      3 computes every weight once, in 64 bits, and adds up, per span, what lies above that interval, what lies below it, and lists what
-//      lies in it.  These sums say exactly whether the interval was right (if not, a neighbour is next); the sorted list says where the nucleus ends.
+//   top_p alone: 2 adds up weights, roughly, per interval of the logit (2048 intervals), which says where the nucleus about ends;
+//      3 computes every weight once, in 64 bits, and adds up, per span, what lies above that interval, what does not, and lists what
+//      lies in it.  These sums say exactly whether the interval was right (if not, the guess is made again from there); the sorted list says
+//      where the nucleus ends.
 //   neither: 3 alone.
 //   Then the span in which the draw falls is walked again.
+// Measured: 192 rows of 151936 with top_p and min_p 150 us (the weights take half of it: 29 million of eight operations of 64 bits; issue slots
+// half busy), 64 rows of 128256 with top_k and top_p 22 us (33 MB, twice), one row of 32000 11 us (latency: four passes that wait for one another).
 // What fits no list (thousands of equal logits at a border, a larger top_k) goes the slow way: bisection of the keys by one CTA.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -63,6 +66,12 @@ __device__ __forceinline__ float least_of(float a, float b, float c) {
     return r;
 }
 
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // NaN and minus infinity have key 0 (never drawn), both zeros one key.
 __device__ __forceinline__ uint32_t key_of(float v) {
     if (!(v > -INFINITY)) return 0;
@@ -83,7 +92,7 @@ struct Shared {
     double scan[kWarps + 1];
     unsigned long long slow[kWarps];
     double cta_below;
-    float low[kWarps], cta_low, cta_top;
+    float low[kWarps], cta_low, cta_top, edge[2];
     int scan_n[kWarps];
     int listed, found, decided;
     uint64_t border;
@@ -100,7 +109,7 @@ struct Weights {
         : k(fmin(1.4426950408889634074 / (double)t, 1099511627776.0 / fabs((double)top))), shift(-(double)top * k), floor(fmaxf(top - 600.f * t, -FLT_MAX)), roots(roots) {}
     // The exponent rounded to 1/128; the power of the rest r by the Taylor series of 2**r (degree 3, |r| <= 1/256: the next term is below 2.3e-12);
     // 128 roots of 2.  Eight operations of 64 bits, less than half the time of exp(), whose last bits no draw needs.
-    __device__ __forceinline__ double operator()(float v) const {
+    __device__ __forceinline__ double of(float v) const {           // (where there is any)
         const double t = fma((double)capped(v), k, shift);
         constexpr double kShift = 6755399441055744.0 / 128.0;      // 1.5 x 2**52 / 128
         const double shifted = t + kShift;
@@ -108,9 +117,10 @@ struct Weights {
         const double r = t - (shifted - kShift);
         constexpr double kLn2 = 0.69314718055994530942;
         const double power = fma(fma(fma(r, kLn2 * kLn2 * kLn2 / 6.0, kLn2 * kLn2 / 2.0), r, kLn2), r, 1.0) * roots[n & 127];
-        const bool any = v >= floor;                               // (not NaN)
-        return __hiloint2double(any ? __double2hiint(power) + ((n >> 7) << 20) : 0, any ? __double2loint(power) : 0);
+        return __hiloint2double(__double2hiint(power) + ((n >> 7) << 20), __double2loint(power));
     }
+    __device__ __forceinline__ bool any(float v) const { return v >= floor; }          // (not NaN)
+    __device__ __forceinline__ double operator()(float v) const { return any(v) ? of(v) : 0.0; }
 };
 
 template <typename R, typename Op>
@@ -327,7 +337,7 @@ __device__ void sample_slowly(const SampleArgs &a, Shared &s, const T *x, int ro
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ SampleArgs a) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared &s = *reinterpret_cast<Shared *>(raw);
     const cg::cluster_group cluster = cg::this_cluster();
@@ -400,9 +410,8 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
     // (rounded by an addition: the conversion unit is slow; of NaN the last)
     const auto bin_of = [&](float v) { return (int)(__float_as_uint(fminf((top - capped(v)) * per_bin, kBins - 1) + 8388608.f) & (kBins - 1)); };
     constexpr int kEach = kBins / kThreads;
-    // counts of all CTAs, of this thread's intervals
-    const auto gather = [&](uint32_t (&c)[kEach]) {
-        cluster.sync();
+    // counts of all CTAs (complete behind a cluster.sync()), of this thread's intervals
+    const auto gather = [&](auto (&c)[kEach]) {
 #pragma unroll
         for (int j = 0; j < kEach; ++j) c[j] = 0;
         for (int r = 0; r < ctas; ++r) {
@@ -430,6 +439,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
             for (int j = 0; j < 2; ++j)
                 if (half_most[j] > -INFINITY) atomicAdd(&s.count[bin_of(half_most[j])], 1u);
             uint32_t c[kEach];
+            cluster.sync();
             gather(c);
             int total, sum = 0;
 #pragma unroll
@@ -515,67 +525,94 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
     }
 
     // ---- 2: the interval in which the nucleus about ends
-    int edge = kBins;                                            // everything lies above it
-    if (use_p) {
-        each_eight<4>(x, i0, i1, a.wide, [&](const float (&v)[8], int) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (v[j] > -INFINITY) atomicAdd(&s.count[bin_of(v[j])], 1u);
-        });
-        uint32_t c[kEach];
+    int edge = kBins, lowest_edge = 0, highest_edge = kBins - 1; // everything lies above it
+    // A token counts with its weight in units of 2**-15 of that of its interval's middle: with 1 for each, a few large weights half an
+    // interval from the middle, or the steps of a 16-bit type, let the guess miss by some intervals, a pass over the row each.  (Sums that
+    // pass 32 bits, of a hundred thousand tokens in an interval, and all else that is rounded here cost a better guess, nothing more.)
+    const float fall = per_bin > 0.f ? -1.442695f / (per_bin * t) : 0.f;
+    // the interval in which the weights of all intervals, from the first on, add up to what aim_of(all) says; the sum before interval `at`
+    const auto interval_of = [&](auto &&aim_of) {
+        float c[kEach], w[kEach], sum = 0.f, total;
         gather(c);
-        // (every CTA finds the same from the same numbers in the same order)
-        const float step = per_bin > 0.f ? -1.442695f / (per_bin * t) : 0.f;
-        float w[kEach], sum = 0.f, total;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) w[j] = c[j] * exp2f((tid * kEach + j) * step), sum += w[j];
+        for (int j = 0; j < kEach; ++j) w[j] = c[j] * exp2f((tid * kEach + j) * fall - 15.f), sum += w[j];
         if (tid == 0) s.decided = kBins - 1;
         float before = block_scan(sum, total, s.low);
-        const float aim = p * total;
+        if (tid == edge / kEach) {
+            float from = before;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                if (j == edge % kEach) s.edge[0] = from, s.edge[1] = from + w[j];
+                from += w[j];
+            }
+        }
+        __syncthreads();
+        const float aim = aim_of(total);
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
             if (before + w[j] >= aim) atomicMin(&s.decided, tid * kEach + j);
             before += w[j];
         }
         __syncthreads();
-        edge = s.decided;
+        return s.decided;
+    };
+    if (use_p) {
+        each_eight<4>(x, i0, i1, a.wide, [&](const float (&v)[8], int) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (v[j] > -INFINITY) {
+                    const float at = fminf((top - capped(v[j])) * per_bin, kBins - 1), middle = at + 8388608.f;
+                    const float units = fmaf(exp2_fast((at - (middle - 8388608.f)) * fall), 32768.f, 8388608.f);
+                    atomicAdd(&s.count[__float_as_uint(middle) & (kBins - 1)], __float_as_uint(units) & 0x7FFFFFu);
+                }
+        });
+        cluster.sync();
+        // (every CTA finds the same from the same numbers in the same order)
+        edge = interval_of([&](float total) { return p * total; });
     }
 
-    // the smallest logit whose weight stays, by a search of the keys 32 at a time (weights of neighbours differ by far more than the rounding)
-    float kept_from = -FLT_MAX;
-    if (least > 0.0) {
-        uint32_t lo = key_of(-FLT_MAX), hi = top_key;           // (the first that stays is one of lo .. hi)
+    // the smallest logit for which `is` holds, which then holds for all larger ones, by a search of the keys 32 at a time; NaN if for none
+    const auto smallest = [&](auto &&is) {
+        uint32_t lo = key_of(-FLT_MAX), hi = top_key + 1;       // (one of lo .. hi)
         while (lo < hi) {
             const uint32_t stride = (hi - lo) / 32 + 1, mid = lo + lane * stride;
-            const unsigned stays = __ballot_sync(kFull, mid >= hi || weight_of(value_of(mid)) >= least);
-            if (stays == kFull) hi = lo;
-            else if (stays == 0) lo += 31 * stride + 1;
+            const unsigned holds = __ballot_sync(kFull, mid >= hi || is(value_of(mid)));
+            if (holds == kFull) hi = lo;
+            else if (holds == 0) lo += 31 * stride + 1;
             else {
-                const uint32_t at = lo + (__ffs(stays) - 1) * stride;
+                const uint32_t at = lo + (__ffs(holds) - 1) * stride;
                 lo = at - stride + 1, hi = at < hi ? at : hi;
             }
         }
-        kept_from = value_of(lo);
-    }
+        return lo > top_key ? NAN : value_of(lo);
+    };
+    // (weights of neighbours differ by far more than the rounding)
+    const float kept_from = least > 0.0 ? smallest([&](float v) { return weight_of(v) >= least; }) : -FLT_MAX;
 
     // ---- 3: what lies above the interval, per span, below it, and what lies in it
     uint64_t border = 0;                                         // the last place that stays
     for (int tries = 0;; ++tries) {
+        // (intervals as logits: one comparison each instead of the interval's number)
+        const float above_from = edge < kBins ? smallest([&](float v) { return bin_of(v) < edge; }) : -FLT_MAX;
+        const float in_from = edge < kBins ? smallest([&](float v) { return bin_of(v) <= edge; }) : NAN;
+        const float stays_from = kept_from > above_from ? kept_from : above_from;
         double above = 0.0, kept = 0.0, below = 0.0;
-        each_eight<2>(x, i0, i1, a.wide, [&](const float (&v)[8], int i) {
+        // (one step at a time: two under way cost more registers than there are, 64 for two CTAs on an SM)
+        each_eight<1>(x, i0, i1, a.wide, [&](const float (&v)[8], int i) {
             unsigned in = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const double w = weight_of(v[j]);
-                const int bin = use_p ? bin_of(v[j]) : 0;
-                if (bin < edge) above += w;
-                if (least > 0.0 && bin < edge && v[j] >= kept_from) kept += w;
-                if (bin > edge) below += w;
-                in |= (v[j] > -INFINITY && bin == edge ? 1u : 0u) << j;
+                const double w = weight_of.of(v[j]);
+                if (weight_of.any(v[j])) {
+                    if (v[j] >= above_from) above += w;
+                    else below += w;
+                    if (v[j] >= stays_from) kept += w;
+                }
+                in |= (v[j] >= in_from && !(v[j] >= above_from) ? 1u : 0u) << j;
             }
             list(in, v, i);
         });
-        above = warp_reduce(above, Plus()), kept = least > 0.0 ? warp_reduce(kept, Plus()) : above;
+        above = warp_reduce(above, Plus()), kept = warp_reduce(kept, Plus());
         if (lane == 0) first.span_all[me] = above, first.span_kept[me] = kept;
         if (use_p) {
             below = block_reduce(below, Plus(), s.scan);
@@ -590,9 +627,9 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
                 next = -2;
             } else {
                 sort_places(s.list, n);
-                double over = 0.0, under = 0.0, total, running = 0.0;
+                double over = 0.0, rest = 0.0, total, running = 0.0;     // (rest: in the interval and below it)
                 over = block_reduce(tid < spans ? s.span_all[tid] : 0.0, Plus(), s.scan);
-                for (int r = 0; r < ctas; ++r) under += cluster.map_shared_rank(&s, r)->cta_below;
+                for (int r = 0; r < ctas; ++r) rest += cluster.map_shared_rank(&s, r)->cta_below;
                 // eight consecutive places per thread
                 constexpr int kPlaces = kList / kThreads;
                 double sum = 0.0;
@@ -601,11 +638,16 @@ __global__ void __launch_bounds__(kThreads) k_sample(const __grid_constant__ Sam
                     if (i < n) sum += weight_of(value_of((uint32_t)(s.list[i] >> 32)));
                 }
                 running = over + block_scan(sum, total, s.scan);
-                const double aim = (double)p * (over + total + under);
-                if (over >= aim && edge > 0) next = edge - 1;
-                else if (over + total < aim && edge < kBins - 1) next = edge + 1;
-                if (tries == 4 && next >= 0) next = -2;
-                if (next == -1) {
+                const double aim = (double)p * (over + rest);
+                const bool early = over >= aim && edge > 0, late = !early && over + total < aim && edge < kBins - 1;
+                if (early || late) {
+                    // the guess again, from where the exact sums are known
+                    if (early) highest_edge = edge - 1;
+                    else lowest_edge = edge + 1;
+                    next = interval_of([&](float) { return early ? s.edge[0] - (float)(over - aim) : s.edge[1] + (float)(aim - (over + total)); });
+                    next = max(lowest_edge, min(next, highest_edge));
+                    if (tries == 6 || lowest_edge > highest_edge) next = -2;
+                } else {
                     int inside = 0, total_inside;
                     for (int j = 0; j < kPlaces; ++j) {
                         const int i = tid * kPlaces + j;

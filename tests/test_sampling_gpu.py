@@ -135,3 +135,15 @@ def test_many_rows():
     g = torch.Generator('cpu').manual_seed(11)
     logits = (torch.randn((600, 513), generator=g) * 2).bfloat16().cuda()
     check(logits, torch.rand(600, generator=g).cuda(), top_k=40, top_p=0.9)
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16', 'fp32'])
+@pytest.mark.parametrize('scale', [0.01, 3.0, 9.0])
+def test_nuclei_of_many_rows(scale, dtype):
+    """Nuclei of a few tokens to most of the vocabulary; logits with a step that is coarse against the nucleus' end, and single heavy tokens."""
+    g = torch.Generator('cpu').manual_seed(5)
+    logits = torch.randn((12, 70001), generator=g) * scale
+    logits[::3, 17] = logits[::3].amax(1) + 2.3
+    logits = logits.to(TYPES[dtype]).cuda()
+    for s in (dict(top_p=0.95, temperature=0.8), dict(top_p=0.6), dict(top_p=0.999, min_p=1e-4, temperature=1.5), dict(top_p=1e-6)):
+        check(logits, torch.rand(12, generator=g).cuda(), **s)
