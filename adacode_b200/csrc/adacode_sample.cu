@@ -1,7 +1,7 @@
 // One token per row of logits: temperature, top-k, top-p, min-p and the draw from a given uniform number.
 //
 // Every cut (the top_k first, the nucleus, min_p) keeps a prefix of the order (descending logit, ascending token); tokens are kept
-// as 64-bit keys of that order.  A row has a cluster of 1 to 4 CTAs, whose warps own consecutive spans of the vocabulary.  Passes over the row, which
+// as 64-bit keys of that order.  A row has a cluster of 1 to 8 CTAs, whose warps own consecutive spans of the vocabulary.  Passes over the row, which
 // after the first come from L2:
 //   1  the largest logit, and of every thread the largest of its tokens, in two halves.
 //   top_k up to kMostK: the k-th largest of those many maxima has at least k tokens above it, and hardly more.  Threads whose maxima reach it list
@@ -32,7 +32,7 @@ namespace {
 
 constexpr unsigned kFull = 0xFFFFFFFFu;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kMostCtas = 4;             // per row
+constexpr int kMostCtas = 8;             // per row
 constexpr int kStep = 256;               // tokens that a warp takes at a time, eight per lane
 constexpr int kBins = 2048;
 constexpr int kList = 4096;
@@ -809,10 +809,11 @@ extern "C" int adacode_sample_tokens(const void *logits, int64_t row_stride, int
     const bool wide = ((uintptr_t)logits & 15) == 0 && (row_stride * size) % 16 == 0;
     const SampleArgs a{logits, row_stride, V, wide, uniforms, temperature, top_p, min_p, top_k, tokens, temperature_all, top_p_all, min_p_all, top_k_all};
     // CTAs per row: up to four, as long as all rows' make no more than three for each of 148 SMs (two fit at a time; more rounds than that only add
-    // the rows' ends) and every warp has a step of the vocabulary.  192 rows of 151936: 218 us with one, 159 with two, 193 with four; 64 rows of
-    // 128256: 34, 22, 21.5 and 37 with eight; one row of 32000: 16, 12.6, 11 and 11.2.
+    // the rows' ends) and every warp has a step of the vocabulary; eight if every CTA then has an SM of its own and every warp two steps.  192 rows of
+    // 151936: 218 us with one, 159 with two, 193 with four (then; 150 with two now); 64 rows of 128256: 34, 22, 21.5 and 37 with eight; one row of
+    // 32000: 16, 12.6, 11 and 11.2; one row of 262144 with top_p 54 with four and 39 with eight, 32 rows of 32000 with top_k 11 and 16.5.
     int ctas = 1;
-    while (ctas < kMostCtas && (int64_t)B * ctas * 2 <= 3 * 148 && V > ctas * kWarps * kStep) ctas *= 2;
+    while (ctas < kMostCtas && (int64_t)B * ctas * 2 <= (ctas < 4 ? 3 * 148 : 148) && V > ctas * kWarps * kStep * (ctas < 4 ? 1 : 2)) ctas *= 2;
     cudaStream_t st = (cudaStream_t)stream;
     const cudaError_t e = dtype == ADACODE_BF16 ? launch<__nv_bfloat16>(a, B, ctas, st)
                           : dtype == ADACODE_FP16 ? launch<__half>(a, B, ctas, st)
