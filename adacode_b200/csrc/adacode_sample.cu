@@ -92,7 +92,7 @@ struct Shared {
     double scan[kWarps + 1];
     unsigned long long slow[kWarps];
     double cta_below;
-    float low[kWarps], cta_low, cta_top, edge[2];
+    float low[kWarps], cta_low, cta_top, cut_low, edge[2];
     int scan_n[kWarps];
     int listed, found, decided;
     uint64_t border;
@@ -406,6 +406,20 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     }
     float range = top - low;
     if (!use_k && range > 30.f * t) range = 30.f * t;           // (weights below e**-30 share an interval)
+    // Tokens that a mask has given a type's lowest value would leave all others in one interval.  What weighs nothing (600 T from the top) has
+    // the last interval of a top_k to itself, and is never listed.
+    const bool cut = use_k && range > 610.f * t;
+    if (cut) {
+        low = INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (capped(half_most[j]) >= top - 610.f * t) low = fminf(low, capped(half_most[j]));
+        low = block_reduce(low, Least(), s.low);
+        if (tid == 0) s.cut_low = low;
+        cluster.sync();
+        for (int r = 0; r < ctas; ++r) low = fminf(low, cluster.map_shared_rank(&s, r)->cut_low);
+        range = fmaxf((top - low) * 1.01f, t);
+    }
     const float per_bin = range > 0.f ? fminf(kBins / range, FLT_MAX) : 0.f;
     // (rounded by an addition: the conversion unit is slow; of NaN the last)
     const auto bin_of = [&](float v) { return (int)(__float_as_uint(fminf((top - capped(v)) * per_bin, kBins - 1) + 8388608.f) & (kBins - 1)); };
@@ -452,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
                 before += c[j];
             }
             __syncthreads();
-            lowest = s.decided;
+            lowest = cut ? min(s.decided, kBins - 2) : s.decided;
         }
         bool look = lowest == kBins;
 #pragma unroll
@@ -559,12 +573,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     if (use_p) {
         each_eight<4>(x, i0, i1, a.wide, [&](const float (&v)[8], int) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (v[j] > -INFINITY) {
-                    const float at = fminf((top - capped(v[j])) * per_bin, kBins - 1), middle = at + 8388608.f;
+            for (int j = 0; j < 8; ++j) {
+                // (what lies behind the intervals, masked tokens not least, has no weight to speak of)
+                const float behind = (top - v[j]) * per_bin;
+                if (behind < kBins) {                            // (not NaN)
+                    const float at = fminf(fmaxf(behind, 0.f), kBins - 1), middle = at + 8388608.f;
                     const float units = fmaf(exp2_fast((at - (middle - 8388608.f)) * fall), 32768.f, 8388608.f);
                     atomicAdd(&s.count[__float_as_uint(middle) & (kBins - 1)], __float_as_uint(units) & 0x7FFFFFu);
                 }
+            }
         });
         cluster.sync();
         // (every CTA finds the same from the same numbers in the same order)

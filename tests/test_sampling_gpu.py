@@ -147,3 +147,18 @@ def test_nuclei_of_many_rows(scale, dtype):
     logits = logits.to(TYPES[dtype]).cuda()
     for s in (dict(top_p=0.95, temperature=0.8), dict(top_p=0.6), dict(top_p=0.999, min_p=1e-4, temperature=1.5), dict(top_p=1e-6)):
         check(logits, torch.rand(12, generator=g).cuda(), **s)
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16', 'fp32'])
+def test_masks_of_the_lowest_value(dtype):
+    """Tokens masked by a type's lowest number instead of minus infinity: whole regions, and nearly all of the vocabulary."""
+    g = torch.Generator('cpu').manual_seed(6)
+    logits = (torch.randn((8, 50000), generator=g) * 3).to(TYPES[dtype]).cuda()
+    lowest = torch.finfo(TYPES[dtype]).min
+    logits[:3, 9000:48000] = lowest
+    logits[3:6, torch.randperm(50000, generator=g)[:49970].cuda()] = lowest
+    logits[6, 1:] = lowest
+    logits[7] = lowest
+    for s in (dict(top_k=50), dict(top_k=50, temperature=0.01), dict(top_k=400, top_p=0.9), dict(top_p=0.95), dict(min_p=0.01), dict(),
+              dict(top_k=20, temperature=1e3)):
+        check(logits, torch.rand(8, generator=g).cuda(), **s)
