@@ -8,8 +8,8 @@
 // CTA finds its run by itself.
 //
 // One CTA: warp 9 finds the pieces and loads the keys, warp 10 the values (one tensor copy per page and 64 columns), warp 8 issues the products
-// of both streams (a warp for each made them interleave, and took a third longer), two warpgroups do the softmax, one row per thread.  S = Q K^T goes to TMEM, the weights go back to where S was, and
-// O += P V takes them from there.  Two streams of S, P and O let one's softmax run while the other's products do:
+// of both streams (a warp for each made them interleave, and took a third longer), two warpgroups do the softmax, one row per thread.  S = Q K^T goes
+// to TMEM, the weights go back to where S was, and O += P V takes them from there.  Two streams of S, P and O let one's softmax run while the other's products do:
 //   PAIR  a unit has 256 rows, stream i the rows 128 i ..; every tile is used by both.
 //   SOLO  a unit has 128 rows; stream i takes every second tile, and the two meet at the end of the piece.  For few rows, where
 //         reading the cache is what takes time, with three instead of two tiles of keys and values on the way.
@@ -17,9 +17,9 @@
 // than 2**8, which spares nearly all rescaling of O; weights stay below 2**8 and sums below 2**8 times the length.
 //
 // Measured (device time): a decode step of 64 sequences of up to 8192 tokens, 32 heads on 8 of 128, 220 us, 6.1 TB/s, bound by memory; two chunks of
-// 2048 tokens behind 16384 645 us, 1100 TFLOP/s, and 509 tokens behind 20557 172 us, 984 TFLOP/s, bound by the chain of one stream's tile (softmax
-// 2300 cycles, products 1300; two streams take turns); one token behind 2050 14 us, bound by latency (finding the run 4500 cycles, one tile
-// 8000, the merge).
+// 2048 tokens behind 16384 644 us, 1103 TFLOP/s, and 509 tokens behind 20557 168 us, 1008 TFLOP/s, bound by the chain of one stream's tile (softmax
+// 2300 cycles, products 1300; two streams take turns); one token behind 2050 12.5 us, bound by latency (finding the run some 3500 cycles, one
+// tile 8000, the merge).
 //
 // Hidden positions get the score minus infinity; their values would still be multiplied by the weight 0.  Values behind the sequence's end are
 // cleared in shared memory.  Others (left padding, later tokens of the chunk) only matter if they are infinite or NaN: a row that ends with such
