@@ -406,8 +406,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     }
     float range = top - low;
     if (!use_k && range > 30.f * t) range = 30.f * t;           // (weights below e**-30 share an interval)
-    // Tokens that a mask has given a type's lowest value would leave all others in one interval.  What weighs nothing (600 T from the top) has
-    // the last interval of a top_k to itself, and is never listed.
+    // Tokens that a mask has given a type's lowest value would leave all others in one interval.  So the intervals of a top_k reach down to the
+    // smallest maximum that weighs something (600 T from the top nothing does), and the last has all that lies below.
     const bool cut = use_k && range > 610.f * t;
     if (cut) {
         low = INFINITY;
@@ -448,6 +448,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
 
     if (use_k) {
         int lowest = kBins;                                      // the lowest interval that is listed (all, of a short row)
+        bool weighty = false;                                    // or, instead, all that weighs anything
         if (V > kList) {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
@@ -466,18 +467,20 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
                 before += c[j];
             }
             __syncthreads();
-            lowest = cut ? min(s.decided, kBins - 2) : s.decided;
+            lowest = s.decided;
+            // Fewer than k maxima lie above the last interval, so tokens among the first k may lie in it, in the shadow of a neighbour that is a
+            // maximum.  What weighs something does (what does not is never drawn, and takes no part in any sum).
+            weighty = cut && lowest >= kBins - 1;
         }
-        bool look = lowest == kBins;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) look |= half_most[j] > -INFINITY && bin_of(half_most[j]) <= lowest;
+        const auto listed = [&](float v) { return weighty ? weight_of.any(v) : v > -INFINITY && (lowest == kBins || bin_of(v) <= lowest); };
+        const bool look = lowest == kBins || listed(half_most[0]) || listed(half_most[1]);
         if (look)
             for (int i = i0 + lane * 8; i < i1; i += kStep) {
                 float v[8];
                 load_eight(x, i, i1, a.wide, v);
                 unsigned in = 0;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) in |= (v[j] > -INFINITY && (lowest == kBins || bin_of(v[j]) <= lowest) ? 1u : 0u) << j;
+                for (int j = 0; j < 8; ++j) in |= (listed(v[j]) ? 1u : 0u) << j;
                 list(in, v, i);
             }
         cluster.sync();

@@ -162,3 +162,23 @@ def test_masks_of_the_lowest_value(dtype):
     for s in (dict(top_k=50), dict(top_k=50, temperature=0.01), dict(top_k=400, top_p=0.9), dict(top_p=0.95), dict(min_p=0.01), dict(),
               dict(top_k=20, temperature=1e3)):
         check(logits, torch.rand(8, generator=g).cuda(), **s)
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16', 'fp32'])
+@pytest.mark.parametrize('V', [5000, 32000, 151936])
+def test_few_neighbours_among_the_lowest_value(V, dtype):
+    """Fewer tokens than top_k that are not masked by the type's lowest number, next to each other: inside one group of tokens that a thread takes
+    at a time, across two, at the row's ends; their logits up to 20 apart, rising and falling."""
+    g = torch.Generator('cpu').manual_seed(V)
+    rows = []
+    for n in (2, 3, 5, 10):
+        for first in (0, 2, 1027, V - n):
+            gap = (0.5, 2.0, 20.0)[len(rows) % 3]
+            line = 10 - gap * torch.arange(n)
+            row = torch.full((V,), torch.finfo(TYPES[dtype]).min)
+            row[first:first + n] = line if len(rows) % 2 else line.flip(0)
+            rows.append(row)
+    logits = torch.stack(rows).to(TYPES[dtype]).cuda()
+    for s in (dict(top_k=50), dict(top_k=400, temperature=4.0), dict(top_k=50, top_p=0.95), dict(top_k=50, temperature=0.05)):
+        for u in (torch.rand(len(rows), generator=g), torch.full((len(rows),), 1 - 2.0 ** -24)):
+            check(logits, u.cuda(), **s)
