@@ -11,14 +11,14 @@ __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
 
-// Sequence of new token i (B if it is behind the last), found by the whole warp, and the tokens of the call up to its end.
+// Sequence of new token i (B if it is before the first or behind the last), found by the whole warp, and the tokens of the call up to its end.
 __device__ __forceinline__ int sequence_of(const adacode_paged_cache &c, int i, int &end) {
     if (!c.cu_seqlens) {
         const int each = c.N / c.B, b = i / each;
         end = (b + 1) * each;
         return b;
     }
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, first = c.cu_seqlens[0];
     int b = 0;
     for (int k = 0; k < c.B; k += 32) {
         const int e = k + lane < c.B ? c.cu_seqlens[k + lane + 1] : INT32_MAX;
@@ -29,7 +29,7 @@ __device__ __forceinline__ int sequence_of(const adacode_paged_cache &c, int i, 
             break;
         }
     }
-    return b;
+    return i < first ? c.B : b;
 }
 
 // The page of position `at` of sequence b, or -1.

@@ -8,7 +8,7 @@ A page of 128 tokens is what ``compress_tiled_tensor`` packs, and a dense cache 
 
 ``seq_lens`` int32 ``[B]`` counts the tokens of every sequence with the new ones of the call.  New tokens lie one sequence
 after the other along the first dimension; ``cu_seqlens`` int32 ``[B + 1]`` says where each sequence begins (without it all have equally
-many), and tokens from ``cu_seqlens[B]`` on are padding, which is left alone.  Tables and lengths stay on the device: a call
+many), and tokens before ``cu_seqlens[0]`` or from ``cu_seqlens[B]`` on are padding, which is left alone.  Tables and lengths stay on the device: a call
 never waits for them, and a captured call may be replayed with others.  What only they can show to be wrong, a position without a page
 of the pool, is never followed: nothing is written there, zeros are read, and the device's
 status word says so (``codec.check_device_status``).

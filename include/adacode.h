@@ -408,7 +408,7 @@ typedef struct adacode_paged_cache {
     const int32_t *seq_lens;                 /* [B] */
     const int32_t *cu_seqlens;               /* [B + 1]: new token i is of the sequence b with cu[b] <= i < cu[b + 1]; NULL: N / B each */
     int32_t table_width, B, n_pages, page_size, Hkv, D, dtype; /* ADACODE_BF16 or ADACODE_FP16 */
-    int32_t N;                               /* new tokens that the call's tensors have room for; those from cu[B] on are left alone */
+    int32_t N;                               /* new tokens that the call's tensors have room for; those before cu[0] and from cu[B] on are left alone */
 } adacode_paged_cache;
 
 /* Rotary positions of adacode_append_rotary: the cosine and sine of half angles per token, for 1 to 4 axes.  Frequency f

@@ -498,3 +498,27 @@ def test_windows_and_lengths_beyond_32_bits(T):
         assert (paged_attention(q, k, v, table, few, seq_starts=starts, window=window, causal=False) == 0).all()
         assert (paged_attention(q, k, v, table, seq, seq_starts=starts, window=window) == 0).all()
     codec.check_device_status(q.device)
+
+
+@pytest.mark.parametrize('first', [1, 4, 70])
+def test_tokens_before_the_first_sequence_are_left_alone(first):
+    """cu_seqlens[0] above 0: what is before it is of no sequence, like what is behind the last."""
+    from adacode_b200 import append_rotary, paged_attention
+    new, lens = [3, 40], [90, 75]
+    k, v, table, seq = oracle.make_cache(lens, 2, 64, 16, torch.bfloat16)
+    N = first + sum(new) + 2
+    q = torch.randn((N, 4, 64), device='cuda').bfloat16()
+    cu = oracle.cumulative(new) + first
+    out = torch.full_like(q, 7.0)
+    paged_attention(q, k, v, table, seq, cu_seqlens=cu, out=out)
+    mine = slice(first, first + sum(new))
+    want, size = oracle.attention(q[mine], k, v, table, lens, new)
+    close(out[mine], want, size, torch.bfloat16, max(lens))
+    rotated, c = torch.full_like(q, 7.0), torch.ones((N, 32), device='cuda')
+    want_k, want_v = k.clone(), v.clone()
+    append_rotary(q[mine, :2], q[mine, 2:], c[mine], 0 * c[mine], want_k, want_v, table, seq, cu_seqlens=oracle.cumulative(new))
+    append_rotary(q[:, :2], q[:, 2:], c, 0 * c, k, v, table, seq, query=q, cu_seqlens=cu, out=rotated)
+    assert torch.equal(k, want_k) and torch.equal(v, want_v)
+    assert torch.equal(rotated[mine], q[mine])
+    for x in (out, rotated):
+        assert (x[:first] == 7).all() and (x[mine.stop:] == 7).all()
