@@ -1049,6 +1049,13 @@ cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, int threads, s
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Two launches hand partial results on in the workspace: threads that share a stream and a workspace must not come between them, whichever
+// kernels their calls are for.
+std::mutex &lock_of(const void *workspace) {
+    static std::mutex locks[64];
+    return locks[((uintptr_t)workspace >> 9) * 0x9E3779B97F4A7C15ull >> 58];
+}
+
 template <typename T, int D, bool SOLO>
 int launch_paged(const PagedArgs &a, const CUtensorMap &keys, const CUtensorMap &values, int ctas, int max_query_len, cudaStream_t st) {
     // the kernel's limit of dynamic shared memory is raised once per device
@@ -1061,10 +1068,7 @@ int launch_paged(const PagedArgs &a, const CUtensorMap &keys, const CUtensorMap 
         if (dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
     }
     constexpr int rows = Shape<D, SOLO>::kRows;
-    // Two launches that hand partial results on in the workspace: threads that share a stream and a workspace must not come
-    // between them.
-    static std::mutex locks[64];
-    const std::lock_guard<std::mutex> both(locks[((uintptr_t)a.part_o >> 9) * 0x9E3779B97F4A7C15ull >> 58]);
+    const std::lock_guard<std::mutex> both(lock_of(a.part_o));
     if (launch_dependent(k_paged_attn<T, D, SOLO>, dim3(ctas), kAttnThreads, bytes, st, a, keys, values) != cudaSuccess) return ADACODE_ERR_CUDA;
     // (a warp for four rows, or one where a unit has few by max_query_len: 256 rows of 148 units by a warp each took the chunk of 509 tokens
     // behind 20557 170.5 us instead of 168)

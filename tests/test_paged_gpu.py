@@ -522,3 +522,41 @@ def test_tokens_before_the_first_sequence_are_left_alone(first):
     assert torch.equal(rotated[mine], q[mine])
     for x in (out, rotated):
         assert (x[:first] == 7).all() and (x[mine.stop:] == 7).all()
+
+
+def test_threads_share_a_stream_and_a_workspace():
+    """C callers of different kernels (types, head sizes, steps and chunks) from four threads: no call's launches come between another's two."""
+    import ctypes
+    import threading
+    from adacode_b200 import _lib, codec, paged_attention
+    L = _lib.lib()
+    shapes = [([1, 1], [3000, 900], 128, 'bf16'), ([150, 33], [1500, 700], 128, 'fp16'), ([150, 9], [1700, 400], 64, 'bf16'), ([1, 2], [2000, 1100], 64, 'fp16')]
+    workspace = torch.empty(max(L.adacode_paged_attn_workspace_bytes(256, 16, 4, 128), L.adacode_paged_attn_workspace_bytes(1, 16, 4, 128)), dtype=torch.uint8,
+                            device='cuda')
+    status, stream = codec.device_status(workspace.device), torch.cuda.current_stream().cuda_stream
+    calls = []
+    for n, (new, lens, D, dtype) in enumerate(shapes):
+        k, v, table, seq = oracle.make_cache(lens, 4, D, 64, TYPES[dtype], seed=n)
+        q, cu = torch.randn((sum(new), 16, D), device='cuda').to(TYPES[dtype]), oracle.cumulative(new)
+        want, outs = paged_attention(q, k, v, table, seq, cu_seqlens=cu, max_query_len=max(new)), [torch.zeros_like(q) for _ in range(50)]
+        c = _lib.PagedCache(k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], table.data_ptr(), table.stride(0), seq.data_ptr(), cu.data_ptr(),
+                            table.shape[1], 2, k.shape[0], 64, 4, D, {'bf16': _lib.BF16, 'fp16': _lib.FP16}[dtype], sum(new))
+        calls.append((c, q, max(new), D ** -0.5, want, outs, (k, v, table, seq, cu)))
+    torch.cuda.synchronize()
+    codes, start = [], threading.Barrier(4)
+
+    def work(c, q, longest, scale, want, outs, held):
+        torch.cuda.set_device(workspace.device)
+        start.wait()
+        for out in outs:
+            codes.append(L.adacode_paged_attn(ctypes.byref(c), q.data_ptr(), *q.stride()[:2], 16, out.data_ptr(), *out.stride()[:2], None, longest, scale, 1, 0,
+                                              workspace.data_ptr(), workspace.numel(), status.data_ptr(), stream))
+    threads = [threading.Thread(target=work, args=x) for x in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert codes == [_lib.OK] * 200
+    assert all(torch.equal(out, x[4]) for x in calls for out in x[5])
+    codec.check_device_status(workspace.device)
