@@ -75,6 +75,7 @@ struct Piece {
     int n, j0;                // tiles, the first of them; n == 0: no more pieces
     int rows, row0;           // of the unit: how many, the first within the sequence's head
     int b, h, q0, fresh, len, start;
+    int lo, hi;               // positions that any of the unit's rows sees: lo .. hi - 1
     int slot;                 // of the partial results, -1: the unit is whole
 };
 
@@ -235,7 +236,7 @@ __device__ __forceinline__ void weigh(const uint32_t (&x)[32], Two c, Two base, 
 // units
 // ---------------------------------------------------------------------------------------
 
-// Positions that new token t (of `fresh`) of a sequence sees: lo .. hi - 1.
+// Positions that new token t (of `fresh`) of a sequence sees: lo .. hi - 1, of those that the table has.
 __device__ __forceinline__ void seen_by(const PagedArgs &a, int t, int fresh, int len, int start, int &lo, int &hi) {
     const int at = len - fresh + t;
     lo = start > 0 ? start : 0;
@@ -243,15 +244,29 @@ __device__ __forceinline__ void seen_by(const PagedArgs &a, int t, int fresh, in
     hi = a.causal && at + 1 < len ? at + 1 : len;
     if (hi > a.room) hi = a.room;
 }
-// Tiles of the unit of rows row0 .. row1 - 1 (one, of hidden positions, if it sees none).
-__device__ __forceinline__ int unit_tiles(const PagedArgs &a, int row0, int row1, int fresh, int len, int start, int &first) {
-    int lo, hi, other;
+// Those that any of rows row0 .. row1 - 1 sees.
+__device__ __forceinline__ void seen_by_unit(const PagedArgs &a, int row0, int row1, int fresh, int len, int start, int &lo, int &hi) {
+    int other;
     seen_by(a, (uint32_t)row0 / a.by_group, fresh, len, start, lo, other);
     seen_by(a, (uint32_t)(row1 - 1) / a.by_group, fresh, len, start, other, hi);
+}
+// Whether the last of them sees a position that the table does not have.
+__device__ __forceinline__ bool beyond_table(const PagedArgs &a, const Piece &p) {
+    if (p.len <= a.room) return false;
+    const int t = (int)((uint32_t)(p.row0 + p.rows - 1) / a.by_group), at = p.len - p.fresh + t, to = a.causal && at + 1 < p.len ? at + 1 : p.len;
+    return to > a.room && p.lo < to;
+}
+// The tiles of positions lo .. hi - 1 (one, of hidden positions, if there are none).
+__device__ __forceinline__ int tiles_of(int lo, int hi, int &first) {
     first = lo / kTile;
     const int n = (hi > 0 ? (hi - 1) / kTile + 1 : 0) - first;
     if (n <= 0) first = 0;
     return n > 0 ? n : 1;
+}
+__device__ __forceinline__ int unit_tiles(const PagedArgs &a, int row0, int row1, int fresh, int len, int start, int &first) {
+    int lo, hi;
+    seen_by_unit(a, row0, row1, fresh, len, start, lo, hi);
+    return tiles_of(lo, hi, first);
 }
 __device__ __forceinline__ void sequence(const PagedArgs &a, int b, int &q0, int &fresh, int &len, int &start) {
     if (a.cache.cu_seqlens) {
@@ -490,7 +505,9 @@ __device__ __forceinline__ bool load_tiles(const PagedArgs &a, const Piece &p, c
         int page = next_page, slot = next_slot;
         if (lane < boxes && (page < 0 || page >= c.n_pages)) {        // (a page behind the pool reads as zeros)
             page = c.n_pages, slot = 0;
-            atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
+            // (pages of which nothing is seen need not exist: windows leave them behind)
+            const int at = at0 + j * kTile;
+            if (at + a.box_rows > p.lo && at < p.hi) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
         }
         next_boxes = boxes_of(j + 1);
         look_up(j + 1);
@@ -537,7 +554,8 @@ __device__ __forceinline__ void load_keys(const PagedArgs &a, Shared<D, SOLO> &s
     cut.n = 0;
     while (left > 0) {
         int first;
-        const int all = unit_tiles(a, p.row0, p.row0 + p.rows, p.fresh, p.len, p.start, first);
+        seen_by_unit(a, p.row0, p.row0 + p.rows, p.fresh, p.len, p.start, p.lo, p.hi);
+        const int all = tiles_of(p.lo, p.hi, first);
         const bool whole = all - skipped <= left;
         p.j0 = first + skipped;
         p.n = whole ? all - skipped : left;
@@ -550,7 +568,7 @@ __device__ __forceinline__ void load_keys(const PagedArgs &a, Shared<D, SOLO> &s
         }
         pr.next();
         ok = load_tiles<D, S::kKeys>(a, p, map, r, s.k, s.k_full, s.k_empty);
-        if (p.len > a.room && lane == 0) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
+        if (beyond_table(a, p) && lane == 0) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
         if (!ok) break;
         left -= p.n;
         if (skipped == 0 && !whole) {

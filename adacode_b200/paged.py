@@ -11,7 +11,8 @@ after the other along the first dimension; ``cu_seqlens`` int32 ``[B + 1]`` says
 many), and tokens before ``cu_seqlens[0]`` or from ``cu_seqlens[B]`` on are padding, which is left alone.  Tables and lengths stay on the device: a call
 never waits for them, and a captured call may be replayed with others.  What only they can show to be wrong, a position without a page
 of the pool, is never followed: nothing is written there, zeros are read, and the device's
-status word says so (``codec.check_device_status``).
+status word says so (``codec.check_device_status``).  Pages of which no new token sees anything (before all windows, inside
+the left padding) need no entry for ``paged_attention``.
 
 The reference has neither: its caches concatenate (float_cache_utils.py:860-881) what the model has rotated with torch
 operations, and rebuild dense keys and values for the model's own attention (:1342).

@@ -397,7 +397,7 @@ int adacode_decode_attn(const void *q_bf16, int64_t q_stride_b, int64_t q_stride
  * last.  All pointers but this struct's own are device memory and nothing of them is read by the host, so that a call can be
  * captured into a graph and replayed with other lengths, tables and contents.
  * A table entry that is none of 0 .. n_pages - 1, or a position behind the table, is never followed (nothing is written there,
- * and zeros are read): ADACODE_STATUS_BAD_PAGE.
+ * and zeros are read): ADACODE_STATUS_BAD_PAGE, unless no new token sees any position of that page.
  */
 typedef struct adacode_paged_cache {
     void *key_pages, *value_pages;           /* [n_pages][Hkv][page_size][D] */

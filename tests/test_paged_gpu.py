@@ -560,3 +560,28 @@ def test_threads_share_a_stream_and_a_workspace():
     assert codes == [_lib.OK] * 200
     assert all(torch.equal(out, x[4]) for x in calls for out in x[5])
     codec.check_device_status(workspace.device)
+
+
+@pytest.mark.parametrize('page', [16, 128])
+@pytest.mark.parametrize('T', [1, 3, 140])
+def test_hidden_pages_need_no_entry(T, page):
+    """Pages before the window and inside the left padding may have been given back: their entries are no pages, and nothing is reported."""
+    from adacode_b200 import _lib, codec, paged_attention
+    lens = [T + 700, T + 390]
+    k, v, table, seq = oracle.make_cache(lens, 2, 64, page, torch.bfloat16, fill=math.nan)
+    q = torch.randn((2 * T, 8, 64), device='cuda').bfloat16()
+    starts = torch.tensor([0, 300], dtype=I32, device='cuda')
+    codec.check_device_status(q.device)
+    for more, hidden in ((dict(window=60), [700 - 59, 390 - 59]), (dict(starts=[0, 300]), [0, 300]), (dict(window=150, starts=[0, 300]), [700 - 149, 300])):
+        args = {('seq_starts' if n == 'starts' else n): (starts if n == 'starts' else x) for n, x in more.items()}
+        want, size = oracle.attention(q, k, v, table, lens, [T, T], **more)
+        for gone in (-1, k.shape[0]):
+            partly = table.clone()
+            for b, n in enumerate(hidden):
+                partly[b, :n // page] = gone
+            close(paged_attention(q, k, v, partly, seq, max_query_len=T, **args), want, size, torch.bfloat16, max(lens))
+            codec.check_device_status(q.device)
+            partly[0, hidden[0] // page] = gone                                          # one more: a page that is seen
+            paged_attention(q, k, v, partly, seq, max_query_len=T, **args)
+            with pytest.raises(_lib.AdacodeError, match='no page'):
+                codec.check_device_status(q.device)
