@@ -21,9 +21,10 @@
 // 2300 cycles, products 1300; two streams take turns); one token behind 2050 12.5 us, bound by latency (finding the run some 3500 cycles, one
 // tile 8000, the merge).
 //
-// Hidden positions get the score minus infinity; their values would still be multiplied by the weight 0.  Values behind the sequence's end are
-// cleared in shared memory.  Others (left padding, later tokens of the chunk) only matter if they are infinite or NaN: a row that ends with such
-// a numerator but a finite sum is computed again by repair_row, which never looks at what is hidden.
+// Hidden positions get the score minus infinity; their values would still be multiplied by the weight 0.  Values that no row of the unit sees
+// (behind its last token, before its first one's window, left padding, which a model may well leave full of NaN) are cleared in shared memory.
+// Others, which some rows see, only matter if they are infinite or NaN: a row that ends with such a numerator but a finite sum is computed again by
+// repair_row, which never looks at what is hidden.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -643,7 +644,7 @@ __device__ __forceinline__ bool multiply_pieces(const PagedArgs &a, Shared<D, SO
     const auto release = [&](uint64_t *bar) { mma_commit(leader, bar); };
     for (;;) {
         if (!warp_wait(&s.piece_full[pr.at], pr.phase, a.status)) return false;
-        const int tiles = s.piece[pr.at].n, rows = s.piece[pr.at].rows, held = s.piece[pr.at].len - s.piece[pr.at].j0 * kTile;
+        const int tiles = s.piece[pr.at].n, rows = s.piece[pr.at].rows, j0 = s.piece[pr.at].j0 * kTile, lo = s.piece[pr.at].lo - j0, hi = s.piece[pr.at].hi - j0;
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.piece_empty[pr.at]);
         pr.next();
@@ -663,12 +664,16 @@ __device__ __forceinline__ bool multiply_pieces(const PagedArgs &a, Shared<D, SO
         }
         for (int t = 0; t < tiles; ++t) {
             if (!warp_wait(&s.v_full[vr.at], vr.phase, a.status)) return false;
-            const int valid = held - t * kTile;
-            if (valid < kTile) {             // rows behind the sequence's end are cleared
-                for (int x = (valid > 0 ? valid : 0) * (D / 8) + lane; x < kTile * (D / 8); x += 32) {
-                    const int row = x / (D / 8), col = x - row * (D / 8);
-                    *reinterpret_cast<uint4 *>(s.v[vr.at] + (col / 8) * S::kHalf + row * 128 + (col % 8) * 16) = make_uint4(0, 0, 0, 0);
-                }
+            const int from = lo - t * kTile, to = hi - t * kTile;
+            if (from > 0 || to < kTile) {    // values that no row of the unit sees are cleared
+                const auto clear = [&](int row0, int row1) {
+                    for (int x = row0 * (D / 8) + lane; x < row1 * (D / 8); x += 32) {
+                        const int row = x / (D / 8), col = x - row * (D / 8);
+                        *reinterpret_cast<uint4 *>(s.v[vr.at] + (col / 8) * S::kHalf + row * 128 + (col % 8) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                };
+                clear(0, from < kTile ? from : kTile);
+                clear(to > 0 ? to : 0, kTile);
                 fence_async_smem();
                 __syncwarp();
             }

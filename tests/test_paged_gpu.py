@@ -585,3 +585,41 @@ def test_hidden_pages_need_no_entry(T, page):
             paged_attention(q, k, v, partly, seq, max_query_len=T, **args)
             with pytest.raises(_lib.AdacodeError, match='no page'):
                 codec.check_device_status(q.device)
+
+
+def milliseconds(call, times=5):
+    """The least of some times on the device."""
+    call()
+    taken = []
+    for _ in range(times):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        call()
+        b.record()
+        b.synchronize()
+        taken.append(a.elapsed_time(b))
+    return min(taken)
+
+
+@pytest.mark.parametrize('T', [1, 5, 200])
+def test_infinities_in_left_padding_cost_nothing(T):
+    """What every row of a sequence's new tokens is kept from seeing (padding, what lies before all windows) is out of the way before it is multiplied:
+    a model's padding may hold NaN in every layer.  (The bound is far above what a call's time varies by: computed again row by row such a
+    call took 80 to 500 times as long.)"""
+    from adacode_b200 import codec, paged_attention
+    B, L = 2, 4000
+    k, v = (torch.randn((B, 8, L, 128), device='cuda').bfloat16() for _ in range(2))
+    table, seq = torch.arange(B, dtype=I32, device='cuda')[:, None], torch.full((B,), L, dtype=I32, device='cuda')
+    q = torch.randn((B * T, 32, 128), device='cuda').bfloat16()
+    for more in (dict(seq_starts=torch.tensor([100, 1000], dtype=I32, device='cuda')), dict(window=1500)):
+        call = lambda: paged_attention(q, k, v, table, seq, max_query_len=T, **more)     # noqa: E731, B023
+        want, plain = call(), milliseconds(call)
+        odd = v.clone()
+        for b, n in enumerate([100, 1000] if 'window' not in more else [L - T - 1500 + 1] * B):
+            odd[b, :, :n] = math.nan
+        v, kept = odd, v
+        assert torch.equal(call(), want)
+        spoilt = milliseconds(call)
+        v = kept
+        assert spoilt < 5 * plain + 0.05, (spoilt, plain)
+    codec.check_device_status(q.device)
