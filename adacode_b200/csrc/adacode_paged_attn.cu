@@ -29,6 +29,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include "adacode.h"
@@ -784,7 +785,7 @@ __device__ __forceinline__ bool soften_pieces(const PagedArgs &a, Shared<D, SOLO
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.f : m * c;
+                const float base = fmaxf(m * c, -FLT_MAX);        // (finite where all scaled scores are minus infinity, which then have no weight)
                 const Two c2 = two(c, c), base2 = two(-base, -base);
                 Two sum[2] = {two(0.f, 0.f), two(0.f, 0.f)};
 #pragma unroll
@@ -798,6 +799,8 @@ __device__ __forceinline__ bool soften_pieces(const PagedArgs &a, Shared<D, SOLO
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.p_full[stream]);
         }
+        // (the largest score has weight 1 when it becomes the maximum, unless its product with the scale has passed 32 bits)
+        if (l == 0.f && m * c > FLT_MAX) l = NAN;
         // the end of the piece; the streams of a SOLO unit are put together, half of the columns per warpgroup
         const int both = SOLO && p.n > 1;
         float f0 = 1.f, f1 = 0.f;

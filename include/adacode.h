@@ -439,7 +439,7 @@ int adacode_append_rotary(const adacode_paged_cache *cache, const adacode_rotary
  *   out[i][h] = softmax over j of (scale * query[i][h] . K[j][h / G]) times V[j][h / G],   G = Hq / Hkv,
  * for the new token at position p over the cached positions j with seq_starts[b] <= j < seq_lens[b], j <= p if `causal`, and
  * j > p - window if window > 0.  A token that sees nothing, and one all of whose scores are minus infinity, gets 0.  What a hidden position
- * holds has no influence, infinities and NaN included; a NaN score that is seen makes its row NaN; an infinite or NaN value that is seen
+ * holds has no influence, infinities and NaN included; a NaN score that is seen makes its row NaN, and so does one above all 32-bit numbers, scaled or not; an infinite or NaN value that is seen
  * gives its column what it has in 32-bit arithmetic.  Products of 16-bit values are summed up in 32 bits, the weights enter the
  * second product in the type of the pages, their sum in 32 bits.
  * `out` must not overlap the queries; scale finite.  max_query_len: the most new tokens of one sequence (an upper bound; it chooses the kernel).  D 64 or 128; pages of 16, 32, 64 or a

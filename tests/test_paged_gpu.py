@@ -623,3 +623,29 @@ def test_infinities_in_left_padding_cost_nothing(T):
         v = kept
         assert spoilt < 5 * plain + 0.05, (spoilt, plain)
     codec.check_device_status(q.device)
+
+
+@pytest.mark.parametrize('T', [1, 200])
+def test_scaled_scores_beyond_32_bits(T):
+    """A score that is finite but whose product with the scale is not counts as an infinite one: no number where it is the largest, no weight
+    where it is negative."""
+    from adacode_b200 import paged_attention
+    lens = [T + 300]
+    k, v, table, seq = oracle.make_cache(lens, 1, 64, 64, torch.bfloat16)
+    q = torch.zeros((T, 2, 64), dtype=torch.bfloat16, device='cuda')
+    q[:, 0, 0], q[:, 1, 0] = 1.0, -1.0
+    at = (int(table[0, 1]), 0, 3)
+    k[..., 0] = 0.0
+    k[at[0], at[1], at[2], 0] = 2.0 ** 120
+    for sign in (1.0, -1.0):
+        got = paged_attention(q, k, v, table, seq, scale=sign * 2.0 ** 10)
+        up, down = (0, 1) if sign > 0 else (1, 0)
+        assert torch.isnan(got[:, up]).all()
+        hidden = k.clone()
+        hidden[at] = 0.0
+        hidden[at[0], at[1], at[2], 0] = math.inf                                        # whose score of `down`, in 64 bits too, is minus infinity
+        want, size = oracle.attention(q[:, down:down + 1], hidden, v, table, lens, [T], scale=sign * 2.0 ** 10)
+        close(got[:, down:down + 1], want, size, torch.bfloat16, lens[0])
+    k[..., 0] = 2.0 ** 120
+    got = paged_attention(q, k, v, table, seq, scale=2.0 ** 10)
+    assert torch.isnan(got[:, 0]).all() and (got[:, 1] == 0).all()
