@@ -576,8 +576,9 @@ __device__ __forceinline__ void load_keys(const PagedArgs &a, Shared<D, SOLO> &s
         if (skipped == 0 && !whole) {
             // the unit goes on behind this run: its last tile is all - p.n tiles further on
             const uint32_t end = share_of(total, blockIdx.x + 1, ctas);
+            // (no CTA is behind the last, even if lengths change while the kernel runs)
             const int last = (int)(((uint64_t)(end + (all - p.n)) * ctas - 1) / total);
-            cut = {last - (int)blockIdx.x + 1, p.rows, p.row0, p.b, p.h, p.q0, p.fresh, p.len, p.start};
+            cut = {(last < ctas ? last : ctas - 1) - (int)blockIdx.x + 1, p.rows, p.row0, p.b, p.h, p.q0, p.fresh, p.len, p.start};
         }
         skipped = 0;
         if (left == 0) break;
