@@ -20,7 +20,8 @@ forward pass and has to be causal behind each sequence's padding.
 
 Limits: every cached token is attended to, head_dim 64 or 128.  A step whose attention mask hides
 any cached position (left-padded batches) or whose layer uses a sliding window cannot be served by
-the kernel; such a step raises instead of attending to the wrong tokens, and ``fused_decode``
+the kernel; such a step raises instead of attending to the wrong tokens, attention sinks (``s_aux``), soft-capped
+scores, additive biases and chunks that are not causal raise too, and ``fused_decode``
 refuses a model whose attention implementation is not the one registered here (its SDPA would see
 one token only).  Results are close to, not bit-identical with, the materialising path
 (different summation order), so generated tokens can differ where two logits are nearly tied.
@@ -33,6 +34,8 @@ from typing import Optional
 import torch
 
 ATTENTION_NAME = 'float11_fused'
+# what models hand over that changes the scores or their sum, and that neither the kernels nor SDPA take
+_NOT_SERVED = ('s_aux', 'softcap', 'position_bias')
 _active_cache = None
 
 
@@ -41,10 +44,17 @@ def float11_fused_attention(module, query, key, value, attention_mask, dropout: 
     """Attention function with the ``AttentionInterface`` signature."""
     cache = _active_cache
     chunks = cache is not None and getattr(cache, '_fused_chunks', False)
+    if cache is not None and getattr(cache, '_fused_decode', False):
+        for name in _NOT_SERVED:
+            if kwargs.get(name) is not None:
+                raise NotImplementedError(f'float11_fused attention has no {name}; use another attention implementation')
     if cache is not None and (query.shape[2] == 1 or (chunks and key.shape[2] == query.shape[2] and _behind_prefill(cache, module, query))) and \
             getattr(cache, '_fused_decode', False):
         layer = cache.layers[module.layer_idx]
         if chunks:
+            is_causal = kwargs.get('is_causal')
+            if query.shape[2] > 1 and attention_mask is None and not (getattr(module, 'is_causal', True) if is_causal is None else is_causal):
+                raise NotImplementedError('float11_fused attention of several tokens is causal; use the materialising path')
             window = getattr(module, 'sliding_window', None) or 0
             starts = None if attention_mask is None else _left_padding(cache, module.layer_idx, attention_mask, query.shape[0], layer.get_seq_length(),
                                                                        window)

@@ -1,0 +1,74 @@
+"""The attention function of a HF model on the CPU: which calls reach the layers' own attention, with what, and which are refused."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from adacode_b200 import hf_attention
+
+B, HQ, T, D, TOTAL = 2, 4, 5, 64, 200
+
+
+class Layer:
+    """A cached layer that notes how it is asked."""
+
+    def __init__(self, total=TOTAL):
+        self.total, self.asked = total, []
+
+    def get_seq_length(self):
+        return self.total
+
+    def chunk_attention(self, query, scale=None, seq_starts=None, window=0):
+        self.asked.append(('chunk', None if seq_starts is None else seq_starts.tolist(), window))
+        return torch.zeros_like(query)
+
+    def decode_attention(self, query, scale=None):
+        self.asked.append(('decode',))
+        return torch.zeros_like(query)
+
+
+def hook(monkeypatch, chunks=True, total=TOTAL):
+    layer = Layer(total)
+    cache = SimpleNamespace(layers=[layer], _fused_decode=True, _fused_chunks=chunks)
+    monkeypatch.setattr(hf_attention, '_active_cache', cache)
+
+    def call(T=T, mask=None, module=None, **more):
+        x = torch.zeros(B, HQ, T, D, dtype=torch.bfloat16)
+        out, weights = hf_attention.float11_fused_attention(module or SimpleNamespace(layer_idx=0), x, x[:, :2], x[:, :2], mask, scaling=D ** -0.5, **more)
+        assert out.shape == (B, T, HQ, D) and weights is None
+        return layer.asked[-1]
+    return call
+
+
+def causal(T, total=TOTAL, window=0, starts=(0, 0)):
+    j, at = torch.arange(total), torch.arange(total - T, total)[:, None]
+    seen = (j <= at) & (j >= torch.tensor(starts)[:, None, None])
+    return (seen & (j > at - window) if window else seen)[:, None]
+
+
+@pytest.mark.parametrize('chunks', [False, True])
+@pytest.mark.parametrize('T', [1, T])
+@pytest.mark.parametrize('name', ['s_aux', 'softcap', 'position_bias'])
+def test_what_the_kernels_leave_out_is_refused(monkeypatch, name, T, chunks):
+    """Sinks, soft-capped scores and additive biases: an attention without them is another one, from the first update on."""
+    call = hook(monkeypatch, chunks)
+    value = 30.0 if name == 'softcap' else torch.zeros(HQ)
+    for total in (TOTAL, T):
+        hf_attention._active_cache.layers[0].total = total
+        with pytest.raises(NotImplementedError, match=name):
+            call(T, **{name: value})
+    hf_attention._active_cache.layers[0].total = TOTAL
+    if chunks or T == 1:
+        assert call(T, **{name: None})[0] == ('decode' if T == 1 else 'chunk')
+
+
+def test_attention_that_is_not_causal_is_refused(monkeypatch):
+    call = hook(monkeypatch)
+    for more in (dict(is_causal=False), dict(module=SimpleNamespace(layer_idx=0, is_causal=False))):
+        with pytest.raises(NotImplementedError, match='causal'):
+            call(**more)
+        assert call(1, **more) == ('decode',)                                   # the last token sees everything either way
+        assert call(mask=causal(T, starts=(0, 7)), **more) == ('chunk', [0, 7], 0)      # a mask says what is seen
+    assert call(is_causal=True) == call(is_causal=None) == ('chunk', None, 0)
+    # what the call says goes before what the module says
+    assert call(is_causal=True, module=SimpleNamespace(layer_idx=0, is_causal=False)) == ('chunk', None, 0)
