@@ -55,9 +55,11 @@ def float11_fused_attention(module, query, key, value, attention_mask, dropout: 
             is_causal = kwargs.get('is_causal')
             if query.shape[2] > 1 and attention_mask is None and not (getattr(module, 'is_causal', True) if is_causal is None else is_causal):
                 raise NotImplementedError('float11_fused attention of several tokens is causal; use the materialising path')
-            window = getattr(module, 'sliding_window', None) or 0
-            starts = None if attention_mask is None else _left_padding(cache, module.layer_idx, attention_mask, query.shape[0], layer.get_seq_length(),
-                                                                       window)
+            # (some models' modules know their window, others hand the config's over; one that hides nothing is none)
+            window, total = kwargs.get('sliding_window') or getattr(module, 'sliding_window', None) or 0, layer.get_seq_length()
+            if window >= total:
+                window = 0
+            starts = None if attention_mask is None else _left_padding(cache, module.layer_idx, attention_mask, query.shape[0], total, window)
             if query.shape[2] > 1 or starts is not None or window:
                 return layer.chunk_attention(query, scale=scaling, seq_starts=starts, window=window).transpose(1, 2).contiguous(), None
             return layer.decode_attention(query, scale=scaling).transpose(1, 2).contiguous(), None

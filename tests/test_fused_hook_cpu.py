@@ -72,3 +72,24 @@ def test_attention_that_is_not_causal_is_refused(monkeypatch):
     assert call(is_causal=True) == call(is_causal=None) == ('chunk', None, 0)
     # what the call says goes before what the module says
     assert call(is_causal=True, module=SimpleNamespace(layer_idx=0, is_causal=False)) == ('chunk', None, 0)
+
+
+@pytest.mark.parametrize('as_argument', [False, True])
+def test_windows(monkeypatch, as_argument):
+    """A window is the module's, or handed over with every call; one that hides nothing is none, and single tokens then stay with the packed planes."""
+    call = hook(monkeypatch)
+    more = (lambda w: dict(sliding_window=w)) if as_argument else (lambda w: dict(module=SimpleNamespace(layer_idx=0, sliding_window=w)))
+    assert call(**more(50), mask=causal(T, window=50)) == ('chunk', [TOTAL - T - 49] * B, 50)
+    assert call(**more(50)) == ('chunk', None, 50)
+    assert call(1, **more(50)) == ('chunk', None, 50)
+    assert call(**more(50), mask=causal(T, window=50, starts=(0, 170))) == ('chunk', [TOTAL - T - 49, 170], 50)
+    with pytest.raises(NotImplementedError, match='masks'):
+        call(**more(50), mask=causal(T))
+    with pytest.raises(NotImplementedError, match='masks'):
+        call(**more(None), mask=causal(T, window=50))
+    for w in (TOTAL, TOTAL + 1, None):
+        assert call(1, **more(w)) == ('decode',)
+        assert call(1, mask=causal(1), **more(w)) == ('decode',)
+        assert call(**more(w), mask=causal(T, window=w or 0)) == ('chunk', None, 0)
+        assert call(**more(w)) == ('chunk', None, 0)
+    assert call(1, **more(TOTAL - 1)) == ('chunk', None, TOTAL - 1)

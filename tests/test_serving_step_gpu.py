@@ -275,3 +275,41 @@ def test_masks_are_read_again_in_every_pass():
             for layer in layers:
                 got, _ = hf_attention.float11_fused_attention(layer, q, k[:, :, -T:], v[:, :, -T:], mask)
                 near(got.reshape(B * T, Hq, D), want, size)
+
+
+def windowed_model(kind, impl=None):
+    """Layers with a sliding window: all of them, which their attention modules hand over with every call, or the second of two."""
+    import transformers
+    common = dict(hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=64, vocab_size=320,
+                  max_position_embeddings=2048, sliding_window=100)
+    cfg = transformers.MistralConfig(**common) if kind == 'all' else transformers.Qwen3Config(**common, use_sliding_window=True, max_window_layers=1)
+    torch.manual_seed(0)
+    model = transformers.AutoModelForCausalLM.from_config(cfg).to(torch.bfloat16).cuda().eval()
+    if impl:
+        model.config._attn_implementation = impl
+    return model
+
+
+@pytest.mark.parametrize('padded', [False, True])
+@pytest.mark.parametrize('kind', ['all', 'second'])
+def test_hf_chunks_with_sliding_windows(kind, padded):
+    from transformers import DynamicCache
+    from adacode_b200 import hf_attention
+    stock, fused = windowed_model(kind), windowed_model(kind, hf_attention.register())
+    g = torch.Generator('cpu').manual_seed(3)
+    turns = [50, 9, 1, 60, 1, 40, 1, 150]                                                # below the window, across and above it
+    ids = torch.randint(3, 320, (2, sum(turns)), generator=g).cuda()
+    mask = torch.ones_like(ids)
+    if padded:
+        mask[1, :21] = 0
+    reference, cache = DynamicCache(config=stock.config), cache_of(2)
+    with torch.no_grad(), hf_attention.fused_decode(cache, fused, chunks=True):
+        at = 0
+        for T in turns:
+            position = (mask[:, :at + T].cumsum(1) - 1).clamp(min=0)[:, at:]
+            a = stock(ids[:, at:at + T], attention_mask=mask[:, :at + T], position_ids=position, past_key_values=reference, use_cache=True).logits
+            b = fused(ids[:, at:at + T], attention_mask=mask[:, :at + T], position_ids=position, past_key_values=cache, use_cache=True).logits
+            at += T
+            real = mask[:, at - T:at].bool()
+            # (two layers in bf16, as in test_hf_chunks)
+            assert float((a - b)[real].float().abs().max()) <= 16 * 2.0 ** -8 * float(a[real].float().abs().max())
