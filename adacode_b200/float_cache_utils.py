@@ -173,8 +173,7 @@ class _Rotary:
             raise ValueError(f'the head size must be even and at most 512, got {D}')
         if any(x.device != key_states.device for x in (query, value_states, cos, sin)):
             raise ValueError('queries, keys, values and angles must be on one device')
-        if torch.is_grad_enabled() and any(x.requires_grad for x in (query, key_states, value_states, cos, sin)):
-            raise RuntimeError('update_rotary has no backward pass: call it under torch.no_grad()')
+        paged.refuse_autograd('update_rotary', (query, key_states, value_states, cos, sin), ())
         if cos.shape != sin.shape or cos.dim() not in (3, 4) or cos.shape[-2] != T or cos.shape[-3] not in (1, B):
             raise ValueError(f'cos and sin must be [B or 1, T, R] or [axes, B or 1, T, R] for B = {B}, T = {T}: got {list(cos.shape)} and {list(sin.shape)}')
         R = cos.shape[-1]

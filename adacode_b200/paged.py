@@ -23,6 +23,7 @@ import ctypes
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .codec import _scratch_for, device_status
@@ -80,7 +81,9 @@ def _states(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype) -> tor
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _refuse_autograd(what: str, read: tuple, written_to: tuple) -> None:
+def refuse_autograd(what: str, read: tuple, written_to: tuple) -> None:
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (*read, *written_to)):
+        raise RuntimeError(f'{what} has no forward-mode derivative: hand over the primal tensors')
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*read, *written_to)):
         raise RuntimeError(f'{what} has no backward pass: call it under torch.no_grad()')
     if not torch.is_inference_mode_enabled() and any(t is not None and t.is_inference() for t in written_to):
@@ -148,7 +151,7 @@ def append_rotary(key: torch.Tensor, value: torch.Tensor, cos: torch.Tensor, sin
             raise ValueError(f'out must be {dtype} {[N, Hq, D]} with unit stride along D')
     elif out is not None:
         raise ValueError('out without query')
-    _refuse_autograd('append_rotary', (key, value, cos, sin, query), (key_pages, value_pages, out))
+    refuse_autograd('append_rotary', (key, value, cos, sin, query), (key_pages, value_pages, out))
     dev = key_pages.device
     sc = _scratch_for(dev)
     _same_device(dev, key=key, value=value, cos=cos, sin=sin, value_pages=value_pages, block_table=block_table, seq_lens=seq_lens, query=query,
@@ -217,7 +220,7 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
         max_query_len = N // cache.B if cu_seqlens is None else N
     elif max_query_len < 0:
         raise ValueError('max_query_len must not be negative')
-    _refuse_autograd('paged_attention', (query, key_pages, value_pages), (out,))
+    refuse_autograd('paged_attention', (query, key_pages, value_pages), (out,))
     dev = key_pages.device
     sc = _scratch_for(dev)
     _same_device(dev, query=query, value_pages=value_pages, block_table=block_table, seq_lens=seq_lens, cu_seqlens=cu_seqlens,

@@ -115,3 +115,41 @@ def test_attention_refuses_scales_and_outputs():
     for more in ({'scale': float('nan')}, {'scale': float('inf')}, {'scale': -1e39}, {'out': q}):
         with pytest.raises(ValueError, match='scale|out'):
             paged_attention(q, k, v, table, lens, **more)
+
+
+def test_no_forward_derivatives():
+    """A tangent that a call would drop is refused; primal tensors inside a dual level are not."""
+    from torch.autograd import forward_ad
+    from adacode_b200 import _lib
+    k, v, table, lens = cache()
+    q, x, c = torch.zeros(4, 4, 64, dtype=BF), torch.zeros(4, 2, 64, dtype=BF), torch.zeros(4, 32)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))            # noqa: E731
+        with torch.no_grad():
+            for args in ((dual(q), k, v, table, lens), (q, dual(k), v, table, lens), (q, k, dual(v), table, lens)):
+                with pytest.raises(RuntimeError, match='derivative'):
+                    paged_attention(*args)
+            with pytest.raises(RuntimeError, match='derivative'):
+                paged_attention(q, k, v, table, lens, out=dual(torch.zeros_like(q)))
+            for i in range(6):
+                args = [x, x, c, c, k, v]
+                args[i] = dual(args[i])
+                with pytest.raises(RuntimeError, match='derivative'):
+                    append_rotary(*args, table, lens)
+            with pytest.raises(RuntimeError, match='derivative'):
+                append_rotary(x, x, c, c, k, v, table, lens, query=dual(q))
+        with pytest.raises(_lib.AdacodeError, match='CUDA'):                    # (as outside: they are on the CPU)
+            paged_attention(q, k, v, table, lens)
+
+
+def test_no_forward_derivatives_through_the_cache():
+    from torch.autograd import forward_ad
+    from adacode_b200.float_cache_utils import _Rotary
+    q, x, c = torch.zeros(1, 4, 3, 64, dtype=BF), torch.zeros(1, 2, 3, 64, dtype=BF), torch.zeros(1, 3, 64)
+    with forward_ad.dual_level(), torch.no_grad():
+        for i in range(5):
+            args = [q, x, x, c, c]
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(RuntimeError, match='derivative'):
+                _Rotary(*args, None, False)
+        _Rotary(q, x, x, c, c, None, False)
