@@ -414,6 +414,16 @@ class float11Layer(DynamicLayer):
     def _active_residual_tensors(self):
         return self._res_k.tensor(), self._res_v.tensor()
 
+    def check_rotary_update(self, key_states: torch.Tensor) -> None:
+        """Refuse new keys (values are like them) that do not go with the cached ones, and buffers that may not be written to, before
+        anything is counted."""
+        buffers = [x.buf for x in (self._res_k, self._res_v) if x.buf is not None]
+        cached = [tuple(x.shape) for x in buffers] + [tuple(x.original_shape) for x in self._key_segments[:1]]
+        B, H, _, D = key_states.shape
+        if any((s[0], s[1], s[3]) != (B, H, D) for s in cached) or (cached and self.cache_device != key_states.device):
+            raise ValueError(f'the cache holds {list(cached[0])} on {self.cache_device}, the keys are {list(key_states.shape)} on {key_states.device}')
+        paged.refuse_autograd('update_rotary', (), tuple(buffers))
+
     def _append_residual(self, key_states: torch.Tensor, value_states: torch.Tensor, rotary: Optional['_Rotary'] = None) -> None:
         if rotary is not None and key_states.shape[-2] > 0:
             # the residual's buffers are the pages: one per sequence, the new tokens are its last
@@ -1201,9 +1211,11 @@ class Float11Cache(Cache):
         launch (``append_rotary``).  ``cos`` and ``sin`` are a HF model's position embeddings ``[B or 1, T, R]``, with ``sections`` ``[axes, B or 1,
         T, R]``.  Returns the rotated queries and what ``update`` returns (where ``update`` returns the keys as they came, because a fused
         attention is to read the cache, they have not been rotated)."""
-        if type(self.layers[layer_idx]).update is not float11Layer.update:
+        layer = self.layers[layer_idx]
+        if type(layer).update is not float11Layer.update:
             raise NotImplementedError('update_rotary needs keys and values with heads; this layer caches something else')
         rotary = _Rotary(query, key_states, value_states, cos, sin, sections, interleaved)
+        layer.check_rotary_update(key_states)
         keys, values = self.update(key_states, value_states, layer_idx, dict(cache_kwargs or {}, float11_rotary=rotary))
         return rotary.queries(), keys, values
 

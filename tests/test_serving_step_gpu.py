@@ -313,3 +313,35 @@ def test_hf_chunks_with_sliding_windows(kind, padded):
             real = mask[:, at - T:at].bool()
             # (two layers in bf16, as in test_hf_chunks)
             assert float((a - b)[real].float().abs().max()) <= 16 * 2.0 ** -8 * float(a[real].float().abs().max())
+
+
+def test_rotary_updates_that_do_not_fit_the_cache_leave_it_alone():
+    """Heads, sequences or head sizes other than the cached ones, and buffers that may only be written to in inference mode."""
+    D, T = 64, 3
+    k, v = (synth.kv_tensor((2, 2, 40, D), seed=s).to('cuda') for s in (7, 8))
+    cos, sin = torch.ones((1, T, D), device='cuda'), torch.zeros((1, T, D), device='cuda')
+    q = torch.randn((2, 2, T, D), device='cuda').to(BF)
+    cache = cache_of()
+    cache.update(k, v, 0)
+    good = (q, k[:, :, :T], v[:, :, :T], cos, sin, 0)
+    for wrong in ((q, k[:, :1, :T], v[:, :1, :T], cos, sin, 0), (q[:1], k[:1, :, :T], v[:1, :, :T], cos, sin, 0),
+                  (q[..., :32], k[:, :, :T, :32], v[:, :, :T, :32], cos[..., :32], sin[..., :32], 0)):
+        with pytest.raises(ValueError):
+            cache.update_rotary(*wrong)
+        assert cache.get_seq_length() == 40 and cache.layers[0]._res_k.length == cache.layers[0]._res_v.length == 40
+        packed = cache_of()                                                              # (nothing but packed blocks)
+        packed.update(*(x.repeat(1, 1, 4, 1)[:, :, :128] for x in (k, v)), 0)
+        with pytest.raises(ValueError):
+            packed.update_rotary(*wrong)
+        assert packed.get_seq_length() == 128
+    _, keys, _ = cache.update_rotary(*good)
+    assert torch.equal(keys, torch.cat([k, k[:, :, :T]], 2))
+    with torch.inference_mode():
+        inner = cache_of()
+        inner.update(k, v, 0)
+    with pytest.raises(RuntimeError, match='inference'):
+        inner.update_rotary(*good)
+    assert inner.get_seq_length() == 40 and inner.layers[0]._res_k.length == 40
+    with torch.inference_mode():
+        _, keys, _ = inner.update_rotary(*good)
+    assert torch.equal(keys, torch.cat([k, k[:, :, :T]], 2))
