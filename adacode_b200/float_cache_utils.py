@@ -189,7 +189,7 @@ class _Rotary:
         if self.cos.dtype not in (torch.bfloat16, torch.float32):
             self.cos, self.sin = self.cos.float(), self.sin.float()
         self.query = query.to(torch.bfloat16).transpose(1, 2).reshape(B * T, Hq, D)
-        self.shape = (B, T, Hq, D)
+        self.shape, self.dtype = (B, T, Hq, D), query.dtype
         self.sections, self.interleaved, self.out = sections, interleaved, self.query
 
     def append(self, key_states, value_states, key_buf, value_buf, total: int) -> None:
@@ -206,8 +206,8 @@ class _Rotary:
         return key_buf, value_buf
 
     def queries(self) -> torch.Tensor:
-        """The rotated queries, ``[B, Hq, T, D]``."""
-        return self.out.view(self.shape).transpose(1, 2)
+        """The rotated queries, ``[B, Hq, T, D]``, in the type that they came in."""
+        return self.out.view(self.shape).transpose(1, 2).to(self.dtype)
 
 
 class float11Layer(DynamicLayer):
@@ -803,9 +803,10 @@ class float11Layer(DynamicLayer):
         """Causal attention of a chunk of queries ``[B, Hq, T, D]``, those of the last T tokens that this layer caches, over all that it
         caches: drafted tokens that are verified, the next turn of a conversation, a chunk of a prompt.  ``seq_starts`` (int32 ``[B]``)
         hides the left padding in front of each sequence, ``window`` all but the last tokens before each query.  The dense view is made as for
-        ``update`` (the packed planes are decoded once, whatever T is) and read by ``paged_attention``, one page per sequence."""
-        if query.dim() != 4:
-            raise ValueError('query must be [B, Hq, T, D]')
+        ``update`` (the packed planes are decoded once, whatever T is) and read by ``paged_attention``, one page per sequence.  Queries of other
+        types are rounded to bf16, as ``update`` does with keys and values; the result has the queries' type."""
+        if query.dim() != 4 or not query.is_floating_point():
+            raise ValueError('query must be [B, Hq, T, D] of a floating type')
         B, Hq, T, D = query.shape
         keys, values = self.materialize_dense()
         if keys is None or keys.dim() != 4:
@@ -813,10 +814,10 @@ class float11Layer(DynamicLayer):
         total = int(keys.shape[2])
         if keys.shape[0] != B or T > total:
             raise ValueError(f'{T} queries of {B} sequences, and {total} cached tokens of {keys.shape[0]}')
-        tokens = query.transpose(1, 2).reshape(B * T, Hq, D)
+        tokens = query.to(torch.bfloat16).transpose(1, 2).reshape(B * T, Hq, D)
         out = paged.paged_attention(tokens, keys, values, *_dense_pages(B, total, keys.device), scale=scale, window=window,
                                     seq_starts=seq_starts)
-        return out.view(B, T, Hq, D).transpose(1, 2)
+        return out.view(B, T, Hq, D).transpose(1, 2).to(query.dtype)
 
     def _empty_states(self):
         if self.cache_device is None:
@@ -1210,7 +1211,8 @@ class Float11Cache(Cache):
         """``update`` for queries and keys that have not been rotated yet: both are, and keys and values written to the cache, in one
         launch (``append_rotary``).  ``cos`` and ``sin`` are a HF model's position embeddings ``[B or 1, T, R]``, with ``sections`` ``[axes, B or 1,
         T, R]``.  Returns the rotated queries and what ``update`` returns (where ``update`` returns the keys as they came, because a fused
-        attention is to read the cache, they have not been rotated)."""
+        attention is to read the cache, they have not been rotated).  Queries of other types than bf16 are rounded to it first, as ``update`` does with
+        keys and values, and come back in their own."""
         layer = self.layers[layer_idx]
         if type(layer).update is not float11Layer.update:
             raise NotImplementedError('update_rotary needs keys and values with heads; this layer caches something else')

@@ -345,3 +345,23 @@ def test_rotary_updates_that_do_not_fit_the_cache_leave_it_alone():
     with torch.inference_mode():
         _, keys, _ = inner.update_rotary(*good)
     assert torch.equal(keys, torch.cat([k, k[:, :, :T]], 2))
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.float32, BF])
+def test_other_types_through_the_cache(dtype):
+    """Queries of a model in another type come back in it; they are rounded to bf16, as keys and values are, on their way."""
+    B, Hq, Hkv, D, T = 1, 4, 2, 64, 5
+    k, v = (synth.kv_tensor((B, Hkv, 70, D), seed=s).to('cuda') for s in (9, 10))
+    q = torch.randn((B, Hq, T, D), device='cuda').to(dtype)
+    c, s = oracle.angles(torch.arange(70 - T, 70), D // 2)
+    cos, sin = (torch.cat([x, x], -1).float().cuda()[None] for x in (c, s))
+    cache, same = cache_of(), cache_of()
+    for x in (cache, same):
+        x.update(k[:, :, :-T], v[:, :, :-T], 0)
+    rq, _, _ = cache.update_rotary(q, k[:, :, -T:].to(dtype), v[:, :, -T:].to(dtype), cos, sin, 0)
+    want, _, _ = same.update_rotary(q.to(BF), k[:, :, -T:], v[:, :, -T:], cos, sin, 0)
+    assert rq.dtype == dtype and torch.equal(rq, want.to(dtype))
+    got = cache.layers[0].chunk_attention(rq)
+    assert got.dtype == dtype and torch.equal(got, same.layers[0].chunk_attention(want).to(dtype))
+    with pytest.raises(ValueError, match='floating'):
+        cache.layers[0].chunk_attention(rq.int())
