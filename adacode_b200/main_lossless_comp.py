@@ -26,6 +26,7 @@ import json
 import os
 import time
 from pathlib import Path
+from typing import Optional
 
 import torch
 
@@ -210,12 +211,25 @@ def get_parse() -> argparse.ArgumentParser:
                    help='with --fused_decode: updates of several tokens behind the prefill, and left-padded batches, too')
     p.add_argument('--fused_sample', action='store_true',
                    help='with --do_sample: tokens are drawn by the fused sampler, with the four settings below')
-    p.add_argument('--temperature', type=float, default=1.0)
-    p.add_argument('--top_k', type=int, default=50)
-    p.add_argument('--top_p', type=float, default=1.0)
-    p.add_argument('--min_p', type=float, default=0.0)
-    p.add_argument('--sample_seed', type=int, default=0)
+    for name, default in _SAMPLER.items():
+        p.add_argument(f'--{name}', type=type(default), default=None, help=f'with --fused_sample (default {default})')
     return p
+
+
+# the fused sampler's settings and what they are without their flags
+_SAMPLER = {'temperature': 1.0, 'top_k': 50, 'top_p': 1.0, 'min_p': 0.0, 'sample_seed': 0}
+
+
+def sampler_settings(args) -> Optional[tuple]:
+    """The fused sampler's settings, None without it; flags that would then have no effect are refused."""
+    given = [name for name in _SAMPLER if getattr(args, name) is not None]
+    if not args.fused_sample:
+        if given:
+            raise ValueError(f'--{given[0]} needs --fused_sample')
+        return None
+    if not args.do_sample:
+        raise ValueError('--fused_sample needs --do_sample')
+    return tuple(getattr(args, name) if name in given else default for name, default in _SAMPLER.items())
 
 
 def run(args) -> dict:
@@ -224,6 +238,9 @@ def run(args) -> dict:
     if args.compress_weights:
         raise NotImplementedError('--compress_weights belongs to the weight-compression subsystem, not to the cache path')
     kv_cache_impl = _resolve_kv_cache_impl(args)
+    settings = sampler_settings(args)
+    if args.fused_chunks and not (args.fused_decode and kv_cache_impl == 'float11'):
+        raise ValueError('--fused_chunks needs --fused_decode and the float11 cache')
     if kv_cache_impl in ('cpu_offload', 'nvcomp_ans'):
         raise NotImplementedError(f'--kv_cache_impl {kv_cache_impl} is a comparator cache of the reference, not provided')
     dataset_names = args.datasets or (['synthetic'] if args.use_synthetic_data else ['longbench'])
@@ -268,12 +285,10 @@ def run(args) -> dict:
         model.config._attn_implementation = hf_attention.register()
 
     sampler = None
-    if args.fused_sample:
-        if not args.do_sample:
-            raise ValueError('--fused_sample needs --do_sample')
+    if settings is not None:
         from transformers import LogitsProcessorList
         from .sampling import FusedSampler
-        sampler = LogitsProcessorList([FusedSampler(args.temperature, args.top_k, args.top_p, args.min_p, args.sample_seed)])
+        sampler = LogitsProcessorList([FusedSampler(*settings)])
 
     dn = 'synthetic'
     all_info_lists[dn] = []
