@@ -801,7 +801,7 @@ class float11Layer(DynamicLayer):
     def chunk_attention(self, query: torch.Tensor, scale: Optional[float] = None, seq_starts: Optional[torch.Tensor] = None,
                         window: int = 0) -> torch.Tensor:
         """Causal attention of a chunk of queries ``[B, Hq, T, D]``, those of the last T tokens that this layer caches, over all that it
-        caches: drafted tokens that are verified, the next turn of a conversation, a chunk of a prompt.  ``seq_starts`` (int32 ``[B]``)
+        caches: the next turn of a conversation, a chunk of a prompt.  ``seq_starts`` (int32 ``[B]``)
         hides the left padding in front of each sequence, ``window`` all but the last tokens before each query.  The dense view is made as for
         ``update`` (the packed planes are decoded once, whatever T is) and read by ``paged_attention``, one page per sequence.  Queries of other
         types are rounded to bf16, as ``update`` does with keys and values; the result has the queries' type."""
@@ -1048,6 +1048,13 @@ class float11Layer(DynamicLayer):
 
     def get_seq_length(self) -> int:
         return self.cumulative_length
+
+    def crop(self, max_length: int) -> None:
+        """Tokens cannot be taken back (packed blocks and the adjuster's counts hold them), so drafted tokens that are rejected, as in
+        assisted generation, need another cache.  Lengths that keep everything are fine."""
+        length = self.get_seq_length()
+        if length > (length + max_length if max_length < 0 else max_length):
+            raise NotImplementedError(f'crop({max_length}): this cache keeps its {length} tokens')
 
     def release(self) -> None:
         """Drop every tensor this layer holds (reference: Float11Cache.synchronize_and_release,

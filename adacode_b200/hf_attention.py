@@ -13,10 +13,11 @@ the dense tensors, as before.
     with fused_decode(cache):
         out = model.generate(ids, past_key_values=cache, ...)
 
-With ``fused_decode(cache, model, chunks=True)`` updates of several tokens behind the prefill (drafted tokens of assisted generation, the next
-turn of a conversation, a chunk of a prompt) go the same way: the chunk's attention is computed by ``paged_attention`` over the dense view,
-without the model's mask in memory.  Left-padded batches are served too, in chunks and single steps: the mask is read once per
-forward pass and has to be causal behind each sequence's padding.
+With ``fused_decode(cache, model, chunks=True)`` updates of several tokens behind the prefill (the next turn of a conversation, a chunk of a
+prompt) go the same way: the chunk's attention is computed by ``paged_attention`` over the dense view.  Left-padded batches are served too, in
+chunks and single steps.  For a chunk behind a prefill transformers makes a mask (``[B, 1, T, S]``), which the kernel does not read; it is compared once
+per forward pass, and waited for, with the causal one behind each sequence's padding, and has to be that.  Assisted generation is not served: the cache
+cannot take rejected tokens back (``crop``).
 
 Limits: every cached token is attended to, head_dim 64 or 128.  A step whose attention mask hides
 any cached position (left-padded batches) or whose layer uses a sliding window cannot be served by
