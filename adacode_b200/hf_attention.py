@@ -60,6 +60,8 @@ def float11_fused_attention(module, query, key, value, attention_mask, dropout: 
             window, total = kwargs.get('sliding_window') or getattr(module, 'sliding_window', None) or 0, layer.get_seq_length()
             if window >= total:
                 window = 0
+            if attention_mask is not None and attention_mask.shape[2] != query.shape[2]:
+                raise NotImplementedError(f'float11_fused attention: a mask of {attention_mask.shape[2]} rows for {query.shape[2]} queries')
             starts = None if attention_mask is None else _left_padding(cache, module.layer_idx, attention_mask, query.shape[0], total, window)
             if query.shape[2] > 1 or starts is not None or window:
                 return layer.chunk_attention(query, scale=scaling, seq_starts=starts, window=window).transpose(1, 2).contiguous(), None

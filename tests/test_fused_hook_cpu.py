@@ -93,3 +93,12 @@ def test_windows(monkeypatch, as_argument):
         assert call(**more(w), mask=causal(T, window=w or 0)) == ('chunk', None, 0)
         assert call(**more(w)) == ('chunk', None, 0)
     assert call(1, **more(TOTAL - 1)) == ('chunk', None, TOTAL - 1)
+
+
+def test_masks_with_one_row_for_all_queries(monkeypatch):
+    """A mask that hides padding alone, the same for all queries, is not a causal one."""
+    call = hook(monkeypatch)
+    with pytest.raises(NotImplementedError, match='mask'):
+        call(mask=causal(1, starts=(0, 9)))
+    assert call(1, mask=causal(1, starts=(0, 9))) == ('chunk', [0, 9], 0)
+    assert call(mask=causal(T, starts=(0, 9))) == ('chunk', [0, 9], 0)
