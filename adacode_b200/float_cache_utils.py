@@ -28,6 +28,7 @@ from __future__ import annotations
 import math
 import time
 import warnings
+import weakref
 from typing import Any, Optional
 
 import torch
@@ -1130,6 +1131,7 @@ class Float11Cache(Cache):
         self.peak_mem = 0
         self._fused_decode = False         # set by hf_attention.fused_decode
         self._fused_chunks = False         # also for more than one token at a time
+        self._fused_keys = {}              # layer -> the keys of its last such update, which its attention has to be asked with
         self.layout = layout
         self.seq_tile_size = seq_tile_size if seq_tile_size is not None else block_size
         self.auto_init_compress_params = auto_init_compress_params
@@ -1155,6 +1157,7 @@ class Float11Cache(Cache):
     def __getstate__(self):
         state = self.__dict__.copy()
         state['_pending_adjusts'] = {}
+        state['_fused_keys'] = {}          # (weak references)
         return state
 
     def __setstate__(self, state):
@@ -1190,6 +1193,8 @@ class Float11Cache(Cache):
         if layer_idx == len(self.layers) - 1:
             self.steps += 1
         if fused:
+            if self._fused_chunks:
+                self._fused_keys[layer_idx] = weakref.ref(key_states)
             return key_states, value_states
         return result['key_states'], result['value_states']
 

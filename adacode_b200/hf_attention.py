@@ -17,7 +17,8 @@ With ``fused_decode(cache, model, chunks=True)`` updates of several tokens behin
 prompt) go the same way: the chunk's attention is computed by ``paged_attention`` over the dense view.  Left-padded batches are served too, in
 chunks and single steps.  For a chunk behind a prefill transformers makes a mask (``[B, 1, T, S]``), which the kernel does not read; it is compared once
 per forward pass, and waited for, with the causal one behind each sequence's padding, and has to be that.  Assisted generation is not served: the cache
-cannot take rejected tokens back (``crop``).
+cannot take rejected tokens back (``crop``).  Keys that are not what the cache's last update of the layer returned, as those of a model that
+runs with another cache or with none inside the context, are refused.
 
 Limits: every cached token is attended to, head_dim 64 or 128.  A step whose attention mask hides
 any cached position (left-padded batches) or whose layer uses a sliding window cannot be served by
@@ -53,6 +54,10 @@ def float11_fused_attention(module, query, key, value, attention_mask, dropout: 
             getattr(cache, '_fused_decode', False):
         layer = cache.layers[module.layer_idx]
         if chunks:
+            updated = getattr(cache, '_fused_keys', {}).get(module.layer_idx)
+            if updated is not None and updated() is not key:
+                raise NotImplementedError('float11_fused attention: these keys are not what the last update of the cache in fused_decode returned '
+                                          '(a model with another cache, or with none?)')
             is_causal = kwargs.get('is_causal')
             if query.shape[2] > 1 and attention_mask is None and not (getattr(module, 'is_causal', True) if is_causal is None else is_causal):
                 raise NotImplementedError('float11_fused attention of several tokens is causal; use the materialising path')
@@ -153,4 +158,5 @@ def fused_decode(cache, model=None, chunks: bool = False):
         cache._fused_decode = cache._fused_chunks = False
         cache._fused_mask_seen = None
         cache._fused_masks_known = -1, []
+        cache._fused_keys = {}
         _active_cache = previous

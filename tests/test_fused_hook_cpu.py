@@ -102,3 +102,43 @@ def test_masks_with_one_row_for_all_queries(monkeypatch):
         call(mask=causal(1, starts=(0, 9)))
     assert call(1, mask=causal(1, starts=(0, 9))) == ('chunk', [0, 9], 0)
     assert call(mask=causal(T, starts=(0, 9))) == ('chunk', [0, 9], 0)
+
+
+def test_keys_of_another_cache_are_refused(monkeypatch):
+    """Inside fused_decode(chunks=True), attention of a model that runs without the cache, or with another one, is not answered from the cache."""
+    import adacode_b200.float_cache_utils as fc
+    from adacode_b200 import Float11Cache
+    from tests.scenarios import StubConfig
+    from tests.test_state_machine_cpu import oracle_codec
+    monkeypatch.setattr(fc, 'codec', oracle_codec)
+    caches = [Float11Cache(StubConfig(1), right=129, exp_bits=4, need_adjust=False, update_steps=0, block_size=128, layout='segmented_tiled') for _ in range(2)]
+    x = torch.randn((B, 2, 150, D)).to(torch.bfloat16)
+    asked = []
+
+    def answer(name):
+        def attend(self, query, **more):
+            asked.append((name, self))
+            return torch.zeros_like(query)
+        return attend
+    monkeypatch.setattr(fc.float11Layer, 'chunk_attention', answer('chunk'))
+    monkeypatch.setattr(fc.float11Layer, 'decode_attention', answer('decode'))
+    module = SimpleNamespace(layer_idx=0)
+    attend = lambda key: hf_attention.float11_fused_attention(module, torch.zeros(B, HQ, key.shape[2], D, dtype=torch.bfloat16), key, key, None)     # noqa: E731
+    with hf_attention.fused_decode(caches[0], chunks=True):
+        for _ in range(2):
+            for n in (100, 5, 1):
+                key, _ = caches[0].update(x[:, :, :n], x[:, :, :n], 0)
+                if caches[0].get_seq_length() > 100:
+                    attend(key)
+                    assert asked.pop() == ('decode' if n == 1 else 'chunk', caches[0].layers[0])
+                    other, _ = caches[1].update(x[:, :, :n], x[:, :, :n], 0)
+                    for foreign in (other[:, :, -n:], x[:, :, :n].clone()):
+                        with pytest.raises(NotImplementedError, match='another'):
+                            attend(foreign)
+        assert not asked
+        import pickle
+        assert pickle.loads(pickle.dumps(caches[0])).get_seq_length() == caches[0].get_seq_length()
+    # outside, and inside a context of single tokens, chunks are SDPA's
+    key = x[:, :, :5].repeat(1, 2, 1, 1)
+    out, _ = hf_attention.float11_fused_attention(SimpleNamespace(layer_idx=0), key, key, key, None)
+    assert out.shape == (B, 5, HQ, D) and not asked
