@@ -469,6 +469,13 @@ bool is_states(const Arg &a, int64_t N, int64_t heads, const Arg &pages) {
     const int64_t D = pages->size(3);
     return a->scalar_type() == pages->scalar_type() && is_shape(a, {N, heads, D}) && (D == 1 || a->stride(2) == 1);
 }
+// (what is written to: a stride of 0 gives several elements one place)
+bool overlaps_itself(const Arg &a) {
+    if (!a.given()) return false;
+    for (int d = 0; d < a->dim(); ++d)
+        if (a->size(d) > 1 && a->stride(d) == 0) return true;
+    return false;
+}
 bool on_sixteen_bytes(const Arg &a) {
     if ((uintptr_t)a.at() & 15) return false;
     for (int d = 0; d + 1 < a->dim(); ++d)
@@ -489,7 +496,7 @@ PyObject *append_rotary(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     const int64_t N = key->size(0);
     adacode_paged_cache c;
     if (!describe_cache(keys, values, table, lens, cu, N, c) || !is_states(key, N, c.Hkv, keys) || !is_states(value, N, c.Hkv, keys)) Py_RETURN_FALSE;
-    if (c.D % 2 != 0 || c.D > 512) Py_RETURN_FALSE;
+    if (c.D % 2 != 0 || c.D > 512 || overlaps_itself(keys) || overlaps_itself(values) || overlaps_itself(given)) Py_RETURN_FALSE;
     const int type = element_type(*cos.t);
     if (sin->sizes() != cos->sizes() || sin->strides() != cos->strides() || sin->scalar_type() != cos->scalar_type() || (type != ADACODE_FP32 && type != c.dtype) ||
         (cos->dim() != 2 && cos->dim() != 3))
@@ -558,7 +565,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n_args) 
         scale = PyFloat_AS_DOUBLE(args[7]);
         if (!std::isfinite((float)scale)) Py_RETURN_FALSE;
     }
-    if (given.given() && given.at() == query.at()) Py_RETURN_FALSE;
+    if ((given.given() && given.at() == query.at()) || overlaps_itself(given)) Py_RETURN_FALSE;
     if (!on_sixteen_bytes(keys) || !on_sixteen_bytes(values) || !on_sixteen_bytes(query) || (given.given() && !on_sixteen_bytes(given))) Py_RETURN_FALSE;
     const c10::cuda::CUDAGuard on(keys->device());
     const Tensor out = given.given() ? *given.t : at::empty({N, Hq, c.D}, query->options());

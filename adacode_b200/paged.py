@@ -81,6 +81,12 @@ def _states(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype) -> tor
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _refuse_overlap(**written_to) -> None:
+    for name, t in written_to.items():
+        if t is not None and any(stride == 0 and n > 1 for stride, n in zip(t.stride(), t.shape)):
+            raise ValueError(f'{name} is written to and must not overlap itself: strides {list(t.stride())}')
+
+
 def refuse_autograd(what: str, read: tuple, written_to: tuple) -> None:
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (*read, *written_to)):
         raise RuntimeError(f'{what} has no forward-mode derivative: hand over the primal tensors')
@@ -104,7 +110,7 @@ def append_rotary(key: torch.Tensor, value: torch.Tensor, cos: torch.Tensor, sin
     frequencies are taken from each axis.
 
     Keys (rotated, in 32 bits and rounded once) and values are written to the last tokens of their sequences.  Returns the rotated
-    queries, in ``out`` if given (which may be ``query``), or None without ``query``.
+    queries, in ``out`` if given (which may be ``query``, and must not overlap any other argument), or None without ``query``.
     """
     if key_pages.is_cuda:
         got = _lib.native().append_rotary(key, value, cos, sin, key_pages, value_pages, block_table, seq_lens, query, cu_seqlens,
@@ -151,6 +157,7 @@ def append_rotary(key: torch.Tensor, value: torch.Tensor, cos: torch.Tensor, sin
             raise ValueError(f'out must be {dtype} {[N, Hq, D]} with unit stride along D')
     elif out is not None:
         raise ValueError('out without query')
+    _refuse_overlap(key_pages=key_pages, value_pages=value_pages, out=out)
     refuse_autograd('append_rotary', (key, value, cos, sin, query), (key_pages, value_pages, out))
     dev = key_pages.device
     sc = _scratch_for(dev)
@@ -220,6 +227,7 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
         max_query_len = N // cache.B if cu_seqlens is None else N
     elif max_query_len < 0:
         raise ValueError('max_query_len must not be negative')
+    _refuse_overlap(out=out)
     refuse_autograd('paged_attention', (query, key_pages, value_pages), (out,))
     dev = key_pages.device
     sc = _scratch_for(dev)

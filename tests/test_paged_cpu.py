@@ -153,3 +153,25 @@ def test_no_forward_derivatives_through_the_cache():
             with pytest.raises(RuntimeError, match='derivative'):
                 _Rotary(*args, None, False)
         _Rotary(q, x, x, c, c, None, False)
+
+
+def test_outputs_that_overlap_themselves_are_refused():
+    """As copy_ refuses them: every element of what is written to has a place of its own."""
+    k, v, table, lens = cache()
+    q, x, c = torch.zeros(4, 4, 64, dtype=BF), torch.zeros(4, 2, 64, dtype=BF), torch.zeros(4, 32)
+    for out in (torch.zeros(1, 4, 64, dtype=BF).expand(4, 4, 64), torch.zeros(4, 1, 64, dtype=BF).expand(4, 4, 64)):
+        with pytest.raises(ValueError, match='overlap'):
+            paged_attention(q, k, v, table, lens, out=out)
+        with pytest.raises(ValueError, match='overlap'):
+            append_rotary(x, x, c, c, k, v, table, lens, query=q, out=out)
+    for n in range(3):
+        shape = list(k.shape)
+        shape[n] = 1
+        flat = torch.zeros(shape, dtype=BF).expand(k.shape)
+        for pages in ((flat, v), (k, flat)):
+            with pytest.raises(ValueError, match='overlap'):
+                append_rotary(x, x, c, c, *pages, table, lens)
+    one = torch.zeros(1, 1, 64, dtype=BF)                                       # (a dimension of one entry may have any stride)
+    from adacode_b200 import _lib
+    with pytest.raises(_lib.AdacodeError, match='CUDA'):
+        paged_attention(one, k[:, :1], v[:, :1], table[:1], lens[:1], out=torch.zeros(64, dtype=BF).as_strided((1, 1, 64), (0, 0, 1)))

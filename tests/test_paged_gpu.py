@@ -649,3 +649,20 @@ def test_scaled_scores_beyond_32_bits(T):
     k[..., 0] = 2.0 ** 120
     got = paged_attention(q, k, v, table, seq, scale=2.0 ** 10)
     assert torch.isnan(got[:, 0]).all() and (got[:, 1] == 0).all()
+
+
+def test_outputs_that_overlap_themselves_are_refused():
+    from adacode_b200 import append_rotary, paged_attention
+    k, v, table, seq = oracle.make_cache([20, 9], 2, 64, 16, torch.bfloat16)
+    q, x, c = torch.randn((4, 4, 64), device='cuda').bfloat16(), torch.randn((4, 2, 64), device='cuda').bfloat16(), torch.ones((4, 32), device='cuda')
+    out = torch.zeros((1, 4, 64), dtype=torch.bfloat16, device='cuda').expand(4, 4, 64)
+    with pytest.raises(ValueError, match='overlap'):
+        paged_attention(q, k, v, table, seq, out=out)
+    with pytest.raises(ValueError, match='overlap'):
+        append_rotary(x, x, c, c, k, v, table, seq, query=q, out=out)
+    with pytest.raises(ValueError, match='overlap'):
+        append_rotary(x, x, c, c, k, v[:, :1].expand(v.shape), table, seq)
+    assert (out == 0).all()
+    # pages that are only read may
+    got = paged_attention(q, k, v, table, seq)
+    assert torch.isfinite(got).all()
