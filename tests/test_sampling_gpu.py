@@ -182,3 +182,16 @@ def test_few_neighbours_among_the_lowest_value(V, dtype):
     for s in (dict(top_k=50), dict(top_k=400, temperature=4.0), dict(top_k=50, top_p=0.95), dict(top_k=50, temperature=0.05)):
         for u in (torch.rand(len(rows), generator=g), torch.full((len(rows),), 1 - 2.0 ** -24)):
             check(logits, u.cuda(), **s)
+
+
+def test_draws_at_every_batch_size():
+    """A row's token is what 64 bits give, whatever stands beside it: how many CTAs have a row changes the order of the sums alone."""
+    from adacode_b200 import sample_tokens
+    g = torch.Generator('cpu').manual_seed(13)
+    row = (torch.randn((1, 40000), generator=g) * 3).cuda()
+    u = torch.rand(1, generator=g).cuda()
+    for s in (dict(), dict(top_p=0.9), dict(top_k=50, top_p=0.9), dict(min_p=0.01)):
+        for B in (1, 40, 100, 400):
+            f32 = {k: float(torch.tensor(v)) if isinstance(v, float) else v for k, v in s.items()}
+            want, near = oracle.sample(row[0].cpu(), u.item(), **f32)
+            assert near > 1e-10 and sample_tokens(row.expand(B, -1), u.expand(B).contiguous(), **s).tolist() == [want] * B
