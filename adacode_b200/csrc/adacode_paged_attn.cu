@@ -64,7 +64,7 @@ struct PagedArgs {
     float scale;              // times log2 e, positive (queries are negated where it is negative; 0 is the smallest there is: hidden
                               // scores are minus infinity, and that times 0 is no number)
     uint32_t negate;
-    int box_rows;             // rows per tensor copy
+    int box_shift;            // 2**box_shift rows per tensor copy
     int room;                 // positions that the table has
     Quotient by_page, by_group;
     float *part_o, *part_ml;  // [2 CTAs][rows][D], [2 CTAs][rows][2]
@@ -478,24 +478,26 @@ __device__ __forceinline__ int find_run(const PagedArgs &a, int cta, Piece &p, i
     return (int)(end - x);
 }
 
-// Loads the keys or the values of a piece.  Lane i has the i-th page (of box_rows slots) of a tile; the table is read one tile ahead, so that its
-// latency hides behind the copies.  A copy brings 64 columns of a page, issued by a lane of its own.  Keys and values have a warp each: with one
-// for both, sixteen sequences of five tokens over pages of 16 took 62 us instead of 48.
+// Loads the keys or the values of a piece.  Lane i has the i-th page (or box of slots of one) of a tile; the table is read one tile ahead, so that
+// its latency hides behind the copies.  Pages of which no row of the unit sees anything are neither looked up, they need not exist, nor copied.  A
+// copy brings 64 columns of a page, issued by a lane of its own.  Keys and values have a warp each: with one for both, sixteen sequences of five
+// tokens over pages of 16 took 62 us instead of 48.
 template <int D, int STAGES>
 __device__ __forceinline__ bool load_tiles(const PagedArgs &a, const Piece &p, const CUtensorMap &map, Ring &r, uint8_t (*stage)[kTile * D * 2],
                                            uint64_t *full, uint64_t *empty) {
     const adacode_paged_cache &c = a.cache;
     const int lane = threadIdx.x & 31;
     const uint32_t leader = lane == 0;
-    const int tiles = p.n, h = p.h, held = p.len - p.j0 * kTile, at0 = p.j0 * kTile + lane * a.box_rows;
+    const int tiles = p.n, h = p.h, held = p.hi - p.j0 * kTile, at0 = p.j0 * kTile + (lane << a.box_shift);
     const int32_t *table = c.block_table + p.b * c.table_stride;
-    const auto boxes_of = [&](int j) {                        // pages of tile j that hold tokens
+    const auto boxes_of = [&](int j) {                        // behind the last page of tile j that is seen
         const int valid = held - j * kTile;
-        return j >= tiles || valid <= 0 ? 0 : valid >= kTile ? kTile / a.box_rows : (valid + a.box_rows - 1) / a.box_rows;
+        return j >= tiles || valid <= 0 ? 0 : valid >= kTile ? kTile >> a.box_shift : (valid + (1 << a.box_shift) - 1) >> a.box_shift;
     };
     int next_boxes = boxes_of(0), next_page = -1, next_slot = 0;
+    int before = p.lo > p.j0 * kTile ? (p.lo - p.j0 * kTile) >> a.box_shift : 0;      // pages of the first tile that are not
     const auto look_up = [&](int j) {
-        if (lane < next_boxes) {
+        if (lane >= before && lane < next_boxes) {
             const int at = at0 + j * kTile, entry = (int)((uint32_t)at / a.by_page);
             next_slot = at - entry * c.page_size;
             next_page = entry < c.table_width ? table[entry] : -1;
@@ -503,28 +505,27 @@ __device__ __forceinline__ bool load_tiles(const PagedArgs &a, const Piece &p, c
     };
     look_up(0);
     for (int j = 0; j < tiles; ++j) {
-        const int boxes = next_boxes;
+        const int boxes = next_boxes, hidden = before;
         int page = next_page, slot = next_slot;
-        if (lane < boxes && (page < 0 || page >= c.n_pages)) {        // (a page behind the pool reads as zeros)
+        if (lane >= hidden && lane < boxes && (page < 0 || page >= c.n_pages)) {      // (a page behind the pool reads as zeros)
             page = c.n_pages, slot = 0;
-            // (pages of which nothing is seen need not exist: windows leave them behind)
-            const int at = at0 + j * kTile;
-            if (at + a.box_rows > p.lo && at < p.hi) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
+            atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
         }
+        before = 0;
         next_boxes = boxes_of(j + 1);
         look_up(j + 1);
         if (!warp_wait(&empty[r.at], r.phase ^ 1, a.status)) return false;
         const uint32_t bar = smem_u32(&full[r.at]), to = smem_u32(stage[r.at]);
         if (leader) {
-            if (boxes) mbar_arrive_expect_tx(&full[r.at], boxes * a.box_rows * D * 2);
+            if (boxes > hidden) mbar_arrive_expect_tx(&full[r.at], (boxes - hidden) * (D * 2) << a.box_shift);
             else mbar_arrive(&full[r.at]);
         }
         __syncwarp();
         const int i = lane / (D / 64), half = lane % (D / 64);
         const int from = __shfl_sync(kFull, page, i), first = __shfl_sync(kFull, slot, i);
-        if (i < boxes)
+        if (i >= hidden && i < boxes)
             asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-                             to + half * (kTile * 128) + i * a.box_rows * 128),
+                             to + half * (kTile * 128) + (i * 128 << a.box_shift)),
                          "l"(&map), "r"(half * 64), "r"(first), "r"(h), "r"(from), "r"(bar)
                          : "memory");
         r.next();
@@ -552,8 +553,7 @@ __device__ __forceinline__ void load_keys(const PagedArgs &a, Shared<D, SOLO> &s
     int skipped = 0, ctas;
     uint32_t total;
     int left = find_run<S::kRows>(a, blockIdx.x, p, skipped, ctas, total);
-    Cut cut;
-    cut.n = 0;
+    bool is_cut = false;
     while (left > 0) {
         int first;
         seen_by_unit(a, p.row0, p.row0 + p.rows, p.fresh, p.len, p.start, p.lo, p.hi);
@@ -570,16 +570,18 @@ __device__ __forceinline__ void load_keys(const PagedArgs &a, Shared<D, SOLO> &s
         }
         pr.next();
         ok = load_tiles<D, S::kKeys>(a, p, map, r, s.k, s.k_full, s.k_empty);
-        if (beyond_table(a, p) && lane == 0) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
         if (!ok) break;
-        left -= p.n;
+        if (beyond_table(a, p) && lane == 0) atomicOr(a.status, ADACODE_STATUS_BAD_PAGE);
         if (skipped == 0 && !whole) {
             // the unit goes on behind this run: its last tile is all - p.n tiles further on
             const uint32_t end = share_of(total, blockIdx.x + 1, ctas);
             // (no CTA is behind the last, even if lengths change while the kernel runs)
             const int last = (int)(((uint64_t)(end + (all - p.n)) * ctas - 1) / total);
-            cut = {(last < ctas ? last : ctas - 1) - (int)blockIdx.x + 1, p.rows, p.row0, p.b, p.h, p.q0, p.fresh, p.len, p.start};
+            is_cut = true;
+            if (lane == 0)
+                a.cuts[blockIdx.x] = {(last < ctas ? last : ctas - 1) - (int)blockIdx.x + 1, p.rows, p.row0, p.b, p.h, p.q0, p.fresh, p.len, p.start};
         }
+        left -= p.n;
         skipped = 0;
         if (left == 0) break;
         p.row0 += S::kRows;
@@ -595,7 +597,7 @@ __device__ __forceinline__ void load_keys(const PagedArgs &a, Shared<D, SOLO> &s
         }
         p.rows = p.fresh * a.G - p.row0 < S::kRows ? p.fresh * a.G - p.row0 : S::kRows;
     }
-    if (lane == 0) a.cuts[blockIdx.x] = cut;
+    if (lane == 0 && (!is_cut || !ok)) a.cuts[blockIdx.x].n = 0;
     if (ok) ok = warp_wait(&s.piece_empty[pr.at], pr.phase ^ 1, a.status);
     if (ok && lane == 0) {
         s.piece[pr.at].n = 0;
@@ -1145,7 +1147,8 @@ int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int6
     a.query = query, a.out = out, a.q_n = query_token, a.q_h = query_head, a.o_n = out_token, a.o_h = out_head, a.starts = seq_starts;
     a.Hq = Hq, a.G = G, a.causal = causal, a.window = window;
     a.scale = fmaxf(fabsf(scale) * kLog2e, 1.4e-45f), a.negate = scale < 0 ? 0x80008000u : 0u;
-    a.box_rows = one_page || cache->page_size > kTile ? kTile : cache->page_size;
+    const int box_rows = one_page || cache->page_size > kTile ? kTile : cache->page_size;         // (16, 32, 64 or 128)
+    for (a.box_shift = 0; 1 << a.box_shift < box_rows; ++a.box_shift) {}
     const size_t rows = 2 * (size_t)ctas * (solo ? kTile : 2 * kTile);
     a.part_o = (float *)workspace, a.part_ml = a.part_o + rows * D, a.cuts = (Cut *)(a.part_ml + rows * 2);
     const long long room = (long long)cache->table_width * cache->page_size;
@@ -1153,8 +1156,8 @@ int adacode_paged_attn(const adacode_paged_cache *cache, const void *query, int6
     a.by_page = quotient_by(cache->page_size), a.by_group = quotient_by(G);
     a.status = status;
     CUtensorMap keys, values;
-    if (!map_pages(keys, cache->key_pages, *cache, cache->key_page, cache->key_head, cache->key_slot, a.box_rows) ||
-        !map_pages(values, cache->value_pages, *cache, cache->value_page, cache->value_head, cache->value_slot, a.box_rows))
+    if (!map_pages(keys, cache->key_pages, *cache, cache->key_page, cache->key_head, cache->key_slot, box_rows) ||
+        !map_pages(values, cache->value_pages, *cache, cache->value_page, cache->value_head, cache->value_slot, box_rows))
         return ADACODE_ERR_INVALID_ARG;
     const cudaStream_t st = (cudaStream_t)stream;
     const int rc = cache->dtype == ADACODE_BF16 ? launch_paged<__nv_bfloat16>(a, solo, keys, values, ctas, max_query_len, st)
