@@ -102,13 +102,15 @@ def _behind_prefill(cache, module, query: torch.Tensor) -> bool:
 def _left_padding(cache, layer_idx: int, mask: torch.Tensor, batch: int, total: int, window: int) -> Optional[torch.Tensor]:
     """First visible position of every sequence (int32 [B]) of a mask that is causal, with the layer's sliding window, behind left padding;
     None where nothing is padded.  All layers of a kind get the same mask object in a forward pass, so the (synchronising) check runs
-    once per pass and kind; a layer that is not behind the last one asked for begins another pass."""
+    once per pass and kind, and again where the mask has been written to since (which a tensor of inference mode does not tell: there, for
+    every layer); a layer that is not behind the last one asked for begins another pass."""
     seen_layer, known = getattr(cache, '_fused_masks_known', (-1, ()))
     known = [k for k in known if layer_idx > seen_layer]
     cache._fused_masks_known = layer_idx, known
+    as_now = None if mask.is_inference() else (mask._version, window, total)
     for k in known:
-        if k[0] is mask and k[1:3] == (window, total):
-            return k[3]
+        if as_now is not None and k[0] is mask and k[1] == as_now:
+            return k[2]
     visible = mask if mask.dtype == torch.bool else mask == 0
     T = visible.shape[2]
     if visible.shape[3] != total:
@@ -120,10 +122,12 @@ def _left_padding(cache, layer_idx: int, mask: torch.Tensor, batch: int, total: 
     causal = (j >= starts[:, None, None]) & (j <= at)
     if window:
         causal &= j > at - window
-    if not bool((visible == causal[:, None]).all()):
+    is_causal, padded = torch.stack([(visible == causal[:, None]).all(), (starts > 0).any()]).tolist()
+    if not is_causal:
         raise NotImplementedError('float11_fused attention takes masks that are causal behind left padding; use the materialising path')
-    out = starts.to(torch.int32).expand(batch).contiguous() if bool((starts > 0).any()) else None
-    known.append((mask, window, total, out))
+    out = starts.to(torch.int32).expand(batch).contiguous() if padded else None
+    if as_now is not None:
+        known.append((mask, as_now, out))
     return out
 
 

@@ -142,3 +142,21 @@ def test_keys_of_another_cache_are_refused(monkeypatch):
     key = x[:, :, :5].repeat(1, 2, 1, 1)
     out, _ = hf_attention.float11_fused_attention(SimpleNamespace(layer_idx=0), key, key, key, None)
     assert out.shape == (B, 5, HQ, D) and not asked
+
+
+@pytest.mark.parametrize('inference', [False, True])
+def test_masks_that_change_between_layers(monkeypatch, inference):
+    """One tensor, written anew between two layers of a pass: each layer has what it holds then; unchanged, it is looked at once."""
+    cache = SimpleNamespace(layers=[Layer() for _ in range(3)], _fused_decode=True, _fused_chunks=True)
+    monkeypatch.setattr(hf_attention, '_active_cache', cache)
+    x = torch.zeros(B, HQ, T, D, dtype=torch.bfloat16)
+    with torch.inference_mode(inference):
+        mask = causal(T, starts=(0, 9)).clone()
+        for i in (0, 1):
+            hf_attention.float11_fused_attention(SimpleNamespace(layer_idx=i), x, x, x, mask)
+        mask.copy_(causal(T, starts=(5, 0)))
+        hf_attention.float11_fused_attention(SimpleNamespace(layer_idx=2), x, x, x, mask)
+        assert [layer.asked for layer in cache.layers] == [[('chunk', [0, 9], 0)], [('chunk', [0, 9], 0)], [('chunk', [5, 0], 0)]]
+        mask.zero_()
+        with pytest.raises(NotImplementedError, match='mask'):
+            hf_attention.float11_fused_attention(SimpleNamespace(layer_idx=2), x, x, x, mask)
