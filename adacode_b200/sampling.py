@@ -15,6 +15,7 @@ import torch
 
 from . import _lib
 from .codec import _scratch_for
+from .paged import refuse_autograd
 from .rows import on_device, stream_ptr, written
 
 _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.FP32}
@@ -63,6 +64,7 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Set
         out = torch.empty(B, dtype=torch.int64, device=dev)
     elif out.dtype != torch.int64 or out.shape != (B,) or not out.is_contiguous() or out.device != dev:
         raise ValueError(f'out must be contiguous int64 [{B}] on {dev}')
+    refuse_autograd('sample_tokens', (), (out,))
     if logits.stride(1) != 1 and V > 1:
         logits = logits.contiguous()
     uniforms = uniforms.contiguous()

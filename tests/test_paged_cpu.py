@@ -175,3 +175,14 @@ def test_outputs_that_overlap_themselves_are_refused():
     from adacode_b200 import _lib
     with pytest.raises(_lib.AdacodeError, match='CUDA'):
         paged_attention(one, k[:, :1], v[:, :1], table[:1], lens[:1], out=torch.zeros(64, dtype=BF).as_strided((1, 1, 64), (0, 0, 1)))
+
+
+def test_sampling_writes_to_inference_tensors_in_inference_mode_only():
+    from adacode_b200 import _lib
+    x, u = torch.zeros(3, 10), torch.zeros(3)
+    with torch.inference_mode():
+        out = torch.zeros(3, dtype=torch.int64)
+        with pytest.raises(_lib.AdacodeError, match='CUDA'):
+            sample_tokens(x, u, out=out)
+    with pytest.raises(RuntimeError, match='inference'):
+        sample_tokens(x, u, out=out)
