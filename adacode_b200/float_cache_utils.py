@@ -1220,8 +1220,8 @@ class Float11Cache(Cache):
 
     def update_rotary(self, query: torch.Tensor, key_states: torch.Tensor, value_states: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                       layer_idx: int, cache_kwargs: Optional[dict] = None, sections=None, interleaved: bool = False) -> tuple:
-        """``update`` for queries and keys that have not been rotated yet: both are, and keys and values written to the cache, in one
-        launch (``append_rotary``).  ``cos`` and ``sin`` are a HF model's position embeddings ``[B or 1, T, R]``, with ``sections`` ``[axes, B or 1,
+        """``update`` for queries and keys that have not been rotated yet: both are, and keys and values written to the cache, by one launch of
+        ``append_rotary`` (two small ones before it make its table and lengths, and angles of several sequences are copied).  ``cos`` and ``sin`` are a HF model's position embeddings ``[B or 1, T, R]``, with ``sections`` ``[axes, B or 1,
         T, R]``.  Returns the rotated queries and what ``update`` returns (where ``update`` returns the keys as they came, because a fused
         attention is to read the cache, they have not been rotated).  Queries of other types than bf16 are rounded to it first, as ``update`` does with
         keys and values, and come back in their own."""
